@@ -416,6 +416,71 @@ int32_t mmh_swiglu_backward(mmh_handle ctx, const float *x, const float *wg, con
 int32_t mmh_embedding_backward(mmh_handle ctx, const int32_t *ids_host, int64_t n,
                                const float *dy, int64_t vocab, int64_t d, float *dtable);
 
+/* ---- The linear layer's training operators ---------------------------------
+ * No counterpart in the reference, whose Linear is the bare matmul and whose
+ * loss takes stored logits. f32, contiguous row-major arrays at any 4-byte
+ * alignment; weights [k, n] (form MMH_GEMM_NN) or [n, k] (MMH_GEMM_NT, a tied
+ * embedding's layout). Sums are f32, the products' as mmh_gemm_* forms them. An
+ * output that overlaps another buffer of the call is MMH_ERR_ARGUMENT, except
+ * where it may be the very same buffer, as stated.
+ *
+ * Dropout draws from Philox4x32-10: block j of the key `seed` is the counter
+ * (offset + j, 0), value i of the array takes word i % 4 of block i / 4 and is
+ * dropped (0, whatever it was) when that word is below floor(p * 2^32);
+ * otherwise it is times 1 / (1 - p). The mask is a function of (i, p, seed,
+ * offset) alone and is stored nowhere: the backward call with the same p, seed
+ * and offset has the same mask. A call on n values uses ceil(n / 4) blocks, so
+ * a caller that draws several masks under one seed moves offset on by as much
+ * (it wraps at 2^64). p in [0, 1]; 0 keeps every value as it is, 1 drops all. */
+
+#define MMH_ACT_NONE 0
+#define MMH_ACT_RELU 1
+#define MMH_ACT_GELU 2      /* x * Phi(x), through erf */
+#define MMH_ACT_GELU_TANH 3 /* its tanh approximation */
+#define MMH_ACT_SILU 4
+
+/* out = residual + dropout(x), n values; residual may be NULL (nothing is
+ * added). out may be x or residual. */
+int32_t mmh_dropout(mmh_handle ctx, const float *x, const float *residual, int64_t n, float p,
+                    uint64_t seed, uint64_t offset, float *out);
+/* dx = dropout(dout) with the mask of the forward call (d residual is dout
+ * itself). dx may be dout. */
+int32_t mmh_dropout_backward(mmh_handle ctx, const float *dout, int64_t n, float p, uint64_t seed,
+                             uint64_t offset, float *dx);
+/* pre = x op(w) + bias, out = residual + dropout(act(pre)): x [rows, k], out
+ * [rows, n], dropout over out's values in row-major order (the mask that
+ * mmh_dropout draws for an array of rows * n). bias [n], residual [rows, n] and
+ * pre [rows, n] may be NULL; pre, when given, receives the values that the
+ * backward of an activation needs. out may be residual. */
+int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w, const float *bias,
+                   const float *residual, int64_t rows, int64_t k, int64_t n, int32_t activation,
+                   float p, uint64_t seed, uint64_t offset, float *pre, float *out);
+/* Its backward for dout [rows, n]: dpre = dropout(dout) * act'(pre), dx = dpre
+ * op(w)^T, dw = x^T dpre in w's layout, dbias the column sums of dpre (d residual
+ * is dout itself). pre as the forward call left it; NULL for MMH_ACT_NONE. Any
+ * of dx, dw, dbias may be NULL (not needed), and then w (for dx), x (for dw) too.
+ * Outputs are overwritten. The derivative of relu at 0 is 0. */
+int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const float *w,
+                            const float *pre, const float *dout, int64_t rows, int64_t k, int64_t n,
+                            int32_t activation, float p, uint64_t seed, uint64_t offset, float *dx,
+                            float *dw, float *dbias);
+/* The cross entropy (as mmh_cross_entropy has it) of the logits x op(w): x [n,
+ * d], w [d, vocab] or [vocab, d], targets on the host. The logits are never
+ * whole in memory: the call's workspace holds a block of rows, 256 MiB (128 rows
+ * where those are more). Rows whose target is `ignore` (any value, -1 say) are
+ * left out: the mean is over the others, and nothing the row holds is read. With
+ * no row left the loss is 0. Other targets outside [0, vocab) are
+ * MMH_ERR_INDEX. */
+int32_t mmh_linear_cross_entropy(mmh_handle ctx, int32_t form, const float *x, const float *w,
+                                 const int32_t *targets_host, int64_t n, int64_t d, int64_t vocab,
+                                 int32_t ignore, float *loss_host);
+/* The same with its gradients dx [n, d] (zeros in ignored rows) and dw (w's
+ * layout) for loss gradient 1, overwritten; each, and loss_host, may be NULL. */
+int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const float *x,
+                                          const float *w, const int32_t *targets_host, int64_t n,
+                                          int64_t d, int64_t vocab, int32_t ignore, float *dx,
+                                          float *dw, float *loss_host);
+
 /* ---- Checkpoints: midman-checkpoint (safetensors.rs, params.rs) -----------
  * TensorFile (safetensors.rs:68-330): named F32 tensors + string metadata,
  * read with the reference's validation (8-byte length, <= 100 MB header of

@@ -921,9 +921,11 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
                     e = p.libm_exp ? expf(x0 - mx) + expf(x1 - mx)
                                    : __builtin_amdgcn_exp2f((x0 - mx) * kLog2e) +
                                          __builtin_amdgcn_exp2f((x1 - mx) * kLog2e);
+                else if (x0 != x0 || x1 != x1)
+                    e = __builtin_nanf("");  // (the maximum passes over a NaN)
                 e = half_sum32(e);
                 if (lr == 0) {
-                    ce_m[wn][rl] = mx;
+                    ce_m[wn][rl] = e != e ? e : mx;
                     ce_s[wn][rl] = e;
                 }
                 const int t = ce_t[rl];

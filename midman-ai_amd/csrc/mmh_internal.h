@@ -206,6 +206,10 @@ void launch_cross_entropy(Context &ctx, const float *logits, const int32_t *targ
 // f64 mean as launch_cross_entropy.
 void launch_ce_combine(Context &ctx, const float *part, int64_t tiles, const float *zt,
                        int64_t n, float *row_loss, float *loss_dev);
+// The row terms alone, and their f64 mean (out: device or pinned memory).
+void launch_ce_combine_rows(Context &ctx, const float *part, int64_t tiles, const float *zt,
+                            int64_t n, float *row_loss);
+void launch_mean(Context &ctx, const float *row_loss, int64_t n, float *out);
 void launch_pack_cols(Context &ctx, const float *src, int64_t rows, int64_t cols, float *dst,
                       int64_t ld_dst, int64_t col_off);
 void launch_pack_gate_up(Context &ctx, const float *wg, const float *wu, int64_t rows,

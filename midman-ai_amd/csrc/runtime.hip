@@ -10,6 +10,7 @@
 
 #include <cstdlib>
 
+#include "mmh_args.h"
 #include "mmh_internal.h"
 
 namespace mmh {
@@ -77,17 +78,6 @@ void check_ids(const int32_t *ids, int64_t n, int64_t vocab, const char *what) {
 }  // namespace mmh
 
 using namespace mmh;
-
-namespace {
-
-void need(const void *p, const char *what) {
-    if (!p) fail(MMH_ERR_ARGUMENT, std::string(what) + " is a null pointer");
-}
-void positive(int64_t v, const char *what) {
-    if (v <= 0) fail(MMH_ERR_SHAPE, std::string(what) + " must be at least 1, got " + std::to_string(v));
-}
-
-}  // namespace
 
 extern "C" {
 

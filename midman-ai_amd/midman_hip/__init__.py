@@ -135,6 +135,16 @@ _SIGNATURES = {
     "mmh_cross_entropy_backward": [_h, _vp, _i32p, _i64, _i64, _vp, _f32p],
     "mmh_swiglu_backward": [_h] + [_vp] * 5 + [_i64] * 3 + [_vp] * 4,
     "mmh_embedding_backward": [_h, _i32p, _i64, _vp, _i64, _i64, _vp],
+    "mmh_dropout": [_h, _vp, _vp, _i64, ctypes.c_float, ctypes.c_uint64, ctypes.c_uint64, _vp],
+    "mmh_dropout_backward": [_h, _vp, _i64, ctypes.c_float, ctypes.c_uint64, ctypes.c_uint64, _vp],
+    "mmh_linear": [_h, _i32] + [_vp] * 4 + [_i64] * 3 + [_i32, ctypes.c_float, ctypes.c_uint64,
+                                                         ctypes.c_uint64, _vp, _vp],
+    "mmh_linear_backward": [_h, _i32] + [_vp] * 4 + [_i64] * 3 + [_i32, ctypes.c_float,
+                                                                  ctypes.c_uint64, ctypes.c_uint64,
+                                                                  _vp, _vp, _vp],
+    "mmh_linear_cross_entropy": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 3 + [_i32, _f32p],
+    "mmh_linear_cross_entropy_backward": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 3 + [_i32, _vp, _vp,
+                                                                                     _f32p],
     "mmh_tensorfile_create": [ctypes.POINTER(_h)],
     "mmh_tensorfile_parse": [ctypes.c_char_p, ctypes.c_uint64, ctypes.POINTER(_h)],
     "mmh_tensorfile_push": [_h, ctypes.c_char_p, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64),
@@ -604,6 +614,127 @@ def embedding_backward(ctx: Context, ids: np.ndarray, dy: DeviceArray, vocab: in
     out = ctx.empty((vocab, d))
     check(lib().mmh_embedding_backward(ctx.handle, _ip(ids), ids.size, dy.ptr, vocab, d, out.ptr))
     return out
+
+
+# ---- the linear layer's training operators ---------------------------------------------
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_FORMS = {"nn": 0, "nt": 1}
+
+
+def _dropout_args(p, seed, offset):
+    if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
+        raise ArgumentError(ERR_ARGUMENT, "dropout: seed and offset are unsigned 64-bit numbers")
+    return p, seed, offset
+
+
+def _linear_args(x, w, form, activation):
+    """(form, activation, rows, k, n) of x [.., k] and w [k, n] (nn) or [n, k] (nt)."""
+    if form not in _FORMS or activation not in ACTIVATIONS:
+        raise ArgumentError(ERR_ARGUMENT, f"linear: unknown form {form!r} or activation {activation!r}")
+    k = x.shape[-1]
+    if len(w.shape) != 2 or w.shape[_FORMS[form]] != k:
+        raise ShapeError(ERR_SHAPE, f"linear: x {x.shape} does not fit w {w.shape} in form {form}")
+    return _FORMS[form], ACTIVATIONS[activation], x.size // k, k, w.shape[1 - _FORMS[form]]
+
+
+def _fits(what, a, shape):
+    if a is not None and a.shape != tuple(shape):
+        raise ShapeError(ERR_SHAPE, f"{what} must have shape {tuple(shape)}, got {a.shape}")
+
+
+def dropout(ctx: Context, x: DeviceArray, p: float, seed: int, offset: int = 0,
+            residual: DeviceArray = None, out: DeviceArray = None):
+    """residual + dropout(x) with the mask of (seed, offset); the mask takes
+    ceil(x.size / 4) counters from offset on. out may be x or residual."""
+    _fits("dropout: residual", residual, x.shape)
+    _fits("dropout: out", out, x.shape)
+    args = _dropout_args(p, seed, offset)
+    out = out or ctx.empty(x.shape)
+    check(lib().mmh_dropout(ctx.handle, x.ptr, _ptr(residual), x.size, *args, out.ptr))
+    return out
+
+
+def dropout_backward(ctx: Context, dout: DeviceArray, p: float, seed: int, offset: int = 0,
+                     out: DeviceArray = None):
+    """dx of dropout: the forward's mask again, from the same (p, seed, offset)."""
+    _fits("dropout_backward: out", out, dout.shape)
+    args = _dropout_args(p, seed, offset)
+    out = out or ctx.empty(dout.shape)
+    check(lib().mmh_dropout_backward(ctx.handle, dout.ptr, dout.size, *args, out.ptr))
+    return out
+
+
+def linear(ctx: Context, x: DeviceArray, w: DeviceArray, bias: DeviceArray = None,
+           residual: DeviceArray = None, form: str = "nn", activation: str = "none",
+           p: float = 0.0, seed: int = 0, offset: int = 0, pre: DeviceArray = None,
+           out: DeviceArray = None):
+    """residual + dropout(act(x op(w) + bias)): x [.., k], w [k, n] (nn) or
+    [n, k] (nt). pre (x's leading axes and n), when given, receives
+    x op(w) + bias for linear_backward. out may be residual."""
+    f, act, rows, k, n = _linear_args(x, w, form, activation)
+    shape = x.shape[:-1] + (n,)
+    _fits("linear: bias", bias, (n,))
+    for what, a in (("residual", residual), ("pre", pre), ("out", out)):
+        _fits("linear: " + what, a, shape)
+    args = _dropout_args(p, seed, offset)
+    out = out or ctx.empty(shape)
+    check(lib().mmh_linear(ctx.handle, f, x.ptr, w.ptr, _ptr(bias), _ptr(residual), rows, k, n, act,
+                           *args, _ptr(pre), out.ptr))
+    return out
+
+
+def linear_backward(ctx: Context, x: DeviceArray, w: DeviceArray, dout: DeviceArray,
+                    pre: DeviceArray = None, form: str = "nn", activation: str = "none",
+                    p: float = 0.0, seed: int = 0, offset: int = 0, dx: DeviceArray = None,
+                    dw: DeviceArray = None, dbias: DeviceArray = None):
+    """linear's gradients (dx, dw, dbias) for dout; pre as linear left it (not
+    needed without an activation)."""
+    f, act, rows, k, n = _linear_args(x, w, form, activation)
+    shape = x.shape[:-1] + (n,)
+    for what, a, s in (("dout", dout, shape), ("pre", pre, shape), ("dx", dx, x.shape),
+                       ("dw", dw, w.shape), ("dbias", dbias, (n,))):
+        _fits("linear_backward: " + what, a, s)
+    args = _dropout_args(p, seed, offset)
+    dx, dw, dbias = dx or ctx.empty(x.shape), dw or ctx.empty(w.shape), dbias or ctx.empty((n,))
+    check(lib().mmh_linear_backward(ctx.handle, f, x.ptr, w.ptr, _ptr(pre), dout.ptr, rows, k, n, act,
+                                    *args, dx.ptr, dw.ptr, dbias.ptr))
+    return dx, dw, dbias
+
+
+def _head_args(x, w, targets, form):
+    f, _, n, d, vocab = _linear_args(x, w, form, "none")
+    targets = np.ascontiguousarray(targets, dtype=np.int32)
+    if targets.size != n:
+        raise ShapeError(ERR_SHAPE, f"linear_cross_entropy: {n} rows but {targets.size} targets")
+    return f, targets, n, d, vocab
+
+
+def linear_cross_entropy(ctx: Context, x: DeviceArray, w: DeviceArray, targets: np.ndarray,
+                         form: str = "nt", ignore: int = -1) -> float:
+    """cross_entropy of the logits x op(w), which are never whole in memory:
+    x [.., d], w [vocab, d] (nt, a tied embedding) or [d, vocab] (nn). Rows whose
+    target is `ignore` are left out of the mean."""
+    f, targets, n, d, vocab = _head_args(x, w, targets, form)
+    loss = ctypes.c_float()
+    check(lib().mmh_linear_cross_entropy(ctx.handle, f, x.ptr, w.ptr, _ip(targets), n, d, vocab,
+                                         ignore, ctypes.byref(loss)))
+    return loss.value
+
+
+def linear_cross_entropy_backward(ctx: Context, x: DeviceArray, w: DeviceArray, targets: np.ndarray,
+                                  form: str = "nt", ignore: int = -1, dx: DeviceArray = None,
+                                  dw: DeviceArray = None):
+    """(loss, dx, dw) of linear_cross_entropy for loss gradient 1."""
+    f, targets, n, d, vocab = _head_args(x, w, targets, form)
+    _fits("linear_cross_entropy_backward: dx", dx, x.shape)
+    _fits("linear_cross_entropy_backward: dw", dw, w.shape)
+    dx, dw = dx or ctx.empty(x.shape), dw or ctx.empty(w.shape)
+    loss = ctypes.c_float()
+    check(lib().mmh_linear_cross_entropy_backward(ctx.handle, f, x.ptr, w.ptr, _ip(targets), n, d,
+                                                  vocab, ignore, dx.ptr, dw.ptr,
+                                                  ctypes.byref(loss)))
+    return loss.value, dx, dw
 
 
 # ---- checkpoints: midman-checkpoint ----------------------------------------------------
