@@ -179,6 +179,39 @@ __device__ __forceinline__ void split_reduce_tile(const KParams &p, int64_t m0, 
     }
 }
 
+// The same for EPI_LINEAR: the sums in split order, then the layer's epilogue.
+__device__ __forceinline__ void split_linear_tile(const KParams &p, int64_t m0, int64_t n0, int tr,
+                                                  int tc, int nthreads) {
+    const int64_t M = p.m, N = p.n, total = M * N;
+#pragma unroll 1
+    for (int e = 4 * (int)threadIdx.x; e < tr * tc; e += 4 * nthreads) {
+        const int64_t row = m0 + e / tc, col = n0 + e % tc;
+        if (row >= M || col >= N) continue;
+        const int count = (int)min(N - col, (int64_t)4);
+        const float *Q = p.partial + row * N + col;
+        TailInputs in;
+        tail_load(p.tail, N, row, col, count, in);
+        float v[4] = {};
+        for (int s0 = 0; s0 < p.splits; s0 += 4) {
+            float u[4][4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s0 + s < p.splits) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        u[s][j] = j < count ? split_get(Q + (int64_t)(s0 + s) * total + j) : 0.0f;
+                }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s0 + s < p.splits) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = s0 + s == 0 ? u[s][j] : __fadd_rn(v[j], u[s][j]);
+                }
+        }
+        tail_finish(p.tail, N, row, col, count, in, v);
+    }
+}
+
 // ---- small-tile GEMM ---------------------------------------------------------
 // For shapes with fewer 128x128 tiles than CUs (the tiny preset's projections,
 // M = 2048 with N and K of a few hundred) the big tile leaves most of the chip
@@ -505,7 +538,35 @@ __global__ __launch_bounds__(256) void gemm_f32_mfma_small(KParams p) {
             const int64_t row = row_of(r);
             if (row < M && col < N) split_put(P + row * N + col, acc[r]);
         }
-        if (split_last(p, tm * p.tiles_n + tn)) split_reduce_tile(p, m0, n0, SBM, SBN, 256);
+        if (split_last(p, tm * p.tiles_n + tn)) {
+            if constexpr (EPI == EPI_LINEAR) split_linear_tile(p, m0, n0, SBM, SBN, 256);
+            else split_reduce_tile(p, m0, n0, SBM, SBN, 256);
+        }
+        return;
+    }
+    if constexpr (EPI == EPI_LINEAR) {
+        // through LDS (free behind the K loop's last barrier): a thread has four
+        // neighbouring columns of a row
+        constexpr int LD = SBN + 4;
+        static_assert(SBM * LD <= 2 * SBM * SKS, "the tile fits A's stages");
+        float *tile = &As[0][0][0];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            tile[(wm * 32 + 8 * (r >> 2) + 4 * lk + (r & 3)) * LD + wn * 32 + lr] = acc[r];
+        __syncthreads();
+#pragma unroll 1
+        for (int e = tid; e < SBM * SBN / 4; e += 256) {
+            const int rl = e / (SBN / 4), c = e % (SBN / 4) * 4;
+            const int64_t row = m0 + rl, cc = n0 + c;
+            if (row >= M || cc >= N) continue;
+            const int count = (int)min(N - cc, (int64_t)4);
+            TailInputs in;
+            tail_load(p.tail, N, row, cc, count, in);
+            float v[4];
+            __builtin_memcpy(v, __builtin_assume_aligned(tile + rl * LD + c, 16), 16);
+            tail_finish(p.tail, N, row, cc, count, in, v);
+        }
         return;
     }
     float *C = p.c + batch * p.stride_c;
@@ -661,6 +722,18 @@ __global__ __launch_bounds__(64 * NW) void gemm_f32_mfma_ksplit(KParams p) {
         }
     }
 
+    // EPI_LINEAR: thread t < 256 finishes columns 4 (t % 8) .. + 3 of row t / 8;
+    // the bias and the residual are read ahead like the others'.
+    TailInputs lin;
+    int lin_count = 0;
+    if constexpr (EPI == EPI_LINEAR) {
+        const int64_t row = m0 + (tid >> 3), cc = n0 + (tid & 7) * 4;
+        if (fin && tid < 256 && row < M && cc < N) {
+            lin_count = (int)min(N - cc, (int64_t)4);
+            tail_load(p.tail, N, row, cc, lin_count, lin);
+        }
+    }
+
     // Each step sums from acc_init; a wave with more steps than one adds them
     // up in its own LDS slots: 16 roundings at a step's size and one at the
     // sum's, so few splits of a long K are no less precise than many (error
@@ -769,6 +842,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_f32_mfma_ksplit(KParams p) {
         if (NORM) v = __fmul_rn(v, sm_inv[rl]);
         if (!fin) {
             if (row < M && col < N) split_put(p.partial + ((int64_t)split * M + row) * N + col, v);
+        } else if (EPI == EPI_LINEAR) {
+            part[0][r][lane] = v;  // (only this thread reads the slots of its registers)
         } else if (EPI == EPI_ACCUM) {
             if (row < M && col < N) C[row * p.ldc + col] = __fadd_rn(pre_r[i], v);
         } else if (EPI == EPI_STORE && p.rope_cos) {
@@ -784,6 +859,20 @@ __global__ __launch_bounds__(64 * NW) void gemm_f32_mfma_ksplit(KParams p) {
         } else {
             block32_epilogue<EPI>(p, C, R, row, col, lr, v);
         }
+    }
+    if constexpr (EPI == EPI_LINEAR) {
+        if (fin) {
+            __syncthreads();
+            if (tid < 256 && lin_count > 0) {
+                const int rl = tid >> 3;  // row 8*(r/4) + 4*h + r%4 is register r of lane half h
+                float v[4];
+                __builtin_memcpy(v, &part[0][rl >> 3 << 2 | (rl & 3)][(rl >> 2 & 1) * 32 + (tid & 7) * 4], 16);
+                tail_finish(p.tail, N, m0 + rl, n0 + (tid & 7) * 4, lin_count, lin, v);
+            }
+            return;
+        }
+        if (split_last(p, tm * p.tiles_n + tn)) split_linear_tile(p, m0, n0, 32, 32, 64 * NW);
+        return;
     }
     if (fin) return;
     if (split_last(p, tm * p.tiles_n + tn)) split_reduce_tile(p, m0, n0, 32, 32, 64 * NW);
@@ -929,7 +1018,7 @@ bool use_small(const Context &ctx, const GemmDesc &d) {
 // other kernels' operand reuse through LDS pays; 0 otherwise.
 int ksplit_kind(const Context &ctx, const GemmDesc &d) {
     const int cus = cus_of(ctx);
-    const bool plain = d.epi == EPI_STORE || d.epi == EPI_ACCUM;
+    const bool plain = d.epi == EPI_STORE || d.epi == EPI_ACCUM || d.epi == EPI_LINEAR;
     const int64_t small_tiles = ((d.m + SBM - 1) / SBM) * ((d.n + SBN - 1) / SBN);
     const int64_t big_tiles = ((d.m + BM - 1) / BM) * ((d.n + BN - 1) / BN);
     if (use_small(ctx, d) && !d.ta && !d.tb && d.batch == 1 && d.k <= 480 &&
@@ -1049,7 +1138,8 @@ constexpr int kMaxTileSplits = 16;
 // choice is 0.9% from the best tile of each, 2.9% with 6 for all. (even: 6 for all.)
 TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int epi, int first,
                       bool even) {
-    const bool may_split = batch == 1 && (epi == EPI_STORE || epi == EPI_ACCUM) && !p.rope_cos;
+    const bool may_split = batch == 1 && (epi == EPI_STORE || epi == EPI_ACCUM || epi == EPI_LINEAR) &&
+                           !p.rope_cos;
     const double cus = cus_of(ctx), ksteps = (double)((p.k + BK - 1) / BK);
     TilePlan best[2];  // of the halvings of K, of the other split counts
     double best_us[2] = {0.0, 0.0};
@@ -1175,6 +1265,11 @@ void gemm(Context &ctx, const GemmDesc &d) {
     if (d.accumulate_into_c && (d.epi != EPI_ACCUM || d.resid))
         fail(MMH_ERR_ARGUMENT, "gemm: accumulate_into_c takes EPI_ACCUM into C itself");
     p.acc_init = d.accumulate_into_c ? -0.0f : 0.0f;
+    if (d.epi == EPI_LINEAR) {
+        if (!d.tail || !d.tail->out || d.ta || d.batch != 1 || d.norm_w || d.rope_cos)
+            fail(MMH_ERR_ARGUMENT, "gemm: the linear epilogue takes one plain nn or nt product");
+        p.tail = *d.tail;
+    }
     if (d.epi == EPI_SWIGLU_BWD || (d.epi == EPI_SWIGLU && d.aux)) {
         if (!d.aux || d.ldaux < (d.epi == EPI_SWIGLU ? d.n : 2 * d.n) || d.ldaux % 4 ||
             !aligned16(d.aux) ||
@@ -1289,7 +1384,8 @@ void gemm(Context &ctx, const GemmDesc &d) {
         }
     }
 
-    const int epi = splits > 1 ? EPI_STORE : d.epi;
+    // (the small tiles' splits finish EPI_LINEAR in the launch)
+    const int epi = splits > 1 && !(d.epi == EPI_LINEAR && !tiled) ? EPI_STORE : d.epi;
     if (tiles > 0x7fffffff || d.batch > 65535) fail(MMH_ERR_SHAPE, "gemm: grid too large");
     dim3 grid((unsigned)tiles, (unsigned)d.batch, (unsigned)splits);
     if (ksplit) {
@@ -1301,6 +1397,9 @@ void gemm(Context &ctx, const GemmDesc &d) {
         const int mode = !vec ? 0 : d.k % 32 == 0 ? 2 : 1;
         if (epi == EPI_SWIGLU)
             launch_ksplit<false, false, EPI_SWIGLU>(ctx, p, grid, mode);
+        else if (epi == EPI_LINEAR)
+            (d.tb ? launch_ksplit<false, true, EPI_LINEAR>
+                  : launch_ksplit<false, false, EPI_LINEAR>)(ctx, p, grid, mode);
         else if (!d.ta && !d.tb)
             (epi == EPI_ACCUM ? launch_ksplit<false, false, EPI_ACCUM>
                               : launch_ksplit<false, false, EPI_STORE>)(ctx, p, grid, mode);
@@ -1312,6 +1411,9 @@ void gemm(Context &ctx, const GemmDesc &d) {
                               : launch_ksplit<true, false, EPI_STORE>)(ctx, p, grid, mode);
     } else if (tiled) {
         launch_gemm_tiles(ctx, p, grid, d.ta, d.tb, epi, plan.tile);
+    } else if (epi == EPI_LINEAR) {
+        if (d.tb) launch<false, true, EPI_LINEAR>(ctx, p, grid);
+        else launch<false, false, EPI_LINEAR>(ctx, p, grid);
     } else if (epi == EPI_SWIGLU) {
         if (d.ta || d.tb) fail(MMH_ERR_ARGUMENT, "gemm: swiglu epilogue needs the nn form");
         launch<false, false, EPI_SWIGLU>(ctx, p, grid);

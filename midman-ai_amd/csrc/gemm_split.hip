@@ -887,7 +887,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
         }
     }
     redo = __syncthreads_or(redo);
-    if (EPI != EPI_CE && !first) return;
+    if (EPI != EPI_CE && EPI != EPI_LINEAR && !first) return;
     if (first && redo) exact_mainloop<TA, TB, CL, WM, WN, MB>(p, A, B, m0, n0, kbeg, kend, acc);
 
     // ---- epilogue: block (i, j) register r of lane l is C[row][col] with
@@ -941,6 +941,45 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
             lse_merge(m, sum, ce_m[2 * u + 1][rl], ce_s[2 * u + 1][rl]);
             reinterpret_cast<float2 *>(p.ce_part)[(m0 + rl) * p.ce_tiles + unit] =
                 make_float2(m, sum);
+        }
+        return;
+    }
+    if constexpr (EPI == EPI_LINEAR) {
+        // 32 rows of each wave at a time through LDS (free behind the barrier
+        // above), so that a thread has four neighbouring columns of a row: one
+        // generator block, and 16-byte accesses to the residual and the
+        // outputs. The loop stays rolled: unrolled, its four copies of the
+        // activations would not fit the instruction cache.
+        constexpr int ROWS = WM * 32, LD = TN + 4, THREADS = NT * WK;
+        static_assert(ROWS * LD * 4 <= WK * 2 * S::STAGE, "a block row fits the stages");
+        static_assert(ROWS * TN % (4 * THREADS) == 0, "whole rounds of units");
+        float *tile = reinterpret_cast<float *>(lds);
+#pragma unroll 1
+        for (int i = 0; i < MB; ++i) {
+            if (first) {
+                unroll_seq([&](auto ic) __attribute__((always_inline)) {
+                    if (ic != i) return;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        *reinterpret_cast<float2 *>(tile + (wm * 32 + 8 * (r >> 2) + 4 * lk + (r & 3)) * LD +
+                                                    wn * 64 + 2 * lr) =
+                            make_float2(acc[ic][0][r], acc[ic][1][r]);
+                }, std::make_integer_sequence<int, MB>{});
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int e = tid; e < ROWS * TN / 4; e += THREADS) {
+                const int rl = e / (TN / 4), c = e % (TN / 4) * 4;
+                const int64_t row = m0 + (rl / 32 * MB + i) * 32 + rl % 32, cc = n0 + c;
+                if (row >= M || cc >= N) continue;
+                const int count = (int)min(N - cc, (int64_t)4);
+                TailInputs in;
+                tail_load(p.tail, N, row, cc, count, in);
+                float v[4];
+                __builtin_memcpy(v, __builtin_assume_aligned(tile + rl * LD + c, 16), 16);
+                tail_finish(p.tail, N, row, cc, count, in, v);
+            }
+            __syncthreads();
         }
         return;
     }
@@ -1006,6 +1045,36 @@ __global__ __launch_bounds__(256) void splitk_reduce(const float *__restrict__ p
     }
 }
 
+// The same for EPI_LINEAR: the sums in split order, then the layer's epilogue,
+// four columns of a row per thread.
+__global__ __launch_bounds__(256) void splitk_linear(const float *__restrict__ partial, LinearTail tail,
+                                                     int64_t m, int64_t n, int splits) {
+    const int64_t units = (n + 3) / 4, total = m * n;
+    for (int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; q < m * units;
+         q += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = q / units, col = (q - row * units) * 4;
+        const int count = (int)min(n - col, (int64_t)4);
+        const float *src = partial + row * n + col;
+        TailInputs in;
+        tail_load(tail, n, row, col, count, in);
+        float v[4];
+        load4(src, count, v);
+        for (int s0 = 1; s0 < splits; s0 += 4) {
+            float u[4][4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s0 + s < splits) load4(src + (int64_t)(s0 + s) * total, count, u[s]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s0 + s < splits) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], u[s][j]);
+                }
+        }
+        tail_finish(tail, n, row, col, count, in, v);
+    }
+}
+
 template <bool TA, bool TB, int EPI, int CL = 0>
 void launch_tile(Context &ctx, const KParams &p, dim3 grid, int tile) {
 #define MMH_GEMM_TILE(WM, WN, MB, WK)                                                        \
@@ -1054,6 +1123,9 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
         launch_tile<false, false, EPI_SWIGLU>(ctx, p, grid, tile);
     } else if (epi == EPI_SWIGLU_BWD) {
         launch_tile<false, true, EPI_SWIGLU_BWD>(ctx, p, grid, tile);
+    } else if (epi == EPI_LINEAR) {
+        if (tb) launch_tile<false, true, EPI_LINEAR>(ctx, p, grid, tile);
+        else launch_tile<false, false, EPI_LINEAR>(ctx, p, grid, tile);
     } else if (p.rope_cos) {  // heads of 64 or 128 columns rotated in registers
         if (p.rope_hd == 64) launch_tile<false, false, EPI_STORE, 1>(ctx, p, grid, tile);
         else launch_tile<false, false, EPI_STORE, 2>(ctx, p, grid, tile);
@@ -1066,6 +1138,13 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
 }
 
 void launch_splitk_reduce(Context &ctx, const KParams &p, int epi) {
+    if (epi == EPI_LINEAR) {
+        const int64_t units = p.m * ((p.n + 3) / 4);
+        hipLaunchKernelGGL(splitk_linear, dim3((unsigned)std::min<int64_t>((units + 255) / 256, 8192)),
+                           dim3(256), 0, ctx.stream, p.partial, p.tail, p.m, p.n, p.splits);
+        check_hip(hipGetLastError(), "split-k linear launch");
+        return;
+    }
     const int64_t total = p.m * p.n;
     const bool vec = p.n % 4 == 0 && p.ldc % 4 == 0 && aligned16(p.c) && aligned16(p.partial) &&
                      (!p.resid || aligned16(p.resid));

@@ -7,7 +7,6 @@
 // Dropout's mask is drawn again wherever it is needed, from the call's key and
 // counter, and never stored.
 #include <algorithm>
-#include <cmath>
 
 #include "mmh_args.h"
 #include "mmh_elementwise.h"
@@ -84,40 +83,47 @@ void launch_dropout(Context &ctx, const float *x, const float *residual, int64_t
     check_hip(hipGetLastError(), "dropout launch");
 }
 
-// out = residual + dropout(act(prod + bias)); pre (when wanted) = prod + bias.
-__global__ __launch_bounds__(256) void linear_finish_kernel(const float *prod, const float *bias,
-                                                            const float *residual, int64_t total,
-                                                            int64_t n, int act, Drop d, float *pre,
-                                                            float *out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float v = prod[i];
-        if (bias) v += bias[i % n];
-        if (pre) pre[i] = v;
-        v = activate(act, v);
-        if (d.on) v = drop_value(d, i, v);
-        out[i] = residual ? residual[i] + v : v;
-    }
-}
-
-// dpre = dropout(dout) * act'(pre)
+// dpre = dropout(dout) * act'(pre) (written where WRITE) and the column sums of
+// a strip of rows of it. A wave walks rows of 256 columns, four per lane: 16-byte
+// accesses, one generator block per four values. Bound by its reads and writes.
+template <bool WRITE>
 __global__ __launch_bounds__(256) void linear_dpre_kernel(const float *dout, const float *pre,
-                                                          int64_t total, int act, Drop d,
-                                                          float *dpre) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float v = dout[i];
-        if (d.on) v = drop_value(d, i, v);
-        dpre[i] = activate_grad(act, pre ? pre[i] : 0.0f, v);
+                                                          int64_t rows, int64_t n, int64_t strip,
+                                                          int act, Drop d, float *dpre, float *sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 256 + 4 * lane;
+    const int64_t first = (int64_t)blockIdx.y * strip, last = min(rows, first + strip);
+    const int count = (int)max((int64_t)0, min(n - col, (int64_t)4));
+    float acc[4] = {};
+    if (count > 0) {
+        for (int64_t row = first + wave; row < last; row += 4) {
+            const int64_t i = row * n + col;
+            float v[4], x[4] = {};
+            load4(dout + i, count, v);
+            if (act != MMH_ACT_NONE) load4(pre + i, count, x);
+            if (d.on) drop4(d, i, v);
+            activate_grad4(act, x, v);
+            if (WRITE) store4(dpre + i, count, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += v[j];
+        }
+    }
+    if (!sums) return;
+    __shared__ __attribute__((aligned(16))) float part[4][256];
+    __builtin_memcpy(&part[wave][4 * lane], acc, 16);
+    __syncthreads();
+    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (j < n) {
+        const int t = threadIdx.x;
+        sums[blockIdx.y * n + j] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
     }
 }
 
-// Column sums of y [rows, n] in 64 bits, a thread per column.
-__global__ __launch_bounds__(64) void column_sums_kernel(const float *y, int64_t rows, int64_t n,
-                                                         float *out) {
-    const int64_t j = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (j >= n) return;
-    double s = 0.0;
-    for (int64_t i = 0; i < rows; ++i) s += (double)y[i * n + j];
-    out[j] = (float)s;
+// Strips of rows for about four workgroups per CU, 16 rows at least.
+int64_t strip_rows(const Context &ctx, int64_t rows, int64_t n) {
+    const int64_t cols = (n + 255) / 256, want = std::max<int64_t>(1, 4 * (int64_t)ctx.cu_count / cols);
+    const int64_t strip = std::max<int64_t>(16, (rows + want - 1) / want);
+    return std::max(strip, (rows + 65534) / 65535);  // (a grid's y)
 }
 
 void check_linear(int32_t form, int64_t rows, int64_t k, int64_t n, int32_t act) {
@@ -134,7 +140,7 @@ void check_linear(int32_t form, int64_t rows, int64_t k, int64_t n, int32_t act)
 }
 
 void product(Context &cx, const float *a, bool ta, const float *b, bool tb, float *c, int64_t m,
-             int64_t k, int64_t n) {
+             int64_t k, int64_t n, const LinearTail *tail = nullptr) {
     GemmDesc g;
     g.a = a;
     g.ta = ta;
@@ -147,6 +153,10 @@ void product(Context &cx, const float *a, bool ta, const float *b, bool tb, floa
     g.m = m;
     g.k = k;
     g.n = n;
+    if (tail) {
+        g.epi = EPI_LINEAR;
+        g.tail = tail;
+    }
     gemm(cx, g);
 }
 
@@ -202,11 +212,14 @@ int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w,
         apart_or_same(so, {sr});
         apart({pre, rows * n, "pre"}, {sx, sw, sb, sr, so});
         Context &cx = context(ctx);
-        float *prod = pre ? pre : static_cast<float *>(cx.workspace(2, (size_t)(rows * n) * 4));
-        product(cx, x, false, w, form == MMH_GEMM_NT, prod, rows, k, n);
-        hipLaunchKernelGGL(linear_finish_kernel, dim3(grid_for(rows * n)), dim3(256), 0, cx.stream, prod,
-                           bias, residual, rows * n, n, activation, d, pre, out);
-        check_hip(hipGetLastError(), "linear epilogue launch");
+        LinearTail tail;
+        tail.bias = bias;
+        tail.residual = residual;
+        tail.pre = pre;
+        tail.out = out;
+        tail.act = activation;
+        tail.drop = d;
+        product(cx, x, false, w, form == MMH_GEMM_NT, nullptr, rows, k, n, &tail);
         return MMH_OK;
     });
 }
@@ -232,17 +245,24 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
         if (!dx && !dw && !dbias) return MMH_OK;
         const bool nt = form == MMH_GEMM_NT;
         const float *dpre = dout;
-        if (activation != MMH_ACT_NONE || d.on) {
-            float *buf = static_cast<float *>(cx.workspace(2, (size_t)(rows * n) * 4));
-            hipLaunchKernelGGL(linear_dpre_kernel, dim3(grid_for(rows * n)), dim3(256), 0, cx.stream, dout,
-                               pre, rows * n, activation, d, buf);
+        const bool changes = activation != MMH_ACT_NONE || d.on;
+        if (changes || dbias) {
+            const int64_t strip = strip_rows(cx, rows, n), strips = (rows + strip - 1) / strip;
+            const size_t values = changes ? ((size_t)(rows * n) + 63) / 64 * 64 : 0;
+            float *buf = static_cast<float *>(
+                cx.workspace(2, (values + (dbias ? (size_t)(strips * n) : 0)) * 4));
+            float *sums = dbias ? buf + values : nullptr;
+            const dim3 grid((unsigned)((n + 255) / 256), (unsigned)strips);
+            if (changes) {
+                hipLaunchKernelGGL(linear_dpre_kernel<true>, grid, dim3(256), 0, cx.stream, dout, pre, rows,
+                                   n, strip, activation, d, buf, sums);
+                dpre = buf;
+            } else {
+                hipLaunchKernelGGL(linear_dpre_kernel<false>, grid, dim3(256), 0, cx.stream, dout, pre, rows,
+                                   n, strip, activation, d, nullptr, sums);
+            }
             check_hip(hipGetLastError(), "linear dpre launch");
-            dpre = buf;
-        }
-        if (dbias) {
-            hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, cx.stream,
-                               dpre, rows, n, dbias);
-            check_hip(hipGetLastError(), "linear dbias launch");
+            if (dbias) launch_sum_rows(cx, sums, strips, n, dbias);
         }
         if (dx) product(cx, dpre, false, w, !nt, dx, rows, n, k);
         if (dw && !nt) product(cx, x, true, dpre, false, dw, k, rows, n);

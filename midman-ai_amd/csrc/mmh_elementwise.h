@@ -7,57 +7,113 @@
 namespace mmh {
 
 // ---- activations ------------------------------------------------------------
-// Written so that no digits cancel: gelu through erfc(-x / sqrt 2) instead of
-// 1 + erf(x / sqrt 2), 1 - sigmoid as the other side's sigmoid.
-constexpr float kRoot1_2 = 0.70710678118654752f, kInvRoot2Pi = 0.39894228040143268f;
-constexpr float kTanhC0 = 0.79788456080286536f, kTanhC1 = 0.044715f;
+// The VALU's time adds to the matrix core's, so these stay short, but each is
+// within a few ulps over the whole range: the hardware's exp2 and reciprocal, with
+// the rounding errors of their arguments carried along, and no digits that
+// cancel (1 - sigmoid is the other side's sigmoid, gelu's far side a tail).
+constexpr float kTanhC0 = 0.79788456080286536f, kTanhC1 = 0.044715f;  // sqrt(2 / pi), gelu_tanh's cubic
 
-// sigmoid(y) and sigmoid(-y): the exponential's argument is never positive.
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
+// exp(x), x <= 0: 2^(x log2 e), the low part of the exponent applied as 1 + low ln 2.
+__device__ __forceinline__ float exp_neg(float x) {
+    constexpr float kHi = 1.44269502f, kLo = 1.92596303e-8f, kLn2 = 0.69314718f;
+    x = fmaxf(x, -104.0f);  // (e^-104 is below the smallest f32)
+    const float t = x * kHi;
+    const float low = __builtin_fmaf(x, kLo, __builtin_fmaf(x, kHi, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, low * kLn2, e);
+}
+// sigmoid(y) and sigmoid(-y).
 __device__ __forceinline__ void sigmoid_pair(float y, float &s, float &r) {
-    const float a = expf(-fabsf(y)), p = __fdiv_rn(1.0f, 1.0f + a), q = a * p;
+    const float a = exp_neg(-fabsf(y)), p = reciprocal(1.0f + a), q = a * p;
     s = y < 0.0f ? q : p;
     r = y < 0.0f ? p : q;
 }
 // gelu's tanh form 0.5 x (1 + tanh(u)) is x sigmoid(2 u), u = C0 (x + C1 x^3).
 __device__ __forceinline__ float tanh_arg2(float x) {
-    return 2.0f * kTanhC0 * x * (1.0f + kTanhC1 * x * x);
+    return 2.0f * kTanhC0 * x * __builtin_fmaf(kTanhC1 * x, x, 1.0f);
+}
+// e = exp(-x^2 / 2) and the normal tail Phi(-|x|) = e erfcx(|x| / sqrt 2) / 2.
+// erfcx is a polynomial in t = 1 / (1 + 0.35 |x| / sqrt 2), fitted here to the
+// least largest relative error over |x| <= 13.15, 1.4e-8 (beyond, e is 0 in f32).
+__device__ __forceinline__ float normal_tail(float x, float &e) {
+    const float ax = fminf(fabsf(x), 15.0f), sq = ax * ax;
+    e = exp_neg(-0.5f * sq);
+    e = __builtin_fmaf(e, -0.5f * __builtin_fmaf(ax, ax, -sq), e);
+    const float t = reciprocal(__builtin_fmaf(0.247487373f, ax, 1.0f));
+    float q = 0.06764230132102966f;
+    q = __builtin_fmaf(q, t, -0.40613067150115967f);
+    q = __builtin_fmaf(q, t, 0.8532063364982605f);
+    q = __builtin_fmaf(q, t, -0.757356584072113f);
+    q = __builtin_fmaf(q, t, 0.6861104369163513f);
+    q = __builtin_fmaf(q, t, -0.08201061189174652f);
+    q = __builtin_fmaf(q, t, 0.2549700140953064f);
+    q = __builtin_fmaf(q, t, 0.18484941124916077f);
+    q = __builtin_fmaf(q, t, 0.1987789422273636f);
+    q = __builtin_fmaf(q, t, -5.9628724557114765e-05f);
+    return 0.5f * e * q;
 }
 
-__device__ __forceinline__ float activate(int act, float x) {
-    switch (act) {
-        case MMH_ACT_RELU: return x < 0.0f ? 0.0f : x;
-        case MMH_ACT_GELU: return 0.5f * x * erfcf(-kRoot1_2 * x);
-        case MMH_ACT_GELU_TANH: return __fdiv_rn(x, 1.0f + expf(-tanh_arg2(x)));
-        case MMH_ACT_SILU: return __fdiv_rn(x, 1.0f + expf(-x));
-        default: return x;
-    }
+__device__ __forceinline__ float gelu_f(float x) {
+    float e;
+    const float tail = normal_tail(x, e);
+    return x * (x < 0.0f ? tail : 1.0f - tail);
 }
-
-// dh * act'(x). The terms x * (something that has reached 0) are 0 for any x,
+__device__ __forceinline__ float gelu_tanh_f(float x) {
+    float s, r;
+    sigmoid_pair(tanh_arg2(x), s, r);
+    return x * s;
+}
+__device__ __forceinline__ float silu_sigmoid_f(float x) {
+    float s, r;
+    sigmoid_pair(x, s, r);
+    return x * s;
+}
+// The slopes. A term x * (something that has reached 0) is 0 for any x,
 // infinities too.
-__device__ __forceinline__ float activate_grad(int act, float x, float dh) {
+__device__ __forceinline__ float gelu_slope(float x) {
+    float e;
+    const float tail = normal_tail(x, e);
+    const float phi = 0.39894228040143268f * e;
+    return (x < 0.0f ? tail : 1.0f - tail) + (phi == 0.0f ? 0.0f : x * phi);
+}
+__device__ __forceinline__ float gelu_tanh_slope(float x) {
+    float s, r;
+    sigmoid_pair(tanh_arg2(x), s, r);
+    const float sr = s * r;
+    return s + (sr == 0.0f ? 0.0f : 2.0f * kTanhC0 * x * __builtin_fmaf(3.0f * kTanhC1 * x, x, 1.0f) * sr);
+}
+__device__ __forceinline__ float silu_slope(float x) {
+    float s, r;
+    sigmoid_pair(x, s, r);
+    const float sr = s * r;
+    return s + (sr == 0.0f ? 0.0f : x * sr);
+}
+
+// v = act(v), four values: one uniform branch for them.
+__device__ __forceinline__ void activate4(int act, float (&v)[4]) {
+#define MMH_EACH4(E) _Pragma("unroll") for (int j = 0; j < 4; ++j) E
     switch (act) {
-        case MMH_ACT_RELU: return x > 0.0f ? dh : 0.0f;
-        case MMH_ACT_GELU: {
-            const float phi = kInvRoot2Pi * expf(-0.5f * x * x);
-            const float t = phi == 0.0f ? 0.0f : x * phi;
-            return dh * (0.5f * erfcf(-kRoot1_2 * x) + t);
-        }
-        case MMH_ACT_GELU_TANH: {
-            float s, r;
-            sigmoid_pair(tanh_arg2(x), s, r);
-            const float sr = s * r;
-            const float t = sr == 0.0f ? 0.0f : 2.0f * kTanhC0 * x * (1.0f + 3.0f * kTanhC1 * x * x) * sr;
-            return dh * (s + t);
-        }
-        case MMH_ACT_SILU: {
-            float s, r;
-            sigmoid_pair(x, s, r);
-            const float sr = s * r;
-            return dh * (s + (sr == 0.0f ? 0.0f : x * sr));
-        }
-        default: return dh;
+        case MMH_ACT_RELU: MMH_EACH4(v[j] = v[j] < 0.0f ? 0.0f : v[j]); break;
+        case MMH_ACT_GELU: MMH_EACH4(v[j] = gelu_f(v[j])); break;
+        case MMH_ACT_GELU_TANH: MMH_EACH4(v[j] = gelu_tanh_f(v[j])); break;
+        case MMH_ACT_SILU: MMH_EACH4(v[j] = silu_sigmoid_f(v[j])); break;
+        default: break;
     }
+}
+// dh *= act'(x)
+__device__ __forceinline__ void activate_grad4(int act, const float (&x)[4], float (&dh)[4]) {
+    switch (act) {
+        case MMH_ACT_RELU: MMH_EACH4(dh[j] = x[j] > 0.0f ? dh[j] : 0.0f); break;
+        case MMH_ACT_GELU: MMH_EACH4(dh[j] *= gelu_slope(x[j])); break;
+        case MMH_ACT_GELU_TANH: MMH_EACH4(dh[j] *= gelu_tanh_slope(x[j])); break;
+        case MMH_ACT_SILU: MMH_EACH4(dh[j] *= silu_slope(x[j])); break;
+        default: break;
+    }
+#undef MMH_EACH4
 }
 
 // ---- dropout ----------------------------------------------------------------
@@ -91,11 +147,76 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint32_t k0, uint32_t k1
 __device__ __forceinline__ float drop_word(const Drop &d, uint32_t word, float x) {
     return word <= d.last ? 0.0f : x * d.scale;
 }
-// Value i alone (a block for one of its four words).
-__device__ __forceinline__ float drop_value(const Drop &d, int64_t i, float x) {
-    const uint4 w = philox(d.offset + ((uint64_t)i >> 2), d.k0, d.k1);
-    const int j = (int)(i & 3);
-    return drop_word(d, j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w, x);
+// Values i .. i + 3 of an array: one block where they are its four words, else
+// two that follow each other.
+__device__ __forceinline__ void drop4(const Drop &d, int64_t i, float (&v)[4]) {
+    const uint64_t block = d.offset + ((uint64_t)i >> 2);
+    const uint4 a = philox(block, d.k0, d.k1);
+    uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    const int first = (int)(i & 3);
+    if (first) {
+        const uint4 b = philox(block + 1, d.k0, d.k1);
+        const uint32_t e[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = first == 1 ? e[j + 1] : first == 2 ? e[j + 2] : e[j + 3];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = drop_word(d, w[j], v[j]);
+}
+
+// Up to four neighbouring values of an array at any 4-byte alignment (gfx950
+// moves 16 bytes at any dword); those past `count` read as 0 and are not written.
+__device__ __forceinline__ void load4(const float *p, int count, float (&v)[4]) {
+    if (count == 4) {
+        __builtin_memcpy(v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = j < count ? p[j] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store4(float *p, int count, const float (&v)[4]) {
+    if (count == 4) {
+        __builtin_memcpy(p, v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) p[j] = v[j];
+    }
+}
+
+// ---- the linear layer's epilogue ---------------------------------------------
+// What follows the product in out = residual + dropout(act(product + bias)),
+// out [rows, n] contiguous. Pointers that are not wanted are null.
+struct LinearTail {
+    const float *bias = nullptr, *residual = nullptr;
+    float *pre = nullptr, *out = nullptr;
+    int act = MMH_ACT_NONE;
+    Drop drop;
+};
+// The part read from memory of columns col .. col + count - 1 of a row.
+struct TailInputs {
+    float b[4], r[4];
+};
+__device__ __forceinline__ void tail_load(const LinearTail &t, int64_t n, int64_t row, int64_t col,
+                                          int count, TailInputs &in) {
+    if (t.bias) load4(t.bias + col, count, in.b);
+    if (t.residual) load4(t.residual + row * n + col, count, in.r);
+}
+__device__ __forceinline__ void tail_finish(const LinearTail &t, int64_t n, int64_t row, int64_t col,
+                                            int count, const TailInputs &in, float (&v)[4]) {
+    const int64_t i = row * n + col;
+    if (t.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += in.b[j];
+    }
+    if (t.pre) store4(t.pre + i, count, v);
+    activate4(t.act, v);
+    if (t.drop.on) drop4(t.drop, i, v);
+    if (t.residual) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = in.r[j] + v[j];
+    }
+    store4(t.out + i, count, v);
 }
 
 }  // namespace mmh

@@ -3,6 +3,7 @@
 // (gemm_split.hip) use.
 #pragma once
 
+#include "mmh_elementwise.h"
 #include "mmh_internal.h"
 
 namespace mmh {
@@ -45,6 +46,7 @@ struct KParams {
     const int32_t *ce_targets;
     float *ce_part, *ce_zt;
     int ce_tiles;  // 128-column units of a row
+    LinearTail tail;  // EPI_LINEAR
     // Large tiles, the exponentials of EPI_SWIGLU and EPI_CE: libm's (and the IEEE
     // division) where the grid has less than a 128x128 tile per CU, as the small
     // kernels have it. The hardware's exp2 of a rounded product, which fuller

@@ -117,8 +117,11 @@ void release_models_of(mmh_handle ctx);
 // exp(z - max)) over its columns, and the tile holding column ce_targets[i]
 // leaves that logit in ce_zt[i] (the head GEMM with the loss folded in; see
 // gemm_ce_tiles and launch_ce_combine).
+// EPI_LINEAR (batch 1, nn and nt): C is not written; the products go through
+// `tail` (bias, activation, dropout, residual) into tail->out.
 enum Epilogue : int { EPI_STORE = 0, EPI_ACCUM = 1, EPI_SWIGLU = 2, EPI_SWIGLU_BWD = 3,
-                      EPI_CE = 4 };
+                      EPI_CE = 4, EPI_LINEAR = 5 };
+struct LinearTail;  // mmh_elementwise.h
 
 // mmh_gemm_noalloc: the partials of the plan its contract is stated in, and the
 // array the kernels' own partials live in (their plans stay below it).
@@ -155,6 +158,7 @@ struct GemmDesc {
     // partials [m, gemm_ce_tiles, 2] and target logits [m] out.
     const int32_t *ce_targets = nullptr;
     float *ce_part = nullptr, *ce_zt = nullptr;
+    const LinearTail *tail = nullptr;  // EPI_LINEAR
     // Device memory for the split-K partials supplied by the caller (null: the
     // context's growable workspace), kNoallocScratchBytes of it: gemm() then
     // takes what mmh_gemm_noalloc takes and refuses the rest (MMH_ERR_SHAPE).
@@ -240,6 +244,8 @@ struct RefLayout {
 void launch_gather_ref(Context &ctx, const RefLayout &p, const float *dev, float *ref);
 // host[0] = *a, host[1] = *b (host: pinned memory), bit for bit.
 void launch_copy_words(Context &ctx, const float *a, const float *b, float *host);
+// out[j] = sum over nrows rows of partial [nrows, d], in a fixed order.
+void launch_sum_rows(Context &ctx, const float *partial, int64_t nrows, int64_t d, float *out);
 int64_t global_norm_scratch_bytes();
 void launch_global_norm(Context &ctx, const float *g, int64_t n, double *scratch, float *norm);
 struct AdamArgs {

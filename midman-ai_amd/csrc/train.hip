@@ -789,6 +789,12 @@ void launch_gather_ref(Context &ctx, const RefLayout &p, const float *dev, float
     check_hip(hipGetLastError(), "reference order launch");
 }
 
+void launch_sum_rows(Context &ctx, const float *partial, int64_t nrows, int64_t d, float *out) {
+    hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)((d + 63) / 64)), dim3(64 * SUM_WAVES), 0,
+                       ctx.stream, partial, nrows, d, out);
+    check_hip(hipGetLastError(), "row sums launch");
+}
+
 int64_t global_norm_scratch_bytes() { return (int64_t)NORM_BLOCKS * 8; }
 
 void launch_global_norm(Context &ctx, const float *g, int64_t n, double *scratch, float *norm) {
