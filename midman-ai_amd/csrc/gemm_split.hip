@@ -800,6 +800,10 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
     // barriers order them before the epilogue reads them)
     __shared__ int ce_t[EPI == EPI_CE ? TM : 1];
     if (EPI == EPI_CE && tid < TM) ce_t[tid] = m0 + tid < M ? p.ce_targets[m0 + tid] : -1;
+    // EPI_LINEAR: the tile's bias likewise (-0 for none, the identity of addition)
+    __shared__ __attribute__((aligned(16))) float bias_s[EPI == EPI_LINEAR ? TN : 1];
+    if (EPI == EPI_LINEAR && tid < TN)
+        bias_s[tid] = p.tail.bias && n0 + tid < N ? p.tail.bias[n0 + tid] : -0.0f;
     split_mainloop<TA, TB, CL, WM, WN, MB, WK>(p, A, B, m0, n0, kbeg, kend, lds, acc);
 
     const int lane = tid & 63, wave = tid % NT >> 6;
@@ -948,36 +952,82 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
         // 32 rows of each wave at a time through LDS (free behind the barrier
         // above), so that a thread has four neighbouring columns of a row: one
         // generator block, and 16-byte accesses to the residual and the
-        // outputs. The loop stays rolled: unrolled, its four copies of the
-        // activations would not fit the instruction cache.
-        constexpr int ROWS = WM * 32, LD = TN + 4, THREADS = NT * WK;
+        // outputs. The residual of up to four units is read ahead (the first ones
+        // before the barrier), the bias before the K loop: a lone workgroup has
+        // nothing else to wait behind. The activations work in place in LDS, in a
+        // loop that stays rolled (unrolled, their copies would not fit the
+        // instruction cache).
+        constexpr int ROWS = WM * 32, LD = TN + 4, THREADS = NT * WK, UNITS = ROWS * TN / 4 / THREADS;
+        constexpr int AHEAD = UNITS < 4 ? UNITS : 4;
+        static_assert(TN <= THREADS, "a thread for each column's bias");
         static_assert(ROWS * LD * 4 <= WK * 2 * S::STAGE, "a block row fits the stages");
-        static_assert(ROWS * TN % (4 * THREADS) == 0, "whole rounds of units");
+        static_assert(UNITS * 4 * THREADS == ROWS * TN && THREADS % (TN / 4) == 0 && UNITS % AHEAD == 0,
+                      "a thread's units are of one column");
+        constexpr int STEP = THREADS / (TN / 4);  // rows from one unit of a thread to its next
         float *tile = reinterpret_cast<float *>(lds);
+        const LinearTail &t = p.tail;
+        const int r0 = tid / (TN / 4), c = tid % (TN / 4) * 4;
+        const int64_t cc = n0 + c;
+        const int count = cc < N ? (int)min(N - cc, (int64_t)4) : 0;
+        const bool values = t.act != MMH_ACT_NONE || t.drop.on || t.pre;
 #pragma unroll 1
         for (int i = 0; i < MB; ++i) {
-            if (first) {
-                unroll_seq([&](auto ic) __attribute__((always_inline)) {
-                    if (ic != i) return;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        *reinterpret_cast<float2 *>(tile + (wm * 32 + 8 * (r >> 2) + 4 * lk + (r & 3)) * LD +
-                                                    wn * 64 + 2 * lr) =
-                            make_float2(acc[ic][0][r], acc[ic][1][r]);
-                }, std::make_integer_sequence<int, MB>{});
-            }
-            __syncthreads();
 #pragma unroll 1
-            for (int e = tid; e < ROWS * TN / 4; e += THREADS) {
-                const int rl = e / (TN / 4), c = e % (TN / 4) * 4;
-                const int64_t row = m0 + (rl / 32 * MB + i) * 32 + rl % 32, cc = n0 + c;
-                if (row >= M || cc >= N) continue;
-                const int count = (int)min(N - cc, (int64_t)4);
-                TailInputs in;
-                tail_load(p.tail, N, row, cc, count, in);
-                float v[4];
-                __builtin_memcpy(v, __builtin_assume_aligned(tile + rl * LD + c, 16), 16);
-                tail_finish(p.tail, N, row, cc, count, in, v);
+            for (int u0 = 0; u0 < UNITS; u0 += AHEAD) {
+                auto row_of = [&](int u) __attribute__((always_inline)) {
+                    const int rl = r0 + (u0 + u) * STEP;
+                    return m0 + (rl / 32 * MB + i) * 32 + rl % 32;
+                };
+                float res[AHEAD][4];
+                if (t.residual && count > 0) {
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u)  // (rows past the edge read the last one)
+                        load4(t.residual + min(row_of(u), M - 1) * N + cc, count, res[u]);
+                }
+                if (u0 == 0) {
+                    if (first) {
+                        unroll_seq([&](auto ic) __attribute__((always_inline)) {
+                            if (ic != i) return;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                *reinterpret_cast<float2 *>(
+                                    tile + (wm * 32 + 8 * (r >> 2) + 4 * lk + (r & 3)) * LD + wn * 64 + 2 * lr) =
+                                    make_float2(acc[ic][0][r], acc[ic][1][r]);
+                        }, std::make_integer_sequence<int, MB>{});
+                    }
+                    __syncthreads();
+                }
+                float *mine = tile + (r0 + u0 * STEP) * LD + c;
+                float bias[4];
+                __builtin_memcpy(bias, __builtin_assume_aligned(bias_s + c, 16), 16);
+                if (values) {
+#pragma unroll 1
+                    for (int u = 0; u < AHEAD; ++u) {
+                        const int64_t row = row_of(u);
+                        if (row >= M || count == 0) break;
+                        float v[4];
+                        __builtin_memcpy(v, __builtin_assume_aligned(mine + u * STEP * LD, 16), 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] += bias[j];
+                        tail_values(t, N, row, cc, count, v);
+                        __builtin_memcpy(__builtin_assume_aligned(mine + u * STEP * LD, 16), v, 16);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int64_t row = row_of(u);
+                    float v[4];
+                    __builtin_memcpy(v, __builtin_assume_aligned(mine + u * STEP * LD, 16), 16);
+                    if (!values) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] += bias[j];
+                    }
+                    if (t.residual) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = res[u][j] + v[j];
+                    }
+                    if (row < M) store4(t.out + row * N + cc, count, v);
+                }
             }
             __syncthreads();
         }

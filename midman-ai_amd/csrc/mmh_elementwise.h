@@ -202,21 +202,26 @@ __device__ __forceinline__ void tail_load(const LinearTail &t, int64_t n, int64_
     if (t.bias) load4(t.bias + col, count, in.b);
     if (t.residual) load4(t.residual + row * n + col, count, in.r);
 }
+// act and dropout of pre = v (stored where it is kept).
+__device__ __forceinline__ void tail_values(const LinearTail &t, int64_t n, int64_t row, int64_t col,
+                                            int count, float (&v)[4]) {
+    const int64_t i = row * n + col;
+    if (t.pre) store4(t.pre + i, count, v);
+    activate4(t.act, v);
+    if (t.drop.on) drop4(t.drop, i, v);
+}
 __device__ __forceinline__ void tail_finish(const LinearTail &t, int64_t n, int64_t row, int64_t col,
                                             int count, const TailInputs &in, float (&v)[4]) {
-    const int64_t i = row * n + col;
     if (t.bias) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += in.b[j];
     }
-    if (t.pre) store4(t.pre + i, count, v);
-    activate4(t.act, v);
-    if (t.drop.on) drop4(t.drop, i, v);
+    tail_values(t, n, row, col, count, v);
     if (t.residual) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = in.r[j] + v[j];
     }
-    store4(t.out + i, count, v);
+    store4(t.out + row * n + col, count, v);
 }
 
 }  // namespace mmh
