@@ -1239,7 +1239,9 @@ void check_noalloc(const Context &ctx, const GemmDesc &d) {
 void gemm(Context &ctx, const GemmDesc &d) {
     if (d.m <= 0 || d.n <= 0 || d.k <= 0 || d.batch <= 0) fail(MMH_ERR_SHAPE, "gemm: empty shape");
     if (d.ta && d.tb) fail(MMH_ERR_ARGUMENT, "gemm: one operand at most is transposed");
-    if (d.epi == EPI_CE && (gemm_ce_tiles(ctx, d) == 0 || !d.ce_targets || !d.ce_part || !d.ce_zt))
+    const bool ce = d.epi == EPI_CE || d.epi == EPI_CE_STORE;
+    if (ce && (gemm_ce_tiles(ctx, d) == 0 || !d.ce_part ||
+               (d.epi == EPI_CE ? !d.ce_targets || !d.ce_zt : !d.c)))
         fail(MMH_ERR_ARGUMENT, "gemm: the loss folds only into the large tiles of one matrix");
     KParams p{};
     p.a = d.a;
@@ -1349,7 +1351,7 @@ void gemm(Context &ctx, const GemmDesc &d) {
         while (tiles * splits < cus && splits < 16 && ktiles / (splits * 2) >= 8)
             splits *= 2;
     }
-    if (d.batch > 1 || d.epi == EPI_SWIGLU || d.epi == EPI_SWIGLU_BWD || d.epi == EPI_CE ||
+    if (d.batch > 1 || d.epi == EPI_SWIGLU || d.epi == EPI_SWIGLU_BWD || ce ||
         p.norm_w || p.rope_cos || kind == 1)
         splits = 1;
     const int64_t kt_per = (ktiles + splits - 1) / splits;

@@ -773,7 +773,8 @@ __device__ __forceinline__ void block_epilogue(const KParams &p, const floatx16 
 template <bool TA, bool TB, int EPI, int CL, int WM, int WN, int MB, int WK>
 __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) {
     static_assert(CL == 0 || EPI == EPI_STORE, "the RoPE column layouts store plain values");
-    static_assert(EPI != EPI_CE || WN % 2 == 0, "the loss takes 128 columns at a time");
+    constexpr bool CE = EPI == EPI_CE || EPI == EPI_CE_STORE;
+    static_assert(!CE || WN % 2 == 0, "the loss takes 128 columns at a time");
     using S = TileShape<WM, WN, MB>;
     constexpr int TM = S::TM, TN = S::TN, NT = S::NT;
     __shared__ __attribute__((aligned(128))) char lds[WK * 2 * S::STAGE];
@@ -891,14 +892,22 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
         }
     }
     redo = __syncthreads_or(redo);
-    if (EPI != EPI_CE && EPI != EPI_LINEAR && !first) return;
+    if (!CE && EPI != EPI_LINEAR && !first) return;
     if (first && redo) exact_mainloop<TA, TB, CL, WM, WN, MB>(p, A, B, m0, n0, kbeg, kend, acc);
 
     // ---- epilogue: block (i, j) register r of lane l is C[row][col] with
     // row = m0 + 32*(MB*wm + i) + 8*(r/4) + 4*(l/32) + r%4 and, for CL 0,
     // col = n0 + 64*wn + 2*(l%32) + j (the other layouts: place_col).
     const int64_t col = n0 + wn * 64 + 2 * lr;
-    if constexpr (EPI == EPI_CE) {
+    if constexpr (EPI == EPI_CE_STORE) {
+        if (first) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+                block_epilogue<EPI_STORE, CL, TM, TN>(p, acc[i][0], acc[i][1], split, batch, m0, n0,
+                                                      (wm * MB + i) * 32, wn, lr, lk);
+        }
+    }
+    if constexpr (CE) {
         // Cross-entropy partials of the tile's columns, 128 at a time
         // (ops_reduce.rs:236-259 split by column units): per row, the max of
         // the logits and the sum of exp(z - max) over the lane's two columns,
@@ -932,9 +941,11 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
                     ce_m[wn][rl] = e != e ? e : mx;
                     ce_s[wn][rl] = e;
                 }
-                const int t = ce_t[rl];
-                if (t == col) p.ce_zt[row] = v0;
-                if (t == col + 1) p.ce_zt[row] = v1;
+                if constexpr (EPI == EPI_CE) {
+                    const int t = ce_t[rl];
+                    if (t == col) p.ce_zt[row] = v0;
+                    if (t == col + 1) p.ce_zt[row] = v1;
+                }
             }
         __syncthreads();
         for (int e = tid; e < TM * (WN / 2); e += NT * WK) {
@@ -1137,10 +1148,10 @@ void launch_tile(Context &ctx, const KParams &p, dim3 grid, int tile) {
         case TILE_256x128: MMH_GEMM_TILE(4, 2, 2, 1); break;
         case TILE_128: MMH_GEMM_TILE(2, 2, 2, 2); break;
         case TILE_128x64:
-            if constexpr (EPI != EPI_CE && CL == 0) MMH_GEMM_TILE(4, 1, 1, 2);
+            if constexpr (EPI != EPI_CE && EPI != EPI_CE_STORE && CL == 0) MMH_GEMM_TILE(4, 1, 1, 2);
             break;
         case TILE_64:
-            if constexpr (EPI != EPI_CE && CL == 0) MMH_GEMM_TILE(2, 1, 1, 4);
+            if constexpr (EPI != EPI_CE && EPI != EPI_CE_STORE && CL == 0) MMH_GEMM_TILE(2, 1, 1, 4);
             break;
     }
 #undef MMH_GEMM_TILE
@@ -1161,7 +1172,8 @@ bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 // does not fit the 256x256 tile's registers (its epilogue spills).
 bool gemm_tile_takes(const KParams &p, int epi, int tile) {
     if (tile == TILE_256) return epi != EPI_SWIGLU_BWD;
-    return (tile != TILE_128x64 && tile != TILE_64) || (epi != EPI_CE && !p.rope_cos);
+    return (tile != TILE_128x64 && tile != TILE_64) ||
+           (epi != EPI_CE && epi != EPI_CE_STORE && !p.rope_cos);
 }
 
 void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool tb, int epi,
@@ -1169,6 +1181,9 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
     if (epi == EPI_CE) {
         if (tb) launch_tile<false, true, EPI_CE>(ctx, p, grid, tile);
         else launch_tile<false, false, EPI_CE>(ctx, p, grid, tile);
+    } else if (epi == EPI_CE_STORE) {
+        if (tb) launch_tile<false, true, EPI_CE_STORE>(ctx, p, grid, tile);
+        else launch_tile<false, false, EPI_CE_STORE>(ctx, p, grid, tile);
     } else if (epi == EPI_SWIGLU) {
         launch_tile<false, false, EPI_SWIGLU>(ctx, p, grid, tile);
     } else if (epi == EPI_SWIGLU_BWD) {

@@ -5,19 +5,22 @@
 // The logits are never whole in memory: the loss alone folds into the head's
 // product (EPI_CE: a maximum and a sum per row and 128 columns), and the
 // gradients take blocks of rows, whose logits become dz in place in a workspace
-// of kLogitBytes. Rows whose target is `ignore` are left out before the first
+// of kLogitBytes. A pass over them reads and writes each row once: up to kRowCols
+// columns from registers; for wider rows the product leaves the same partials
+// beside the logits, which costs its epilogue more than the second read of a
+// row costs elsewhere. Rows whose target is `ignore` are left out before the first
 // product, so nothing they hold (infinities, NaN) reaches a sum.
 #include <algorithm>
-#include <vector>
 
 #include "mmh_args.h"
+#include "mmh_elementwise.h"
 #include "mmh_internal.h"
 
 namespace mmh {
 namespace {
 
 // The workspace of a block's logits, and the rows that a block has at least.
-constexpr int64_t kLogitBytes = int64_t(256) << 20;
+constexpr int64_t kLogitBytes = int64_t(512) << 20;
 constexpr int64_t kMinRows = 128;
 
 int64_t block_rows(int64_t n, int64_t row_bytes) {
@@ -42,55 +45,132 @@ __global__ __launch_bounds__(256) void spread_rows_kernel(const float *__restric
     }
 }
 
-// A row's loss, max + ln(sum exp(z - max)) - z[target], and with GRAD dz =
-// (exp(z - max) / sum - onehot) * scale in its place. One workgroup per row,
-// rows of ld (a multiple of 4, 16-byte aligned) floats of which v are logits;
-// the maximum first, so that a NaN anywhere reaches the sum.
-template <bool GRAD>
-__global__ __launch_bounds__(256) void loss_rows_kernel(float *z, const int32_t *targets, int64_t ld,
-                                                        int64_t v, float scale, float *row_loss) {
-    __shared__ float red_m[4], red_s[4];
+// Rows of stored logits of up to kRowCols columns: the row's loss, max + ln(sum
+// exp(z - max)) - z[target], and with GRAD dz = (exp(z - max) / sum - onehot) *
+// scale in its place. A workgroup holds a row in registers, NV float4s per
+// thread, so it passes through once; rows are ld (a multiple of 4, 16-byte
+// aligned) floats of which v are logits. A NaN anywhere reaches the sum. Bound by
+// the logits' read and write.
+constexpr int64_t kRowCols = 32768;
+template <int NT, int NV, bool GRAD>
+__global__ __launch_bounds__(NT) void loss_rows_kernel(float *z, const int32_t *targets, int64_t ld, int v,
+                                                       float scale, float *row_loss) {
+    __shared__ float red_m[NT / 64], red_s[NT / 64];
     const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, v4 = (v + 3) / 4;
     float4 *z4 = reinterpret_cast<float4 *>(z + row * ld);
-    const int64_t v4 = (v + 3) / 4;
-    const int32_t t = targets[row];
-    const float zt = z[row * ld + t];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    auto load = [&](int64_t q) {
-        float4 a = z4[q];
-        if (4 * q + 1 >= v) a.y = -INFINITY;
-        if (4 * q + 2 >= v) a.z = -INFINITY;
-        if (4 * q + 3 >= v) a.w = -INFINITY;
-        return a;
-    };
-    float m = -INFINITY;
-    for (int64_t q = threadIdx.x; q < v4; q += 256) {
-        const float4 a = load(q);
-        m = fmaxf(m, fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)));
+    const int t = targets[row];
+    float4 e[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int q = tid + NT * i;
+        e[i] = z4[min(q, v4 - 1)];
+        if (4 * q >= v) e[i].x = -INFINITY;
+        if (4 * q + 1 >= v) e[i].y = -INFINITY;
+        if (4 * q + 2 >= v) e[i].z = -INFINITY;
+        if (4 * q + 3 >= v) e[i].w = -INFINITY;
     }
+    const float zt = tid == 0 ? z[row * ld + t] : 0.0f;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m = fmaxf(m, fmaxf(fmaxf(e[i].x, e[i].y), fmaxf(e[i].z, e[i].w)));
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     if (lane == 0) red_m[wave] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) m = fmaxf(m, red_m[i]);
     float s = 0.0f;
-    for (int64_t q = threadIdx.x; q < v4; q += 256) {
-        const float4 a = load(q);
-        s += (expf(a.x - m) + expf(a.y - m)) + (expf(a.z - m) + expf(a.w - m));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        // (columns past the row hold -inf: exp gives 0)
+        e[i] = make_float4(exp_neg(e[i].x - m), exp_neg(e[i].y - m), exp_neg(e[i].z - m),
+                           exp_neg(e[i].w - m));
+        s += (e[i].x + e[i].y) + (e[i].z + e[i].w);
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if (lane == 0) red_s[wave] = s;
+    __syncthreads();  // (z[target] has been read, too)
+    s = red_s[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) s += red_s[i];
+    if (tid == 0) row_loss[row] = (m + logf(s)) - zt;
+    if constexpr (!GRAD) return;
+    const float f = __fdiv_rn(scale, s);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int q = tid + NT * i;
+        if (q >= v4) break;
+        float4 a = make_float4(e[i].x * f, e[i].y * f, e[i].z * f, e[i].w * f);
+        if (t >> 2 == q) {
+            if ((t & 3) == 0) a.x -= scale;
+            if ((t & 3) == 1) a.y -= scale;
+            if ((t & 3) == 2) a.z -= scale;
+            if ((t & 3) == 3) a.w -= scale;
+        }
+        z4[q] = a;
+    }
+}
+
+template <bool GRAD>
+void launch_loss_rows(Context &cx, float *z, const int32_t *targets, int64_t rows, int64_t ld, int64_t v,
+                      float scale, float *row_loss) {
+    auto launch = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, cx.stream, z, targets, ld, (int)v,
+                           scale, row_loss);
+    };
+    if (v <= 1024) launch(loss_rows_kernel<256, 1, GRAD>, 256);
+    else if (v <= 4096) launch(loss_rows_kernel<256, 4, GRAD>, 256);
+    else if (v <= 8192) launch(loss_rows_kernel<512, 4, GRAD>, 512);
+    else if (v <= 16384) launch(loss_rows_kernel<512, 8, GRAD>, 512);
+    else if (v <= kRowCols) launch(loss_rows_kernel<512, 16, GRAD>, 512);
+    else fail(MMH_ERR_OTHER, "linear_cross_entropy: rows of " + std::to_string(v) + " logits without partials");
+    check_hip(hipGetLastError(), "loss launch");
+}
+
+// dz in place of wider rows, whose product left (max, sum) per 128 columns beside
+// the logits (EPI_CE_STORE). A workgroup has a chunk of a row: it merges the row's partials
+// (at most a few KB, read by each of the row's workgroups), then its columns pass
+// through once. Bound by the logits' read and write.
+__global__ __launch_bounds__(256) void loss_grad_kernel(float *z, const float2 *part,
+                                                        const int32_t *targets, int64_t ld, int64_t v,
+                                                        int64_t units, int64_t chunk, float scale,
+                                                        float *row_loss) {
+    __shared__ float red_m[4], red_s[4];
+    const int64_t row = blockIdx.x, q0 = blockIdx.y * (chunk / 4);
+    float4 *z4 = reinterpret_cast<float4 *>(z + row * ld);
+    const int32_t t = targets[row];
+    const bool has_t = t / chunk == (int64_t)blockIdx.y;
+    const float zt = has_t ? z[row * ld + t] : 0.0f;
+    float m = -INFINITY, s = 0.0f;
+    for (int64_t j = threadIdx.x; j < units; j += 256) {
+        const float2 a = part[row * units + j];
+        lse_merge(m, s, a.x, a.y);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(m, off, 64), s2 = __shfl_xor(s, off, 64);
+        lse_merge(m, s, m2, s2);
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        red_m[wave] = m;
+        red_s[wave] = s;
+    }
     __syncthreads();  // (z[target] has been read by every thread, too)
-    s = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
-    if (threadIdx.x == 0) row_loss[row] = (m + logf(s)) - zt;
-    if (!GRAD) return;
+    m = red_m[0];
+    s = red_s[0];
+    for (int i = 1; i < 4; ++i) lse_merge(m, s, red_m[i], red_s[i]);
+    if (has_t && threadIdx.x == 0) row_loss[row] = (m + logf(s)) - zt;
+    const float f = __fdiv_rn(scale, s);
     auto grad = [&](float x, int64_t j) {
-        const float d = __fdiv_rn(expf(x - m), s) * scale;
+        const float d = exp_neg(x - m) * f;
         return j == t ? d - scale : d;
     };
-    for (int64_t q = threadIdx.x; q < v4; q += 256) {
-        float4 a = load(q);
+    const int64_t q1 = min((v + 3) / 4, q0 + chunk / 4);
+    for (int64_t q = q0 + threadIdx.x; q < q1; q += 256) {
+        float4 a = z4[q];  // (columns past v are padding of the row)
         a.x = grad(a.x, 4 * q);
         a.y = grad(a.y, 4 * q + 1);
         a.z = grad(a.z, 4 * q + 2);
@@ -99,12 +179,17 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(float *z, const int32_t 
     }
 }
 
-template <bool GRAD>
-void launch_loss_rows(Context &cx, float *z, const int32_t *targets, int64_t rows, int64_t ld, int64_t v,
-                      float scale, float *row_loss) {
-    hipLaunchKernelGGL(loss_rows_kernel<GRAD>, dim3((unsigned)rows), dim3(256), 0, cx.stream, z, targets,
-                       ld, v, scale, row_loss);
-    check_hip(hipGetLastError(), "loss launch");
+// Columns of a workgroup of loss_grad_kernel: whole rows where there are eight
+// workgroups per CU of them, else parts of 8192 columns at least (a grid has at
+// most 65535 in y).
+int64_t grad_chunk(const Context &cx, int64_t rows, int64_t v) {
+    const int64_t parts = std::max<int64_t>(1, std::min((8 * (int64_t)cx.cu_count + rows - 1) / rows, (v + 8191) / 8192));
+    return std::max((v + parts - 1) / parts, v / 65535 + 1) / 4 * 4 + 4;
+}
+
+__global__ __launch_bounds__(256) void copy_ids_kernel(const int32_t *host, int64_t n, int32_t *dev) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) dev[i] = host[i];
 }
 
 // Floats of a row of stored logits: whole float4s, for the products too.
@@ -114,9 +199,8 @@ int64_t logit_row(int64_t vocab) { return (vocab + 31) / 32 * 32; }
 struct Rows {
     int64_t kept = 0;
     const float *x = nullptr;          // [kept, d]
-    const int32_t *targets = nullptr;  // device, [kept]
+    const int32_t *targets = nullptr;  // [kept], where kernels read them
     const int32_t *map = nullptr;      // device, [n]: a row's place among the kept ones, or -1; null: all are kept
-    std::vector<int32_t> host;         // what the upload reads
 };
 
 struct Head {
@@ -144,30 +228,35 @@ void check_head(const Head &h) {
                                     " is out of range for " + std::to_string(h.vocab));
 }
 
-// Uploads the targets; with ignored rows also the kept rows' indexes and the
-// map back, and packs those rows of x into `packed`.
-void stage_rows(Context &cx, const Head &h, float *packed, Rows &r) {
-    const int64_t pad = (h.n + 63) / 64 * 64;
-    int32_t *dev = static_cast<int32_t *>(cx.workspace(1, (size_t)(3 * pad) * 4));
-    r.targets = dev;
+// The targets into pinned memory, which the kernels that read a row's target
+// once take them from; into device memory for the product that reads them in
+// every tile (`device`), and with ignored rows, where the kept rows' indexes and
+// the map back go along and those rows of x are packed.
+void stage_rows(Context &cx, const Head &h, bool device, float *packed, Rows &r) {
+    const int64_t pad = (h.n + 63) / 64 * 64, total = r.kept == h.n ? h.n : 3 * pad;
+    int32_t *t = static_cast<int32_t *>(cx.pinned_ids((size_t)total * 4));
+    r.x = h.x;
     if (r.kept == h.n) {
-        check_hip(hipMemcpyAsync(dev, h.targets, (size_t)h.n * 4, hipMemcpyHostToDevice, cx.stream),
-                  "targets upload");
-        r.x = h.x;
-        return;
+        std::copy(h.targets, h.targets + h.n, t);
+        r.targets = t;
+        if (!device) return;
+    } else {
+        int32_t *index = t + pad, *map = index + pad, at = 0;
+        std::fill(t, t + total, 0);
+        for (int64_t i = 0; i < h.n; ++i) {
+            const bool keep = h.targets[i] != h.ignore;
+            map[i] = keep ? at : -1;
+            if (!keep) continue;
+            t[at] = h.targets[i];
+            index[at++] = (int32_t)i;
+        }
     }
-    r.host.assign((size_t)(3 * pad), 0);
-    int32_t *t = r.host.data(), *index = t + pad, *map = index + pad;
-    int32_t at = 0;
-    for (int64_t i = 0; i < h.n; ++i) {
-        const bool keep = h.targets[i] != h.ignore;
-        map[i] = keep ? at : -1;
-        if (!keep) continue;
-        t[at] = h.targets[i];
-        index[at++] = (int32_t)i;
-    }
-    check_hip(hipMemcpyAsync(dev, t, (size_t)(3 * pad) * 4, hipMemcpyHostToDevice, cx.stream),
-              "targets upload");
+    int32_t *dev = static_cast<int32_t *>(cx.workspace(1, (size_t)total * 4));
+    r.targets = dev;
+    hipLaunchKernelGGL(copy_ids_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, cx.stream, t,
+                       total, dev);
+    check_hip(hipGetLastError(), "targets launch");
+    if (r.kept == h.n) return;
     r.map = dev + 2 * pad;
     launch_embedding(cx, h.x, h.d, dev + pad, r.kept, packed);
     r.x = packed;
@@ -214,7 +303,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
     const size_t part = round64(std::max(floats(block), floats((r.kept - 1) % block + 1)));
     float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block)) * 4));
     float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
-    stage_rows(cx, h, ws, r);
+    stage_rows(cx, h, true, ws, r);
     float *buf = ws + packed, *zt = buf + part;
     for (int64_t at = 0; at < r.kept; at += block) {
         const int64_t rows = std::min(block, r.kept - at);
@@ -247,21 +336,35 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
         return;
     }
     const bool all = r.kept == h.n, nt = h.form == MMH_GEMM_NT;
+    const int64_t units = (h.vocab + 127) / 128;
     const int64_t ld = logit_row(h.vocab), block = block_rows(r.kept, ld * 4);
     const size_t packed = all ? 0 : round64(r.kept * h.d);
     float *ws = static_cast<float *>(
-        cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld)) * 4));
+        cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2)) * 4));
     float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
-    stage_rows(cx, h, ws, r);
-    float *z = ws + packed, *dxk = all ? dx : z + round64(block * ld);
+    stage_rows(cx, h, false, ws, r);
+    float *z = ws + packed, *part = z + round64(block * ld);
+    float *dxk = all ? dx : part + round64(block * units * 2);
     const float scale = 1.0f / (float)r.kept;
     for (int64_t at = 0; at < r.kept; at += block) {
         const int64_t rows = std::min(block, r.kept - at);
         GemmDesc g = head_product(h, r.x + at * h.d, rows);
         g.c = z;
         g.ldc = ld;
-        gemm(cx, g);
-        launch_loss_rows<true>(cx, z, r.targets + at, rows, ld, h.vocab, scale, row_loss + at);
+        if (h.vocab > kRowCols) {
+            g.epi = EPI_CE_STORE;
+            g.ce_part = part;
+            gemm(cx, g);
+            const int64_t chunk = grad_chunk(cx, rows, h.vocab);
+            const dim3 grid((unsigned)rows, (unsigned)((h.vocab + chunk - 1) / chunk));
+            hipLaunchKernelGGL(loss_grad_kernel, grid, dim3(256), 0, cx.stream, z,
+                               reinterpret_cast<const float2 *>(part), r.targets + at, ld, h.vocab, units,
+                               chunk, scale, row_loss + at);
+            check_hip(hipGetLastError(), "loss gradient launch");
+        } else {
+            gemm(cx, g);
+            launch_loss_rows<true>(cx, z, r.targets + at, rows, ld, h.vocab, scale, row_loss + at);
+        }
         if (dx) {  // dz [rows, vocab] . op(W)^T
             GemmDesc p;
             p.a = z;
@@ -300,8 +403,8 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     if (loss_host) {
         launch_mean(cx, row_loss, r.kept, cx.words);
         finish_loss(cx, loss_host);
-    } else {  // the upload has read the targets
-        check_hip(hipStreamSynchronize(cx.stream), "targets upload sync");
+    } else {  // the pinned targets have been read
+        check_hip(hipStreamSynchronize(cx.stream), "targets sync");
     }
 }
 

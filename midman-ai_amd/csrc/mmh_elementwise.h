@@ -20,7 +20,7 @@ __device__ __forceinline__ float reciprocal(float d) {
 // exp(x), x <= 0: 2^(x log2 e), the low part of the exponent applied as 1 + low ln 2.
 __device__ __forceinline__ float exp_neg(float x) {
     constexpr float kHi = 1.44269502f, kLo = 1.92596303e-8f, kLn2 = 0.69314718f;
-    x = fmaxf(x, -104.0f);  // (e^-104 is below the smallest f32)
+    x = x < -104.0f ? -104.0f : x;  // (e^-104 is below the smallest f32; a NaN stays)
     const float t = x * kHi;
     const float low = __builtin_fmaf(x, kLo, __builtin_fmaf(x, kHi, -t));
     const float e = __builtin_amdgcn_exp2f(t);

@@ -86,6 +86,11 @@ struct Context {
     int32_t *tickets = nullptr;
     // Two words of pinned host memory for results read back (one thread per context).
     float *words = nullptr;
+    // Pinned host memory for ids on their way to the device. Growing it waits for
+    // queued work; a call that fills it waits for its kernels before it returns.
+    void *pinned = nullptr;
+    size_t pinned_bytes = 0;
+    void *pinned_ids(size_t bytes);
     // Allocations made through mmh_alloc, freed at destroy.
     std::vector<void *> owned;
 
@@ -117,10 +122,11 @@ void release_models_of(mmh_handle ctx);
 // exp(z - max)) over its columns, and the tile holding column ce_targets[i]
 // leaves that logit in ce_zt[i] (the head GEMM with the loss folded in; see
 // gemm_ce_tiles and launch_ce_combine).
+// EPI_CE_STORE: the partials, and the logits in C (no targets).
 // EPI_LINEAR (batch 1, nn and nt): C is not written; the products go through
 // `tail` (bias, activation, dropout, residual) into tail->out.
 enum Epilogue : int { EPI_STORE = 0, EPI_ACCUM = 1, EPI_SWIGLU = 2, EPI_SWIGLU_BWD = 3,
-                      EPI_CE = 4, EPI_LINEAR = 5 };
+                      EPI_CE = 4, EPI_LINEAR = 5, EPI_CE_STORE = 6 };
 struct LinearTail;  // mmh_elementwise.h
 
 // mmh_gemm_noalloc: the partials of the plan its contract is stated in, and the

@@ -45,6 +45,21 @@ void *Context::workspace(int slot, size_t bytes) {
     return ws[slot];
 }
 
+void *Context::pinned_ids(size_t bytes) {
+    if (bytes > pinned_bytes) {
+        if (pinned) {
+            check_hip(hipStreamSynchronize(stream), "pinned sync");
+            check_hip(hipHostFree(pinned), "pinned free");
+            pinned = nullptr;
+            pinned_bytes = 0;
+        }
+        const size_t rounded = (bytes + 65535) & ~size_t(65535);
+        check_hip(hipHostMalloc(&pinned, rounded, hipHostMallocDefault), "pinned alloc");
+        pinned_bytes = rounded;
+    }
+    return pinned;
+}
+
 int32_t *Context::stage_ids(const int32_t *host, int64_t n, int which) {
     // Two halves of slot 1: inputs at 0, targets after them.
     const size_t half = ((size_t)n * 4 + 255) & ~size_t(255);
@@ -132,6 +147,7 @@ int32_t mmh_context_destroy(mmh_handle ctx) {
             if (c->ws[s]) (void)hipFree(c->ws[s]);
         if (c->tickets) (void)hipFree(c->tickets);
         if (c->words) (void)hipHostFree(c->words);
+        if (c->pinned) (void)hipHostFree(c->pinned);
         (void)hipEventDestroy(c->t0);
         (void)hipEventDestroy(c->t1);
         (void)hipStreamDestroy(c->stream);

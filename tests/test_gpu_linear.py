@@ -374,12 +374,12 @@ def test_far_logits_and_special_rows(ctx):
 
 def test_row_blocks(ctx):
     """More logits than the workspace holds: blocks of rows, the last a smaller one, gradients added up over blocks."""
-    for n, d, V, share in ((1100, 16, 64003, 0.0), (600, 24, 131072, 0.02)):
+    for n, d, V, share in ((1100, 16, 64003, 0.0), (2300, 12, 64003, 0.02)):
         print(f"\n[row blocks] {n} {d} {V}", flush=True)
         x, w, t = head(n, d, V, seed=n)
         t[np.random.default_rng(1).random(n) < share] = -1
         got = run_loss(ctx, 1, x, w, t)
-        want = R.cross_entropy(x, w, t, blocks=8)
+        want = R.cross_entropy(x, w, t, blocks=2)
         check_loss(got, want, f"{n}: ")
 
 
