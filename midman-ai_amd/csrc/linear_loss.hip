@@ -19,9 +19,17 @@
 namespace mmh {
 namespace {
 
-// The workspace of a block's logits, and the rows that a block has at least.
+// The workspace of a block's logits, and the rows that a block has at least. Twice
+// as large as 256 MiB, since a block's last tiles of rows and what its part adds to
+// dW are paid per block: 817 rows x 1024 x 131071 4510 -> 4020 us, 4096 x 2048 x
+// 32000 7585 -> 7445.
 constexpr int64_t kLogitBytes = int64_t(512) << 20;
 constexpr int64_t kMinRows = 128;
+// Up to so many rows the loss takes stored logits: the tiles that fold it have
+// 128 rows at least, those of the plain product 32 or 64 (35 rows x 1344 x 153411
+// 367 -> 266 us for the product, 64 rows 372 -> 274, 128 rows 384 -> 341 and 33
+// for the stored logits' two ways).
+constexpr int64_t kFewRows = 64;
 
 int64_t block_rows(int64_t n, int64_t row_bytes) {
     int64_t rows = std::max(kMinRows, kLogitBytes / row_bytes);
@@ -129,6 +137,50 @@ void launch_loss_rows(Context &cx, float *z, const int32_t *targets, int64_t row
     check_hip(hipGetLastError(), "loss launch");
 }
 
+// The (max, sum) of each kPartCols columns of stored logits, and the target's
+// logit: the partials of wider rows where there are too few of them for the
+// product's tiles to leave any (kFewRows). A workgroup has a row's piece in registers.
+constexpr int64_t kPartCols = 8192;
+__global__ __launch_bounds__(256) void loss_parts_kernel(const float *z, const int32_t *targets, int64_t ld,
+                                                         int64_t v, int64_t units, float2 *part, float *zt) {
+    __shared__ float red_m[4], red_s[4];
+    const int64_t row = blockIdx.y, unit = blockIdx.x, c0 = unit * kPartCols;
+    const float4 *z4 = reinterpret_cast<const float4 *>(z + row * ld + c0);
+    const int tid = threadIdx.x, wave = tid >> 6, n = (int)min(v - c0, kPartCols);
+    const int64_t t = targets[row] - c0;
+    float4 e[8];
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int q = tid + 256 * i;
+        e[i] = z4[min(q, (n + 3) / 4 - 1)];
+        if (4 * q >= n) e[i].x = -INFINITY;
+        if (4 * q + 1 >= n) e[i].y = -INFINITY;
+        if (4 * q + 2 >= n) e[i].z = -INFINITY;
+        if (4 * q + 3 >= n) e[i].w = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fmaxf(e[i].x, e[i].y), fmaxf(e[i].z, e[i].w)));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    if ((tid & 63) == 0) red_m[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    const float m0 = m == -INFINITY ? 0.0f : m;  // (then every exponential is 0, or NaN)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        s += (exp_neg(e[i].x - m0) + exp_neg(e[i].y - m0)) + (exp_neg(e[i].z - m0) + exp_neg(e[i].w - m0));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if ((tid & 63) == 0) red_s[wave] = s;
+    __syncthreads();
+    if (tid != 0) return;
+    s = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
+    // a NaN sum keeps its place beside any maximum (a piece of -inf and NaN has no other)
+    part[row * units + unit] = make_float2(s != s ? s : m, s);
+    if (t >= 0 && t < n) zt[row] = z[row * ld + c0 + t];
+}
+
 // dz in place of wider rows, whose product left (max, sum) per 128 columns beside
 // the logits (EPI_CE_STORE). A workgroup has a chunk of a row: it merges the row's partials
 // (at most a few KB, read by each of the row's workgroups), then its columns pass
@@ -185,6 +237,16 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(float *z, const float2 *
 int64_t grad_chunk(const Context &cx, int64_t rows, int64_t v) {
     const int64_t parts = std::max<int64_t>(1, std::min((8 * (int64_t)cx.cu_count + rows - 1) / rows, (v + 8191) / 8192));
     return std::max((v + parts - 1) / parts, v / 65535 + 1) / 4 * 4 + 4;
+}
+
+int64_t part_units(int64_t v) { return (v + kPartCols - 1) / kPartCols; }
+
+void launch_loss_parts(Context &cx, const float *z, const int32_t *targets, int64_t rows, int64_t ld,
+                       int64_t v, float *part, float *zt) {
+    const int64_t units = part_units(v);
+    hipLaunchKernelGGL(loss_parts_kernel, dim3((unsigned)units, (unsigned)rows), dim3(256), 0, cx.stream, z,
+                       targets, ld, v, units, reinterpret_cast<float2 *>(part), zt);
+    check_hip(hipGetLastError(), "loss partials launch");
 }
 
 __global__ __launch_bounds__(256) void copy_ids_kernel(const int32_t *host, int64_t n, int32_t *dev) {
@@ -294,17 +356,21 @@ void forward(Context &cx, const Head &h, float *loss_host) {
         return;
     }
     const int64_t units = (h.vocab + 127) / 128;
-    auto folds = [&](int64_t rows) { return gemm_ce_tiles(cx, head_product(h, h.x, rows)) > 0; };
+    // (more columns than kRowCols always fill the tiles that fold the loss)
+    auto folds = [&](int64_t rows) {
+        return rows > kFewRows && (h.vocab > kRowCols || gemm_ce_tiles(cx, head_product(h, h.x, rows)) > 0);
+    };
     const int64_t ld = logit_row(h.vocab);
     const int64_t block = block_rows(r.kept, folds(r.kept) ? units * 8 : ld * 4);
     // a block's partials, or the logits of one too small for the product to fold them (the last, often)
     auto floats = [&](int64_t rows) { return rows * (folds(rows) ? units * 2 : ld); };
     const size_t packed = r.kept < h.n ? round64(r.kept * h.d) : 0;
     const size_t part = round64(std::max(floats(block), floats((r.kept - 1) % block + 1)));
-    float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block)) * 4));
+    const size_t parts_floats = round64(2 * kFewRows * part_units(h.vocab));
+    float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block) + parts_floats) * 4));
     float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
-    stage_rows(cx, h, true, ws, r);
-    float *buf = ws + packed, *zt = buf + part;
+    stage_rows(cx, h, folds(block), ws, r);
+    float *buf = ws + packed, *zt = buf + part, *stats = zt + round64(block);
     for (int64_t at = 0; at < r.kept; at += block) {
         const int64_t rows = std::min(block, r.kept - at);
         GemmDesc g = head_product(h, r.x + at * h.d, rows);
@@ -319,7 +385,13 @@ void forward(Context &cx, const Head &h, float *loss_host) {
             g.c = buf;
             g.ldc = ld;
             gemm(cx, g);
-            launch_loss_rows<false>(cx, buf, r.targets + at, rows, ld, h.vocab, 0.0f, row_loss + at);
+            if (h.vocab <= kRowCols) {
+                launch_loss_rows<false>(cx, buf, r.targets + at, rows, ld, h.vocab, 0.0f, row_loss + at);
+            } else {
+                const int64_t parts = part_units(h.vocab);
+                launch_loss_parts(cx, buf, r.targets + at, rows, ld, h.vocab, stats, zt);
+                launch_ce_combine_rows(cx, stats, parts, zt, rows, row_loss + at);
+            }
         }
     }
     launch_mean(cx, row_loss, r.kept, cx.words);
@@ -340,11 +412,11 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     const int64_t ld = logit_row(h.vocab), block = block_rows(r.kept, ld * 4);
     const size_t packed = all ? 0 : round64(r.kept * h.d);
     float *ws = static_cast<float *>(
-        cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2)) * 4));
+        cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2) + kFewRows) * 4));
     float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
     stage_rows(cx, h, false, ws, r);
     float *z = ws + packed, *part = z + round64(block * ld);
-    float *dxk = all ? dx : part + round64(block * units * 2);
+    float *zt = part + round64(block * units * 2), *dxk = all ? dx : zt + kFewRows;
     const float scale = 1.0f / (float)r.kept;
     for (int64_t at = 0; at < r.kept; at += block) {
         const int64_t rows = std::min(block, r.kept - at);
@@ -352,13 +424,20 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
         g.c = z;
         g.ldc = ld;
         if (h.vocab > kRowCols) {
-            g.epi = EPI_CE_STORE;
-            g.ce_part = part;
-            gemm(cx, g);
+            int64_t stats = units;
+            if (rows > kFewRows) {
+                g.epi = EPI_CE_STORE;
+                g.ce_part = part;
+                gemm(cx, g);
+            } else {
+                stats = part_units(h.vocab);
+                gemm(cx, g);
+                launch_loss_parts(cx, z, r.targets + at, rows, ld, h.vocab, part, zt);
+            }
             const int64_t chunk = grad_chunk(cx, rows, h.vocab);
             const dim3 grid((unsigned)rows, (unsigned)((h.vocab + chunk - 1) / chunk));
             hipLaunchKernelGGL(loss_grad_kernel, grid, dim3(256), 0, cx.stream, z,
-                               reinterpret_cast<const float2 *>(part), r.targets + at, ld, h.vocab, units,
+                               reinterpret_cast<const float2 *>(part), r.targets + at, ld, h.vocab, stats,
                                chunk, scale, row_loss + at);
             check_hip(hipGetLastError(), "loss gradient launch");
         } else {

@@ -289,7 +289,7 @@ def run_loss(ctx, form, x, w, targets, ignore=-1, grads=("dx", "dw"), shift=0, l
 # (n, d, vocab): stored logits of small products and folded ones of large tiles; a vocabulary of one, of less than a unit
 # of 128 columns, odd ones, wider than a row's registers
 HEADS = [(1, 1, 1), (1, 7, 2), (3, 16, 65), (24, 16, 12), (5, 33, 129), (130, 64, 256), (257, 48, 1001), (64, 300, 4099),
-         (2048, 128, 4096), (1021, 770, 5003), (33, 40, 32769), (129, 24, 70001), (4100, 31, 2050), (1, 512, 40000)]
+         (2048, 128, 4096), (1021, 770, 5003), (33, 40, 32769), (129, 24, 70001), (4100, 31, 2050), (1, 512, 40000), (64, 48, 131072), (65, 48, 32768), (40, 20, 8192)]
 
 
 def head(n, d, V, seed, sharp=1.0):
@@ -363,7 +363,7 @@ def test_far_logits_and_special_rows(ctx):
     rest = np.arange(300) != 17
     near(got["dx"][rest], want["dx"][0][rest], want["dx"][1][rest], "dx")
     # a NaN in a lone column, the first, one inside, the last (alone in its unit of 128, at 4097), that is no row's target
-    for V, d, n in ((515, 64, 300), (4097, 64, 1200)):
+    for V, d, n in ((515, 64, 300), (4097, 64, 1200), (40001, 24, 40), (40001, 24, 100)):
         for at in (0, 77, V - 1):
             x, w, t = head(n, d, V, seed=9)
             t[t == at] = 1
