@@ -929,13 +929,12 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
                 const float mx = half_max32(fmaxf(x0, x1));
                 // exp(z - max) through the hardware's exp2 (no flush concern: the
                 // terms that matter are within a few hundred of 1) or libm_exp
-                float e = 0.0f;
-                if (mx != -INFINITY)
-                    e = p.libm_exp ? expf(x0 - mx) + expf(x1 - mx)
-                                   : __builtin_amdgcn_exp2f((x0 - mx) * kLog2e) +
-                                         __builtin_amdgcn_exp2f((x1 - mx) * kLog2e);
-                else if (x0 != x0 || x1 != x1)
-                    e = __builtin_nanf("");  // (the maximum passes over a NaN)
+                // (a floor under the maximum: -inf alone leaves 0, and a NaN, which the
+                // maximum passes over, stays one in the sum)
+                const float top = fmaxf(mx, -3.402823466e38f);
+                float e = p.libm_exp ? expf(x0 - top) + expf(x1 - top)
+                                     : __builtin_amdgcn_exp2f((x0 - top) * kLog2e) +
+                                           __builtin_amdgcn_exp2f((x1 - top) * kLog2e);
                 e = half_sum32(e);
                 if (lr == 0) {
                     ce_m[wn][rl] = e != e ? e : mx;
