@@ -1137,7 +1137,7 @@ constexpr int kMaxTileSplits = 16;
 // x 3763 57 / 51, 2142 x 90 x 1728 27 / 16). Over 260 products of K 33 to 4096 the
 // choice is 0.9% from the best tile of each, 2.9% with 6 for all. (even: 6 for all.)
 TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int epi, int first,
-                      bool even) {
+                      bool even, int64_t split_bytes) {
     const bool may_split = batch == 1 && (epi == EPI_STORE || epi == EPI_ACCUM || epi == EPI_LINEAR) &&
                            !p.rope_cos;
     const double cus = cus_of(ctx), ksteps = (double)((p.k + BK - 1) / BK);
@@ -1150,7 +1150,7 @@ TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int e
                              (double)((p.n + t.cols - 1) / t.cols) * (double)batch;
         for (int s = 1; s <= kMaxTileSplits; ++s) {
             // a split keeps 128 of K, as many as its prologue costs
-            if (s > 1 && (!may_split || p.k < 128 * s || s * p.m * p.n * 4 > kSplitBytes)) break;
+            if (s > 1 && (!may_split || p.k < 128 * s || s * p.m * p.n * 4 > split_bytes)) break;
             const double g = tiles * s, setup = even ? 6.0 : t.setup;
             double us = std::max(std::ceil(g / cus) * t.alone, g / cus * t.full) * (ksteps / s + setup);
             if (s > 1) us += 4.0 + (double)(s + 1) * (double)(p.m * p.n) * 4.0 / 3.5e6;
@@ -1170,11 +1170,13 @@ TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int e
 // taken where its steps win, not for its setup: the products of 92 to 480 of K that
 // the setups alone would move to it gain 4-18% over 256x128 and lose a factor of
 // 2.8 in precision.
-TilePlan choose_tile(const Context &ctx, const KParams &p, int64_t batch, int epi) {
-    const TilePlan best = fastest_tile(ctx, p, batch, epi, TILE_256, false);
-    if (best.tile != TILE_256 || fastest_tile(ctx, p, batch, epi, TILE_256, true).tile == TILE_256)
+TilePlan choose_tile(const Context &ctx, const KParams &p, int64_t batch, int epi,
+                     int64_t split_bytes) {
+    const TilePlan best = fastest_tile(ctx, p, batch, epi, TILE_256, false, split_bytes);
+    if (best.tile != TILE_256 ||
+        fastest_tile(ctx, p, batch, epi, TILE_256, true, split_bytes).tile == TILE_256)
         return best;
-    return fastest_tile(ctx, p, batch, epi, TILE_256x128, false);
+    return fastest_tile(ctx, p, batch, epi, TILE_256x128, false, split_bytes);
 }
 
 // mmh_gemm_noalloc's contract: which products it takes is stated in terms of a
@@ -1329,7 +1331,7 @@ void gemm(Context &ctx, const GemmDesc &d) {
     }
 
     TilePlan plan;
-    if (tiled) plan = choose_tile(ctx, p, d.batch, d.epi);
+    if (tiled) plan = choose_tile(ctx, p, d.batch, d.epi, d.split_bytes ? d.split_bytes : kSplitBytes);
     const int64_t tile_m = ksplit ? 32 : tiled ? kGemmTiles[plan.tile].rows : SBM;
     const int64_t tile_n = ksplit ? 32 : tiled ? kGemmTiles[plan.tile].cols : SBN;
     p.tiles_m = (int)((d.m + tile_m - 1) / tile_m);

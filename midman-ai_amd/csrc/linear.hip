@@ -119,10 +119,12 @@ __global__ __launch_bounds__(256) void linear_dpre_kernel(const float *dout, con
     }
 }
 
-// Strips of rows for about four workgroups per CU, 16 rows at least.
+// Strips of rows for about four workgroups per CU, of 16 rows at least and 1024 at
+// most (a lane then adds 256 values one after another, and the strips' sums follow
+// in 16 chains: the bias gradient of 2^21 rows rounds about 400 times).
 int64_t strip_rows(const Context &ctx, int64_t rows, int64_t n) {
     const int64_t cols = (n + 255) / 256, want = std::max<int64_t>(1, 4 * (int64_t)ctx.cu_count / cols);
-    const int64_t strip = std::max<int64_t>(16, (rows + want - 1) / want);
+    const int64_t strip = std::min<int64_t>(1024, std::max<int64_t>(16, (rows + want - 1) / want));
     return std::max(strip, (rows + 65534) / 65535);  // (a grid's y)
 }
 
@@ -153,6 +155,7 @@ void product(Context &cx, const float *a, bool ta, const float *b, bool tb, floa
     g.m = m;
     g.k = k;
     g.n = n;
+    g.split_bytes = kTrainSplitBytes;
     if (tail) {
         g.epi = EPI_LINEAR;
         g.tail = tail;
@@ -249,9 +252,10 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
         if (changes || dbias) {
             const int64_t strip = strip_rows(cx, rows, n), strips = (rows + strip - 1) / strip;
             const size_t values = changes ? ((size_t)(rows * n) + 63) / 64 * 64 : 0;
+            const bool several = dbias && strips > 1;
             float *buf = static_cast<float *>(
-                cx.workspace(2, (values + (dbias ? (size_t)(strips * n) : 0)) * 4));
-            float *sums = dbias ? buf + values : nullptr;
+                cx.workspace(2, (values + (several ? (size_t)(strips * n) : 0)) * 4));
+            float *sums = several ? buf + values : dbias;
             const dim3 grid((unsigned)((n + 255) / 256), (unsigned)strips);
             if (changes) {
                 hipLaunchKernelGGL(linear_dpre_kernel<true>, grid, dim3(256), 0, cx.stream, dout, pre, rows,
@@ -262,7 +266,7 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
                                    n, strip, activation, d, nullptr, sums);
             }
             check_hip(hipGetLastError(), "linear dpre launch");
-            if (dbias) launch_sum_rows(cx, sums, strips, n, dbias);
+            if (several) launch_sum_rows(cx, sums, strips, n, dbias);
         }
         if (dx) product(cx, dpre, false, w, !nt, dx, rows, n, k);
         if (dw && !nt) product(cx, x, true, dpre, false, dw, k, rows, n);

@@ -30,6 +30,20 @@ constexpr int64_t kMinRows = 128;
 // 367 -> 266 us for the product, 64 rows 372 -> 274, 128 rows 384 -> 341 and 33
 // for the stored logits' two ways).
 constexpr int64_t kFewRows = 64;
+// So few rows past a block's last whole 256 are a part of their own beside
+// weights of kTailWeights values or more: in the tiles of 256 rows they would cost
+// a whole one, and they read W again for less (817 rows x 1024 x 131071 4000 ->
+// 3780 us, 545 x 2048 x 32000 1480 -> 1307, 1044 x 4096 x 16000 2330 -> 2065;
+// with fewer weights the further launches take that back: 320 x 1024 x 40000 617 ->
+// 621, the loss alone of 1044 x 768 x 50000 521 -> 565).
+constexpr int64_t kTailWeights = int64_t(52) << 20;
+
+// The rows of the part of a block that starts at `at` of its `rows`.
+int64_t part_rows(int64_t rows, int64_t at, int64_t weights) {
+    const int64_t tail = rows % 256;
+    if (at > 0 || rows < 256 || tail > kFewRows || weights < kTailWeights) return rows - at;
+    return rows - tail;
+}
 
 int64_t block_rows(int64_t n, int64_t row_bytes) {
     int64_t rows = std::max(kMinRows, kLogitBytes / row_bytes);
@@ -338,6 +352,7 @@ GemmDesc head_product(const Head &h, const float *x, int64_t rows) {
     g.lda = h.d;
     g.tb = h.form == MMH_GEMM_NT;
     g.ldb = g.tb ? h.d : h.vocab;
+    g.split_bytes = kTrainSplitBytes;
     return g;
 }
 
@@ -364,15 +379,19 @@ void forward(Context &cx, const Head &h, float *loss_host) {
     const int64_t block = block_rows(r.kept, folds(r.kept) ? units * 8 : ld * 4);
     // a block's partials, or the logits of one too small for the product to fold them (the last, often)
     auto floats = [&](int64_t rows) { return rows * (folds(rows) ? units * 2 : ld); };
+    const int64_t weights = h.d * h.vocab, last = (r.kept - 1) % block + 1;
+    int64_t most = 0;
+    for (int64_t rows : {block, last})
+        for (int64_t at = 0, n; at < rows; at += n) most = std::max(most, floats(n = part_rows(rows, at, weights)));
     const size_t packed = r.kept < h.n ? round64(r.kept * h.d) : 0;
-    const size_t part = round64(std::max(floats(block), floats((r.kept - 1) % block + 1)));
+    const size_t part = round64(most);
     const size_t parts_floats = round64(2 * kFewRows * part_units(h.vocab));
     float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block) + parts_floats) * 4));
     float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
     stage_rows(cx, h, folds(block), ws, r);
     float *buf = ws + packed, *zt = buf + part, *stats = zt + round64(block);
-    for (int64_t at = 0; at < r.kept; at += block) {
-        const int64_t rows = std::min(block, r.kept - at);
+    for (int64_t at = 0, rows; at < r.kept; at += rows) {
+        rows = part_rows(std::min(block, r.kept - at / block * block), at % block, weights);
         GemmDesc g = head_product(h, r.x + at * h.d, rows);
         if (folds(rows)) {
             g.epi = EPI_CE;
@@ -418,10 +437,10 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     float *z = ws + packed, *part = z + round64(block * ld);
     float *zt = part + round64(block * units * 2), *dxk = all ? dx : zt + kFewRows;
     const float scale = 1.0f / (float)r.kept;
-    for (int64_t at = 0; at < r.kept; at += block) {
-        const int64_t rows = std::min(block, r.kept - at);
+    // dz of the rows at .. at + rows in z, and their dx
+    auto logits = [&](float *zp, int64_t at, int64_t rows) {
         GemmDesc g = head_product(h, r.x + at * h.d, rows);
-        g.c = z;
+        g.c = zp;
         g.ldc = ld;
         if (h.vocab > kRowCols) {
             int64_t stats = units;
@@ -432,21 +451,21 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
             } else {
                 stats = part_units(h.vocab);
                 gemm(cx, g);
-                launch_loss_parts(cx, z, r.targets + at, rows, ld, h.vocab, part, zt);
+                launch_loss_parts(cx, zp, r.targets + at, rows, ld, h.vocab, part, zt);
             }
             const int64_t chunk = grad_chunk(cx, rows, h.vocab);
             const dim3 grid((unsigned)rows, (unsigned)((h.vocab + chunk - 1) / chunk));
-            hipLaunchKernelGGL(loss_grad_kernel, grid, dim3(256), 0, cx.stream, z,
+            hipLaunchKernelGGL(loss_grad_kernel, grid, dim3(256), 0, cx.stream, zp,
                                reinterpret_cast<const float2 *>(part), r.targets + at, ld, h.vocab, stats,
                                chunk, scale, row_loss + at);
             check_hip(hipGetLastError(), "loss gradient launch");
         } else {
             gemm(cx, g);
-            launch_loss_rows<true>(cx, z, r.targets + at, rows, ld, h.vocab, scale, row_loss + at);
+            launch_loss_rows<true>(cx, zp, r.targets + at, rows, ld, h.vocab, scale, row_loss + at);
         }
         if (dx) {  // dz [rows, vocab] . op(W)^T
             GemmDesc p;
-            p.a = z;
+            p.a = zp;
             p.b = h.w;
             p.c = dxk + at * h.d;
             p.m = rows;
@@ -456,7 +475,15 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
             p.tb = !nt;
             p.ldb = nt ? h.d : h.vocab;
             p.ldc = h.d;
+            p.split_bytes = kTrainSplitBytes;
             gemm(cx, p);
+        }
+    };
+    for (int64_t at = 0; at < r.kept; at += block) {
+        const int64_t rows = std::min(block, r.kept - at);
+        for (int64_t sub = 0, n; sub < rows; sub += n) {
+            n = part_rows(rows, sub, h.d * h.vocab);
+            logits(z + sub * ld, at + sub, n);
         }
         if (dw) {  // x^T dz [d, vocab], or dz^T x [vocab, d]; later blocks are added
             GemmDesc p;
@@ -470,6 +497,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
             p.lda = nt ? ld : h.d;
             p.ldb = nt ? h.d : ld;
             p.ldc = p.n;
+            p.split_bytes = kTrainSplitBytes;
             p.epi = at ? EPI_ACCUM : EPI_STORE;
             gemm(cx, p);
         }

@@ -134,6 +134,11 @@ struct LinearTail;  // mmh_elementwise.h
 constexpr int64_t kNoallocLimitBytes = int64_t(16) << 20;
 constexpr int64_t kNoallocScratchBytes = int64_t(64) << 20;
 
+// What the training operators' products may take: outputs of 129 to 190 tiles of
+// 256x256 (4136 x 2048, a head's dx) need it for their second split, without which
+// half of the CUs idle.
+constexpr int64_t kTrainSplitBytes = int64_t(128) << 20;
+
 struct GemmDesc {
     const float *a = nullptr;
     const float *b = nullptr;
@@ -173,6 +178,8 @@ struct GemmDesc {
     // With scratch: kTickets zeroed tile counters for the in-kernel split
     // reduction (null: the context's own).
     int32_t *scratch_tickets = nullptr;
+    // Bytes of split partials that the plan may take (0: what the no-alloc array holds).
+    int64_t split_bytes = 0;
     // Receives rows and columns of a tile and the K splits; nothing runs then.
     int32_t *plan = nullptr;
     // EPI_ACCUM with the GEMM seam's rule (kernels.rs:48, C += A.B): C's own

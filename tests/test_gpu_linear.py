@@ -383,6 +383,16 @@ def test_row_blocks(ctx):
         check_loss(got, want, f"{n}: ")
 
 
+@pytest.mark.parametrize("n,d,V,form,share", [(300, 520, 105001, 0, 0.0), (330, 1700, 32100, 1, 0.1), (260, 1664, 32768, 0, 0.0),
+                                             (257, 500, 110001, 1, 0.0)])
+def test_a_few_rows_past_the_last_tile(ctx, n, d, V, form, share):
+    """Beside large weights the few rows past a block's last 256 are a part of their own."""
+    print(f"\n[few rows past a tile] {n} {d} {V} {form}", flush=True)
+    x, w, t = head(n, d, V, seed=n)
+    t[np.random.default_rng(1).random(n) < share] = -1
+    check_loss(run_loss(ctx, form, x, w, t), R.cross_entropy(x, w, t), f"{n}: ")
+
+
 def test_row_blocks_of_the_loss_alone(ctx):
     """More partial sums than the workspace holds: the mean over all rows against that of calls on a few thousand each,
     which take one block. Both are within the bound of a row's term, which other tests hold to 64 bits."""
@@ -517,3 +527,55 @@ def test_the_same_bits_again_and_on_two_contexts(ctx):
         assert np.array_equal(u, v)
     for u, v in zip(first, all_of(ctx)):
         assert np.array_equal(u, v)
+
+
+def test_arrays_beyond_32_bits(ctx):
+    """More than 2^32 values: dropout in place, and a linear layer's output, whose last rows are read back."""
+    n, tail = 2 ** 32 + 4099, 8192
+    seed, offset = 5, 77
+    print("\n[beyond 32 bits] dropout", flush=True)
+    try:
+        buf = ctx.empty((n,))
+    except mh.DeviceError:
+        pytest.skip("needs 17 GB of free device memory")
+    r = np.random.default_rng(0)
+    x = r.standard_normal(tail).astype(np.float32)
+    at = buf.offset(n - tail)
+    mh.check(mh.lib().mmh_upload(ctx.handle, at, x.ctypes.data, x.nbytes))
+    mh.check(mh.lib().mmh_dropout(ctx.handle, buf.ptr, None, n, 0.5, seed, offset, buf.ptr))
+    got = np.empty(tail, np.float32)
+    mh.check(mh.lib().mmh_download(ctx.handle, got.ctypes.data, at, got.nbytes))
+    first = n - tail  # the mask from there on: whole blocks, and the values before the first one
+    keep = R.kept(tail + first % 4, 0.5, seed, offset + first // 4)[first % 4:]
+    assert np.array_equal(got, np.where(keep, x * np.float32(2), np.float32(0)))
+
+    print("[beyond 32 bits] linear", flush=True)
+    cols, k = 2047, 3
+    rows = n // cols
+    xs = r.standard_normal((rows, k)).astype(np.float32)
+    w, b = r.standard_normal((k, cols)).astype(np.float32), r.standard_normal(cols).astype(np.float32)
+    X, W, B = ctx.to_device(xs), ctx.to_device(w), ctx.to_device(b)
+    mh.check(mh.lib().mmh_linear(ctx.handle, 0, X.ptr, W.ptr, B.ptr, None, rows, k, cols, R_ACT["silu"], 0.25, seed, offset,
+                                 None, buf.ptr))
+    last = 300
+    got = np.empty((last, cols), np.float32)
+    mh.check(mh.lib().mmh_download(ctx.handle, got.ctypes.data, buf.offset((rows - last) * cols), got.nbytes))
+    want, tol, _, _ = R.linear(xs[-last:], w, b, None, "silu", 0.0, 0, 0)
+    first = (rows - last) * cols
+    keep = R.kept(last * cols + first % 4, 0.25, seed, offset + first // 4)[first % 4:].reshape(last, cols)
+    scale = 1.0 / 0.75
+    near(got, np.where(keep, want * scale, 0.0), np.where(keep, tol * scale + 2 * R.U * np.abs(want) * scale, 0.0), "out")
+
+    # the column sums of its |values|, whole and in two parts: each call rounds at most 256 + 4 + 129 + 16 times
+    print("[beyond 32 bits] bias gradient", flush=True)
+    mh.check(mh.lib().mmh_linear(ctx.handle, 0, X.ptr, W.ptr, B.ptr, None, rows, k, cols, R_ACT["relu"], 0.0, 0, 0, None,
+                                 buf.ptr))
+    db = [ctx.empty((cols,)) for _ in range(3)]
+    half = rows // 2
+    for out, start, count in ((db[0], 0, rows), (db[1], 0, half), (db[2], half, rows - half)):
+        mh.check(mh.lib().mmh_linear_backward(ctx.handle, 0, None, None, None, buf.offset(start * cols), count, k, cols, 0, 0.0,
+                                              0, 0, None, None, out.ptr))
+    whole, a, b2 = (v.numpy().astype(np.float64) for v in db)
+    near(whole, a + b2, 2 * 405 * R.U * (a + b2), "dbias")
+    for v in (buf, X, W, B, *db):
+        v.free()
