@@ -277,6 +277,7 @@ struct Rows {
     const float *x = nullptr;          // [kept, d]
     const int32_t *targets = nullptr;  // [kept], where kernels read them
     const int32_t *map = nullptr;      // device, [n]: a row's place among the kept ones, or -1; null: all are kept
+    float *loss = nullptr;             // pinned, [kept]: the rows' terms
 };
 
 struct Head {
@@ -310,7 +311,8 @@ void check_head(const Head &h) {
 // the map back go along and those rows of x are packed.
 void stage_rows(Context &cx, const Head &h, bool device, float *packed, Rows &r) {
     const int64_t pad = (h.n + 63) / 64 * 64, total = r.kept == h.n ? h.n : 3 * pad;
-    int32_t *t = static_cast<int32_t *>(cx.pinned_ids((size_t)total * 4));
+    int32_t *t = static_cast<int32_t *>(cx.pinned_rows(((size_t)total + (size_t)r.kept) * 4));
+    r.loss = reinterpret_cast<float *>(t + total);
     r.x = h.x;
     if (r.kept == h.n) {
         std::copy(h.targets, h.targets + h.n, t);
@@ -358,9 +360,15 @@ GemmDesc head_product(const Head &h, const float *x, int64_t rows) {
 
 size_t round64(int64_t floats) { return ((size_t)floats + 63) / 64 * 64; }
 
-void finish_loss(Context &cx, float *loss_host) {
+// Waits for the call's kernels. The row terms lie in pinned memory, and their mean
+// is taken here, in f64 and in eight sums of a fixed order: a launch of its own
+// would take longer than the sum of a few thousand.
+float mean_loss(Context &cx, const float *rows, int64_t n) {
     check_hip(hipStreamSynchronize(cx.stream), "loss sync");
-    *loss_host = cx.words[0];
+    double sum[8] = {};
+    for (int64_t i = 0; i < n; ++i) sum[i & 7] += (double)rows[i];
+    const double total = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+    return (float)(total / (double)n);
 }
 
 void forward(Context &cx, const Head &h, float *loss_host) {
@@ -387,8 +395,8 @@ void forward(Context &cx, const Head &h, float *loss_host) {
     const size_t part = round64(most);
     const size_t parts_floats = round64(2 * kFewRows * part_units(h.vocab));
     float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block) + parts_floats) * 4));
-    float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
     stage_rows(cx, h, folds(block), ws, r);
+    float *row_loss = r.loss;
     float *buf = ws + packed, *zt = buf + part, *stats = zt + round64(block);
     for (int64_t at = 0, rows; at < r.kept; at += rows) {
         rows = part_rows(std::min(block, r.kept - at / block * block), at % block, weights);
@@ -413,8 +421,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
             }
         }
     }
-    launch_mean(cx, row_loss, r.kept, cx.words);
-    finish_loss(cx, loss_host);
+    *loss_host = mean_loss(cx, r.loss, r.kept);
 }
 
 void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host) {
@@ -432,8 +439,8 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     const size_t packed = all ? 0 : round64(r.kept * h.d);
     float *ws = static_cast<float *>(
         cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2) + kFewRows) * 4));
-    float *row_loss = static_cast<float *>(cx.workspace(3, round64(r.kept) * 4));
     stage_rows(cx, h, false, ws, r);
+    float *row_loss = r.loss;
     float *z = ws + packed, *part = z + round64(block * ld);
     float *zt = part + round64(block * units * 2), *dxk = all ? dx : zt + kFewRows;
     const float scale = 1.0f / (float)r.kept;
@@ -507,12 +514,8 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
                            cx.stream, dxk, r.map, h.n, h.d, dx);
         check_hip(hipGetLastError(), "gradient rows launch");
     }
-    if (loss_host) {
-        launch_mean(cx, row_loss, r.kept, cx.words);
-        finish_loss(cx, loss_host);
-    } else {  // the pinned targets have been read
-        check_hip(hipStreamSynchronize(cx.stream), "targets sync");
-    }
+    const float loss = mean_loss(cx, r.loss, r.kept);  // (waits: the pinned targets have been read)
+    if (loss_host) *loss_host = loss;
 }
 
 }  // namespace

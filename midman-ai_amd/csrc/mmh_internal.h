@@ -86,11 +86,12 @@ struct Context {
     int32_t *tickets = nullptr;
     // Two words of pinned host memory for results read back (one thread per context).
     float *words = nullptr;
-    // Pinned host memory for ids on their way to the device. Growing it waits for
-    // queued work; a call that fills it waits for its kernels before it returns.
+    // Pinned host memory for a call's ids on their way to the device and its row
+    // terms on their way back. Growing it waits for queued work; a call that uses
+    // it waits for its kernels before it returns.
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
-    void *pinned_ids(size_t bytes);
+    void *pinned_rows(size_t bytes);
     // Allocations made through mmh_alloc, freed at destroy.
     std::vector<void *> owned;
 
@@ -223,10 +224,9 @@ void launch_cross_entropy(Context &ctx, const float *logits, const int32_t *targ
 // f64 mean as launch_cross_entropy.
 void launch_ce_combine(Context &ctx, const float *part, int64_t tiles, const float *zt,
                        int64_t n, float *row_loss, float *loss_dev);
-// The row terms alone, and their f64 mean (out: device or pinned memory).
+// The row terms alone.
 void launch_ce_combine_rows(Context &ctx, const float *part, int64_t tiles, const float *zt,
                             int64_t n, float *row_loss);
-void launch_mean(Context &ctx, const float *row_loss, int64_t n, float *out);
 void launch_pack_cols(Context &ctx, const float *src, int64_t rows, int64_t cols, float *dst,
                       int64_t ld_dst, int64_t col_off);
 void launch_pack_gate_up(Context &ctx, const float *wg, const float *wu, int64_t rows,

@@ -470,12 +470,6 @@ void launch_rope(Context &ctx, const float *x, int64_t bh, int64_t t, int64_t hd
     check_hip(hipGetLastError(), "rope launch");
 }
 
-void launch_mean(Context &ctx, const float *row_loss, int64_t n, float *loss_dev) {
-    hipLaunchKernelGGL(mean_f64_kernel, dim3(1), dim3(256), 0, ctx.stream, row_loss, n,
-                       loss_dev);
-    check_hip(hipGetLastError(), "loss mean launch");
-}
-
 void launch_cross_entropy(Context &ctx, const float *logits, const int32_t *targets_dev,
                           int64_t n, int64_t v, float *row_loss, float *loss_dev) {
     if (n > 0x7fffffff) fail(MMH_ERR_SHAPE, "cross_entropy: too many rows");
@@ -483,7 +477,9 @@ void launch_cross_entropy(Context &ctx, const float *logits, const int32_t *targ
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)n), dim3(256), 0, ctx.stream, logits,
                        targets_dev, n, v, row_loss, vec);
     check_hip(hipGetLastError(), "cross_entropy launch");
-    launch_mean(ctx, row_loss, n, loss_dev);
+    hipLaunchKernelGGL(mean_f64_kernel, dim3(1), dim3(256), 0, ctx.stream, row_loss, n,
+                       loss_dev);
+    check_hip(hipGetLastError(), "loss mean launch");
 }
 
 void launch_ce_combine_rows(Context &ctx, const float *part, int64_t tiles, const float *zt,
@@ -497,7 +493,9 @@ void launch_ce_combine_rows(Context &ctx, const float *part, int64_t tiles, cons
 void launch_ce_combine(Context &ctx, const float *part, int64_t tiles, const float *zt,
                        int64_t n, float *row_loss, float *loss_dev) {
     launch_ce_combine_rows(ctx, part, tiles, zt, n, row_loss);
-    launch_mean(ctx, row_loss, n, loss_dev);
+    hipLaunchKernelGGL(mean_f64_kernel, dim3(1), dim3(256), 0, ctx.stream, row_loss, n,
+                       loss_dev);
+    check_hip(hipGetLastError(), "loss mean launch");
 }
 
 // Grid of the row-walking copy kernels: enough threads for a row's units in

@@ -45,7 +45,7 @@ void *Context::workspace(int slot, size_t bytes) {
     return ws[slot];
 }
 
-void *Context::pinned_ids(size_t bytes) {
+void *Context::pinned_rows(size_t bytes) {
     if (bytes > pinned_bytes) {
         if (pinned) {
             check_hip(hipStreamSynchronize(stream), "pinned sync");
