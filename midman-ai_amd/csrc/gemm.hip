@@ -1153,6 +1153,10 @@ TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int e
             if (s > 1 && (!may_split || p.k < 128 * s || s * p.m * p.n * 4 > split_bytes)) break;
             const double g = tiles * s, setup = even ? 6.0 : t.setup;
             double us = std::max(std::ceil(g / cus) * t.alone, g / cus * t.full) * (ksteps / s + setup);
+            // The linear layer's epilogue, 0.1 (bare) to 0.65 (all of it) ns per value
+            // of the busiest CU's tiles: nothing overlaps it there (4096 x 5632 from K
+            // 2048: 582 us on two rounds of 256x256, 510 on three of 256x128).
+            if (epi == EPI_LINEAR && s == 1) us += std::ceil(g / cus) * t.rows * t.cols * 0.3e-3;
             if (s > 1) us += 4.0 + (double)(s + 1) * (double)(p.m * p.n) * 4.0 / 3.5e6;
             if (s > 8) us += 0.2 * (s - 8);
             const int fine = s > 8 || (s & (s - 1)) ? 1 : 0;

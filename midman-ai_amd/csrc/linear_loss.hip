@@ -2,14 +2,15 @@
 //   z = x op(W), loss = mean over the kept rows of ln sum_j exp(z_j) - z_target,
 //   dz = (softmax(z) - onehot) / kept, dx = dz op(W)^T, dW = x^T dz (or dz^T x).
 //
-// The logits are never whole in memory: the loss alone folds into the head's
-// product (EPI_CE: a maximum and a sum per row and 128 columns), and the
-// gradients take blocks of rows, whose logits become dz in place in a workspace
-// of kLogitBytes. A pass over them reads and writes each row once: up to kRowCols
-// columns from registers; for wider rows the product leaves the same partials
-// beside the logits, which costs its epilogue more than the second read of a
-// row costs elsewhere. Rows whose target is `ignore` are left out before the first
-// product, so nothing they hold (infinities, NaN) reaches a sum.
+// The loss alone folds into the head's product (EPI_CE: a maximum and a sum per
+// row and 128 columns) and stores no logits; the gradients take blocks of rows,
+// whose logits become dz in place in a workspace of kLogitBytes, however many rows
+// there are. (Dropping them and forming them again for dx and dW would cost a
+// fourth product, a third of the time.) A pass over them reads and writes each
+// row once: up to kRowCols columns from registers; for wider rows the product
+// leaves the same partials beside the logits (three passes over such rows instead:
+// 817 x 1024 x 131071 4650 us, 4500 so). Rows whose target is `ignore` are left out
+// before the first product, so nothing they hold (infinities, NaN) reaches a sum.
 #include <algorithm>
 
 #include "mmh_args.h"
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(256) void spread_rows_kernel(const float *__restric
 // scale in its place. A workgroup holds a row in registers, NV float4s per
 // thread, so it passes through once; rows are ld (a multiple of 4, 16-byte
 // aligned) floats of which v are logits. A NaN anywhere reaches the sum. Bound by
-// the logits' read and write.
+// the logits' read and write (4096 x 32000: 194 us, 5.4 TB/s).
 constexpr int64_t kRowCols = 32768;
 template <int NT, int NV, bool GRAD>
 __global__ __launch_bounds__(NT) void loss_rows_kernel(float *z, const int32_t *targets, int64_t ld, int v,
@@ -196,9 +197,10 @@ __global__ __launch_bounds__(256) void loss_parts_kernel(const float *z, const i
 }
 
 // dz in place of wider rows, whose product left (max, sum) per 128 columns beside
-// the logits (EPI_CE_STORE). A workgroup has a chunk of a row: it merges the row's partials
-// (at most a few KB, read by each of the row's workgroups), then its columns pass
-// through once. Bound by the logits' read and write.
+// the logits (EPI_CE_STORE) or which loss_parts_kernel has been through. A
+// workgroup has a chunk of a row: it merges the row's partials (a few KB, read by
+// each of the row's workgroups), then its columns pass through once. Bound by the
+// logits' read and write (817 x 131071: 170 us, 5.0 TB/s).
 __global__ __launch_bounds__(256) void loss_grad_kernel(float *z, const float2 *part,
                                                         const int32_t *targets, int64_t ld, int64_t v,
                                                         int64_t units, int64_t chunk, float scale,
@@ -360,11 +362,22 @@ GemmDesc head_product(const Head &h, const float *x, int64_t rows) {
 
 size_t round64(int64_t floats) { return ((size_t)floats + 63) / 64 * 64; }
 
+// A call that fails after its first launch still waits for its kernels: they use
+// the pinned memory that the next call writes.
+struct Drain {
+    Context &cx;
+    bool done = false;
+    ~Drain() {
+        if (!done) (void)hipStreamSynchronize(cx.stream);
+    }
+};
+
 // Waits for the call's kernels. The row terms lie in pinned memory, and their mean
 // is taken here, in f64 and in eight sums of a fixed order: a launch of its own
 // would take longer than the sum of a few thousand.
-float mean_loss(Context &cx, const float *rows, int64_t n) {
-    check_hip(hipStreamSynchronize(cx.stream), "loss sync");
+float mean_loss(Drain &drain, const float *rows, int64_t n) {
+    drain.done = true;
+    check_hip(hipStreamSynchronize(drain.cx.stream), "loss sync");
     double sum[8] = {};
     for (int64_t i = 0; i < n; ++i) sum[i & 7] += (double)rows[i];
     const double total = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
@@ -395,6 +408,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
     const size_t part = round64(most);
     const size_t parts_floats = round64(2 * kFewRows * part_units(h.vocab));
     float *ws = static_cast<float *>(cx.workspace(2, (packed + part + round64(block) + parts_floats) * 4));
+    Drain drain{cx};
     stage_rows(cx, h, folds(block), ws, r);
     float *row_loss = r.loss;
     float *buf = ws + packed, *zt = buf + part, *stats = zt + round64(block);
@@ -421,7 +435,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
             }
         }
     }
-    *loss_host = mean_loss(cx, r.loss, r.kept);
+    *loss_host = mean_loss(drain, r.loss, r.kept);
 }
 
 void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host) {
@@ -439,6 +453,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     const size_t packed = all ? 0 : round64(r.kept * h.d);
     float *ws = static_cast<float *>(
         cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2) + kFewRows) * 4));
+    Drain drain{cx};
     stage_rows(cx, h, false, ws, r);
     float *row_loss = r.loss;
     float *z = ws + packed, *part = z + round64(block * ld);
@@ -514,7 +529,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
                            cx.stream, dxk, r.map, h.n, h.d, dx);
         check_hip(hipGetLastError(), "gradient rows launch");
     }
-    const float loss = mean_loss(cx, r.loss, r.kept);  // (waits: the pinned targets have been read)
+    const float loss = mean_loss(drain, r.loss, r.kept);  // (waits: the pinned targets have been read)
     if (loss_host) *loss_host = loss;
 }
 
