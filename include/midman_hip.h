@@ -419,7 +419,7 @@ int32_t mmh_embedding_backward(mmh_handle ctx, const int32_t *ids_host, int64_t 
 /* ---- The linear layer's training operators ---------------------------------
  * No counterpart in the reference, whose Linear is the bare matmul and whose
  * loss takes stored logits. f32, contiguous row-major arrays at any 4-byte
- * alignment; weights [k, n] (form MMH_GEMM_NN) or [n, k] (MMH_GEMM_NT, a tied
+ * alignment, each extent below 2^31; weights [k, n] (form MMH_GEMM_NN) or [n, k] (MMH_GEMM_NT, a tied
  * embedding's layout). Sums are f32, the products' as mmh_gemm_* forms them. An
  * output that overlaps another buffer of the call is MMH_ERR_ARGUMENT, except
  * where it may be the very same buffer, as stated.
@@ -459,18 +459,20 @@ int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w,
  * op(w)^T, dw = x^T dpre in w's layout, dbias the column sums of dpre (d residual
  * is dout itself). pre as the forward call left it; NULL for MMH_ACT_NONE. Any
  * of dx, dw, dbias may be NULL (not needed), and then w (for dx), x (for dw) too.
- * Outputs are overwritten. The derivative of relu at 0 is 0. */
+ * Outputs are overwritten. The derivative of relu at 0 is 0. dpre takes rows * n
+ * floats of the context's workspace where it is not dout itself. */
 int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const float *w,
                             const float *pre, const float *dout, int64_t rows, int64_t k, int64_t n,
                             int32_t activation, float p, uint64_t seed, uint64_t offset, float *dx,
                             float *dw, float *dbias);
 /* The cross entropy (as mmh_cross_entropy has it) of the logits x op(w): x [n,
- * d], w [d, vocab] or [vocab, d], targets on the host. The logits are never
- * whole in memory: the call's workspace holds a block of rows, 256 MiB (128 rows
- * where those are more). Rows whose target is `ignore` (any value, -1 say) are
- * left out: the mean is over the others, and nothing the row holds is read. With
- * no row left the loss is 0. Other targets outside [0, vocab) are
- * MMH_ERR_INDEX. */
+ * d], w [d, vocab] or [vocab, d], targets on the host. Rows whose target is
+ * `ignore` (any value, -1 say) are left out: the mean is over the others, and
+ * nothing the row holds is read. With no row left the loss is 0. Other targets
+ * outside [0, vocab) are MMH_ERR_INDEX, and nothing runs. However many rows there
+ * are, the context's workspace holds the logits of a block of them: 512 MiB of
+ * rows, or 128 rows where those are more. Both calls wait for their work (the
+ * targets have been read and the loss is there when they return). */
 int32_t mmh_linear_cross_entropy(mmh_handle ctx, int32_t form, const float *x, const float *w,
                                  const int32_t *targets_host, int64_t n, int64_t d, int64_t vocab,
                                  int32_t ignore, float *loss_host);

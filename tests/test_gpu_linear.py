@@ -157,6 +157,38 @@ def test_linear_dropped_values_and_special_values(ctx):
     assert (out == 0).all()
 
 
+# every product kernel: 32x32 and 64x64 tiles, K split in the launch, large tiles whole and split over launches
+@pytest.mark.parametrize("shape", [(64, 64, 176), (33, 300, 64), (520, 200, 515), (300, 5003, 301), (2300, 64, 2301),
+                                   (3300, 70, 3000), (1000, 2050, 4100)])
+@pytest.mark.parametrize("form", [0, 1])
+def test_values_outside_the_split(ctx, shape, form):
+    """Rows of x with an infinity, a NaN, values from 2^104 on and subnormal ones, beside ordinary rows: the ordinary ones
+    keep their bounds, the others follow IEEE (row r of the result depends on row r of x alone)."""
+    rows, k, n = shape
+    print(f"\n[values outside the split] {shape} {form}", flush=True)
+    x, w, b, res = operands(rows, k, n, 31)
+    x[3, 1], x[7, 2] = np.inf, np.nan
+    x[11, :4] = np.float32(2.0) ** 106 * np.array([1, -1, 2, 0.5], np.float32)
+    x[15] *= np.float32(2.0) ** -120
+    seed, offset = 8, 1
+    out, pre = run_linear(ctx, form, x, w, b, res, "silu", 0.25, seed, offset, True)
+    odd = [3, 7]
+    rest = np.setdiff1d(np.arange(rows), odd)
+    x0 = x.copy()
+    x0[odd] = 0
+    want, tol, want_pre, pre_tol = R.linear(x0, w, b, res, "silu", 0.25, seed, offset)
+    # a subnormal product or input may be flushed by the fp32 kernels: one smallest normal value per term
+    tiny = k * R.TINY
+    near(pre[rest], want_pre[rest], pre_tol[rest] + tiny, "pre")
+    near(out[rest], want[rest], tol[rest] + 2 * tiny, "out")
+    with np.errstate(invalid="ignore"):
+        sign = np.where(np.isnan(w[1]) | (w[1] == 0), np.nan, np.sign(w[1]) * np.inf)
+    assert np.array_equal(pre[3], sign.astype(np.float32), equal_nan=True)
+    assert np.isnan(pre[7]).all()
+    keep = R.kept(rows * n, 0.25, seed, offset).reshape(rows, n)
+    assert np.array_equal(out[7][~keep[7]], res[7][~keep[7]]) and np.isnan(out[7][keep[7]]).all()
+
+
 def test_activations_far_out(ctx):
     """Large arguments of either sign: k = 1 products of 1 and the value itself."""
     v = np.array([0.0, -0.0, 1e-30, -1e-30, 0.5, -0.5, 3, -3, 6, -6, 9, -9, 20, -20, 88, -88, 104, -104, 1e4, -1e4, 1e20,
@@ -527,6 +559,55 @@ def test_the_same_bits_again_and_on_two_contexts(ctx):
         assert np.array_equal(u, v)
     for u, v in zip(first, all_of(ctx)):
         assert np.array_equal(u, v)
+
+
+def test_a_refused_call_runs_nothing(ctx):
+    x, w, t = head(40, 16, 70, seed=3)
+    X, W = ctx.to_device(x), ctx.to_device(stored(w, 1))
+    dx, dw = ctx.to_device(np.full((40, 16), 3, np.float32)), ctx.to_device(np.full((70, 16), 4, np.float32))
+    for bad in (70, -1, 2 ** 31 - 1):
+        t[33] = bad
+        with pytest.raises(mh.IndexOutOfRange):
+            mh.linear_cross_entropy_backward(ctx, X, W, t, ignore=-2, dx=dx, dw=dw)
+        with pytest.raises(mh.IndexOutOfRange):
+            mh.linear_cross_entropy(ctx, X, W, t, ignore=-2)
+    with pytest.raises(mh.ArgumentError):
+        mh.linear_cross_entropy_backward(ctx, X, W, np.zeros(40, np.int32), dx=X, dw=dw)
+    with pytest.raises(mh.ArgumentError):
+        mh.dropout(ctx, X, 1.5, 1, out=dx)
+    with pytest.raises(mh.ArgumentError):
+        mh.linear(ctx, X, W, form="nt", activation="gelu", p=-1.0, out=ctx.empty((40, 70)))
+    assert (dx.numpy() == 3).all() and (dw.numpy() == 4).all() and np.array_equal(X.numpy(), x)
+
+
+def test_two_threads_with_a_context_each(ctx):
+    """Calls of two threads at once, each on its own context, give what they give alone."""
+    import threading
+    x, w, t = head(300, 64, 2050, seed=41)
+    t[::9] = -1
+    a, wl, b, res = operands(300, 200, 260, 42)
+    pre = np.random.default_rng(1).standard_normal((300, 260)).astype(np.float32)
+
+    def work(c, found, turns):
+        for _ in range(turns):
+            l = run_loss(c, 0, x, w, t)
+            out, _ = run_linear(c, 1, a, wl, b, res, "gelu", 0.3, 1, 2, True)
+            g = run_backward(c, 1, a, wl, pre, res, "silu", 0.3, 1, 2)
+            found.append([l["dx"], l["dw"], np.float32(l["loss"]), np.float32(l["forward"]), out, *g.values()])
+
+    alone = []
+    work(ctx, alone, 1)
+    with mh.Context(0) as c1, mh.Context(0) as c2:
+        found = [[], []]
+        threads = [threading.Thread(target=work, args=(c, f, 8)) for c, f in zip((c1, c2), found)]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+    for f in found:
+        assert len(f) == 8
+        for got in f:
+            assert all(np.array_equal(u, v) for u, v in zip(got, alone[0]))
 
 
 def test_arrays_beyond_32_bits(ctx):
