@@ -538,35 +538,7 @@ __global__ __launch_bounds__(256) void gemm_f32_mfma_small(KParams p) {
             const int64_t row = row_of(r);
             if (row < M && col < N) split_put(P + row * N + col, acc[r]);
         }
-        if (split_last(p, tm * p.tiles_n + tn)) {
-            if constexpr (EPI == EPI_LINEAR) split_linear_tile(p, m0, n0, SBM, SBN, 256);
-            else split_reduce_tile(p, m0, n0, SBM, SBN, 256);
-        }
-        return;
-    }
-    if constexpr (EPI == EPI_LINEAR) {
-        // through LDS (free behind the K loop's last barrier): a thread has four
-        // neighbouring columns of a row
-        constexpr int LD = SBN + 4;
-        static_assert(SBM * LD <= 2 * SBM * SKS, "the tile fits A's stages");
-        float *tile = &As[0][0][0];
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            tile[(wm * 32 + 8 * (r >> 2) + 4 * lk + (r & 3)) * LD + wn * 32 + lr] = acc[r];
-        __syncthreads();
-#pragma unroll 1
-        for (int e = tid; e < SBM * SBN / 4; e += 256) {
-            const int rl = e / (SBN / 4), c = e % (SBN / 4) * 4;
-            const int64_t row = m0 + rl, cc = n0 + c;
-            if (row >= M || cc >= N) continue;
-            const int count = (int)min(N - cc, (int64_t)4);
-            TailInputs in;
-            tail_load(p.tail, N, row, cc, count, in);
-            float v[4];
-            __builtin_memcpy(v, __builtin_assume_aligned(tile + rl * LD + c, 16), 16);
-            tail_finish(p.tail, N, row, cc, count, in, v);
-        }
+        if (split_last(p, tm * p.tiles_n + tn)) split_reduce_tile(p, m0, n0, SBM, SBN, 256);
         return;
     }
     float *C = p.c + batch * p.stride_c;
@@ -1419,9 +1391,8 @@ void gemm(Context &ctx, const GemmDesc &d) {
                               : launch_ksplit<true, false, EPI_STORE>)(ctx, p, grid, mode);
     } else if (tiled) {
         launch_gemm_tiles(ctx, p, grid, d.ta, d.tb, epi, plan.tile);
-    } else if (epi == EPI_LINEAR) {
-        if (d.tb) launch<false, true, EPI_LINEAR>(ctx, p, grid);
-        else launch<false, false, EPI_LINEAR>(ctx, p, grid);
+    } else if (epi == EPI_LINEAR) {  // (small products of one matrix split K)
+        fail(MMH_ERR_OTHER, "gemm: no 64x64 tiles with the linear epilogue");
     } else if (epi == EPI_SWIGLU) {
         if (d.ta || d.tb) fail(MMH_ERR_ARGUMENT, "gemm: swiglu epilogue needs the nn form");
         launch<false, false, EPI_SWIGLU>(ctx, p, grid);
