@@ -1078,6 +1078,7 @@ namespace {
 
 struct TilePlan {
     int tile = TILE_128, splits = 1;
+    double us = 0.0;  // the estimate
 };
 
 // Split partials of the large tiles stay below this: the no-alloc entry point's
@@ -1136,6 +1137,7 @@ TilePlan fastest_tile(const Context &ctx, const KParams &p, int64_t batch, int e
                 best_us[fine] = us;
                 best[fine].tile = tile;
                 best[fine].splits = s;
+                best[fine].us = us;
             }
         }
     }
@@ -1410,6 +1412,130 @@ void gemm(Context &ctx, const GemmDesc &d) {
         launch_rope_strided(ctx, d.c, d.rope_seq * d.ldc, d.rope_hd, d.ldc, d.m / d.rope_seq,
                             d.rope_cols / d.rope_hd, d.rope_seq, d.rope_hd, d.rope_cos,
                             d.rope_sin);
+}
+
+namespace {
+
+// When the last of g1 workgroups of length l1, then g2 of l2, each given to the CU
+// that is free first, ends.
+double list_end(int64_t cus, int64_t g1, double l1, int64_t g2, double l2) {
+    const int64_t q = g1 / cus, r = g1 % cus;  // r CUs are free at (q + 1) l1, the others at q l1
+    const double early = (double)q * l1, late = r ? early + l1 : early;
+    // the earliest end of a whole number of l2 on either that leaves room for g2
+    auto room = [&](double t) {
+        auto fit = [&](double from) { return t < from ? 0.0 : std::floor((t - from) / l2 + 1e-9); };
+        return (double)(cus - r) * fit(early) + (double)r * fit(late);
+    };
+    double best = 1e30;
+    for (double from : {early, late}) {
+        double n = std::max(0.0, std::floor(((double)g2 * l2 / (double)cus + early - from) / l2) - 1.0);
+        while (room(from + n * l2) < (double)g2) n += 1.0;
+        best = std::min(best, from + n * l2);
+    }
+    return std::max(best, late);
+}
+
+KParams plain_params(const GemmDesc &d, const GemmTileInfo &t, int splits) {
+    KParams p{};
+    p.a = d.a;
+    p.b = d.b;
+    p.c = d.c;
+    p.m = d.m;
+    p.n = d.n;
+    p.k = d.k;
+    p.lda = d.lda;
+    p.ldb = d.ldb;
+    p.ldc = d.ldc;
+    p.vec_c = d.ldc % 2 == 0 && (reinterpret_cast<uintptr_t>(d.c) & 7) == 0;
+    p.tiles_m = (int)((d.m + t.rows - 1) / t.rows);
+    p.tiles_n = (int)((d.n + t.cols - 1) / t.cols);
+    const int64_t ktiles = (d.k + BK - 1) / BK, per = (ktiles + splits - 1) / splits;
+    p.k_per_split = per * BK;
+    p.splits = (int)((ktiles + per - 1) / per);
+    return p;
+}
+
+}  // namespace
+
+void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b) {
+    if (a.ta || !b.ta || b.tb || a.epi != EPI_STORE || b.epi != EPI_STORE || a.batch != 1 || b.batch != 1 ||
+        a.norm_w || b.norm_w || a.rope_cos || b.rope_cos || a.scratch || b.scratch)
+        fail(MMH_ERR_ARGUMENT, "gemm: a pair is one plain nn or nt and one plain tn product");
+    const int cus = cus_of(ctx);
+    const GemmDesc *d[2] = {&a, &b};
+    TilePlan best;
+    int splits[2] = {1, 1};
+    bool tiled = true;
+    for (const GemmDesc *x : d) tiled = tiled && !use_small(ctx, *x) && ksplit_kind(ctx, *x) == 0;
+    if (tiled) {
+        // One after the other, and each a launch; together only where the estimate is
+        // 8% lower: over 80 pairs of 0.3 to 40 G multiply-adds the measured times
+        // together were 0.83 to 1.17 of theirs, and those estimated closer were up to
+        // 9% slower.
+        double apart_us = 6.0;
+        for (const GemmDesc *x : d) {
+            KParams p{};
+            p.m = x->m;
+            p.n = x->n;
+            p.k = x->k;
+            apart_us += choose_tile(ctx, p, 1, EPI_STORE, x->split_bytes ? x->split_bytes : kSplitBytes).us;
+        }
+        best.us = 0.92 * apart_us;
+        bool found = false;
+        constexpr int kCounts[] = {1, 2, 3, 4, 6, 8};
+        for (int tile = TILE_256; tile < TILE_COUNT; ++tile) {
+            const GemmTileInfo &t = kGemmTiles[tile];
+            double steps[2], cost[2][6];
+            int64_t tiles[2];
+            int counts[2];
+            for (int i = 0; i < 2; ++i) {
+                const GemmDesc &x = *d[i];
+                const int64_t limit = x.split_bytes ? x.split_bytes : kSplitBytes;
+                tiles[i] = ((x.m + t.rows - 1) / t.rows) * ((x.n + t.cols - 1) / t.cols);
+                steps[i] = (double)((x.k + BK - 1) / BK);
+                counts[i] = 0;
+                for (int s : kCounts) {
+                    if (s > 1 && (x.k < 128 * s || s * x.m * x.n * 4 > limit)) break;
+                    cost[i][counts[i]++] = s == 1 ? 0.0 : 4.0 + (double)(s + 1) * (double)(x.m * x.n) * 4.0 / 3.5e6;
+                }
+            }
+            for (int i = 0; i < counts[0]; ++i)
+                for (int j = 0; j < counts[1]; ++j) {
+                    const double l1 = steps[0] / kCounts[i] + t.setup, l2 = steps[1] / kCounts[j] + t.setup;
+                    const double g1 = (double)(tiles[0] * kCounts[i]), g2 = (double)(tiles[1] * kCounts[j]);
+                    const double full = (g1 * l1 + g2 * l2) / cus * t.full + cost[0][i] + cost[1][j] + 3.0;
+                    if (full >= best.us) continue;
+                    const double us = std::max(full, list_end(cus, (int64_t)g1, l1, (int64_t)g2, l2) * t.alone +
+                                                         cost[0][i] + cost[1][j] + 3.0);
+                    if (us >= best.us) continue;
+                    found = true;
+                    best.us = us;
+                    best.tile = tile;
+                    splits[0] = kCounts[i];
+                    splits[1] = kCounts[j];
+                }
+        }
+        tiled = found;
+    }
+    if (!tiled) {
+        gemm(ctx, a);
+        gemm(ctx, b);
+        return;
+    }
+    KParams p[2];
+    int64_t floats[2];
+    for (int i = 0; i < 2; ++i) {
+        p[i] = plain_params(*d[i], kGemmTiles[best.tile], splits[i]);
+        floats[i] = p[i].splits > 1 ? ((int64_t)p[i].splits * p[i].m * p[i].n + 63) / 64 * 64 : 0;
+    }
+    if (floats[0] + floats[1] > 0) {
+        float *partial = static_cast<float *>(ctx.get_scratch((size_t)(floats[0] + floats[1]) * 4));
+        p[0].partial = partial;
+        p[1].partial = partial + floats[0];
+    }
+    launch_gemm_pair(ctx, p[0], p[1], a.tb, best.tile);
+    for (const KParams &x : p)
+        if (x.splits > 1) launch_splitk_reduce(ctx, x, EPI_STORE);
 }
 
 double mfma_peak_tflops(Context &ctx) {

@@ -770,41 +770,19 @@ __device__ __forceinline__ void block_epilogue(const KParams &p, const floatx16 
     }
 }
 
-template <bool TA, bool TB, int EPI, int CL, int WM, int WN, int MB, int WK>
-__global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) {
-    static_assert(CL == 0 || EPI == EPI_STORE, "the RoPE column layouts store plain values");
-    constexpr bool CE = EPI == EPI_CE || EPI == EPI_CE_STORE;
-    static_assert(!CE || WN % 2 == 0, "the loss takes 128 columns at a time");
+// The sums of one tile: the K loop, the groups' sums added in group order by group
+// 0, and what the split does not hold done again. True in group 0, whose acc has
+// them. Every thread of the workgroup calls it; lds is free behind it. SIGNED:
+// sums that start from acc_init (C is read for its zeros).
+template <bool TA, bool TB, bool SIGNED, int CL, int WM, int WN, int MB, int WK>
+__device__ __forceinline__ bool tile_sums(const KParams &p, const float *__restrict__ A,
+                                          const float *__restrict__ B, const float *C, int64_t m0,
+                                          int64_t n0, int64_t kbeg, int64_t kend, char *lds,
+                                          floatx16 (&acc)[MB][2]) {
     using S = TileShape<WM, WN, MB>;
-    constexpr int TM = S::TM, TN = S::TN, NT = S::NT;
-    __shared__ __attribute__((aligned(128))) char lds[WK * 2 * S::STAGE];
-
-    const int tid = threadIdx.x;
-    // XCD-aware renumbering, then grouped tile order
-    const int64_t kbeg = (int64_t)blockIdx.z * p.k_per_split;
-    const int64_t kend = min(p.k, kbeg + p.k_per_split);
-    const int nb = (int)gridDim.x, q = nb >> 3, r8 = nb & 7;
-    const int xcd = (int)blockIdx.x & 7, local = (int)blockIdx.x >> 3;
-    const int bid = xcd * q + (xcd < r8 ? xcd : r8) + local;
-    int tm, tn;
-    grouped_tile(p, group_rows(TM), bid, tm, tn);
-    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
-
-    const int64_t batch = blockIdx.y;
-    const int split = blockIdx.z;
-    const float *__restrict__ A = p.a + batch * p.stride_a;
-    const float *__restrict__ B = p.b + batch * p.stride_b;
+    constexpr int NT = S::NT;
     const int64_t M = p.m, N = p.n;
-
-    floatx16 acc[MB][2];
-    // EPI_CE: the tile's target ids go to LDS before the K loop (whose
-    // barriers order them before the epilogue reads them)
-    __shared__ int ce_t[EPI == EPI_CE ? TM : 1];
-    if (EPI == EPI_CE && tid < TM) ce_t[tid] = m0 + tid < M ? p.ce_targets[m0 + tid] : -1;
-    // EPI_LINEAR: the tile's bias likewise (-0 for none, the identity of addition)
-    __shared__ __attribute__((aligned(16))) float bias_s[EPI == EPI_LINEAR ? TN : 1];
-    if (EPI == EPI_LINEAR && tid < TN)
-        bias_s[tid] = p.tail.bias && n0 + tid < N ? p.tail.bias[n0 + tid] : -0.0f;
+    const int tid = threadIdx.x;
     split_mainloop<TA, TB, CL, WM, WN, MB, WK>(p, A, B, m0, n0, kbeg, kend, lds, acc);
 
     const int lane = tid & 63, wave = tid % NT >> 6;
@@ -855,7 +833,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
                 }
         redo = !(nf == 0.0f);
     }
-    if (EPI == EPI_STORE || EPI == EPI_ACCUM) {
+    if (SIGNED) {
         if (first && __float_as_uint(p.acc_init) != 0) {
             // A sum of zero that is added to a -0 of C keeps its own sign (a
             // split's too: C is as it was until splitk_reduce). Any other C or
@@ -863,7 +841,6 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
             // reads of C alone: eight at a time, since a read under each sum's
             // own test would wait by itself (512 x 2048 x 1408 tn, a quarter of k
             // zero: 50.5 us so, 38.2 this way, 34.2 dense).
-            const float *C = p.c + batch * p.stride_c;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -892,8 +869,52 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
         }
     }
     redo = __syncthreads_or(redo);
-    if (!CE && EPI != EPI_LINEAR && !first) return;
     if (first && redo) exact_mainloop<TA, TB, CL, WM, WN, MB>(p, A, B, m0, n0, kbeg, kend, acc);
+    return first;
+}
+
+template <bool TA, bool TB, int EPI, int CL, int WM, int WN, int MB, int WK>
+__global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) {
+    static_assert(CL == 0 || EPI == EPI_STORE, "the RoPE column layouts store plain values");
+    constexpr bool CE = EPI == EPI_CE || EPI == EPI_CE_STORE;
+    static_assert(!CE || WN % 2 == 0, "the loss takes 128 columns at a time");
+    using S = TileShape<WM, WN, MB>;
+    constexpr int TM = S::TM, TN = S::TN, NT = S::NT;
+    __shared__ __attribute__((aligned(128))) char lds[WK * 2 * S::STAGE];
+
+    const int tid = threadIdx.x;
+    // XCD-aware renumbering, then grouped tile order
+    const int64_t kbeg = (int64_t)blockIdx.z * p.k_per_split;
+    const int64_t kend = min(p.k, kbeg + p.k_per_split);
+    const int nb = (int)gridDim.x, q = nb >> 3, r8 = nb & 7;
+    const int xcd = (int)blockIdx.x & 7, local = (int)blockIdx.x >> 3;
+    const int bid = xcd * q + (xcd < r8 ? xcd : r8) + local;
+    int tm, tn;
+    grouped_tile(p, group_rows(TM), bid, tm, tn);
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+
+    const int64_t batch = blockIdx.y;
+    const int split = blockIdx.z;
+    const float *__restrict__ A = p.a + batch * p.stride_a;
+    const float *__restrict__ B = p.b + batch * p.stride_b;
+    const int64_t M = p.m, N = p.n;
+
+    floatx16 acc[MB][2];
+    // EPI_CE: the tile's target ids go to LDS before the K loop (whose
+    // barriers order them before the epilogue reads them)
+    __shared__ int ce_t[EPI == EPI_CE ? TM : 1];
+    if (EPI == EPI_CE && tid < TM) ce_t[tid] = m0 + tid < M ? p.ce_targets[m0 + tid] : -1;
+    // EPI_LINEAR: the tile's bias likewise (-0 for none, the identity of addition)
+    __shared__ __attribute__((aligned(16))) float bias_s[EPI == EPI_LINEAR ? TN : 1];
+    if (EPI == EPI_LINEAR && tid < TN)
+        bias_s[tid] = p.tail.bias && n0 + tid < N ? p.tail.bias[n0 + tid] : -0.0f;
+    const bool first = tile_sums<TA, TB, EPI == EPI_STORE || EPI == EPI_ACCUM, CL, WM, WN, MB, WK>(
+        p, A, B, p.c + batch * p.stride_c, m0, n0, kbeg, kend, lds, acc);
+    if (!CE && EPI != EPI_LINEAR && !first) return;
+
+    const int lane = tid & 63, wave = tid % NT >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    const int lr = lane & 31, lk = lane >> 5;
 
     // ---- epilogue: block (i, j) register r of lane l is C[row][col] with
     // row = m0 + 32*(MB*wm + i) + 8*(r/4) + 4*(l/32) + r%4 and, for CL 0,
@@ -1051,6 +1072,41 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split(KParams p) 
     }
 }
 
+// Two products in one launch, which need not wait for each other: workgroups
+// below `first` (a multiple of 8, so both keep their XCDs' runs of tiles) take the
+// splits of the tiles of p1, an nn or nt product, the others p2's, a tn one. The
+// second's tiles fill the CUs that the first leaves idle at its end or throughout:
+// the gradients of a linear layer of 1003 x 770 x 1517 took 61 us one after the
+// other and take 52 so, of 2048 x 1024 x 1024 70 and 58, of 80 shapes 13% less on
+// average. (On two streams the events cost more than that: 1003 x 770 x 1517 72.)
+template <bool TA, bool TB, int WM, int WN, int MB, int WK>
+__device__ __forceinline__ void pair_tile(const KParams &p, int index, char *lds) {
+    using S = TileShape<WM, WN, MB>;
+    const int tiles = p.tiles_m * p.tiles_n, split = index / tiles, x = index - split * tiles;
+    if (split >= p.splits) return;
+    const int q = tiles >> 3, r8 = tiles & 7, xcd = x & 7;
+    int tm, tn;
+    grouped_tile(p, group_rows(S::TM), xcd * q + (xcd < r8 ? xcd : r8) + (x >> 3), tm, tn);
+    const int64_t m0 = (int64_t)tm * S::TM, n0 = (int64_t)tn * S::TN;
+    const int64_t kbeg = (int64_t)split * p.k_per_split, kend = min(p.k, kbeg + p.k_per_split);
+    floatx16 acc[MB][2];
+    if (!tile_sums<TA, TB, false, 0, WM, WN, MB, WK>(p, p.a, p.b, p.c, m0, n0, kbeg, kend, lds, acc)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid % S::NT >> 6;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        block_epilogue<EPI_STORE, 0, S::TM, S::TN>(p, acc[i][0], acc[i][1], split, 0, m0, n0,
+                                                   (wave / WN * MB + i) * 32, wave % WN, lane & 31, lane >> 5);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+template <bool TB1, int WM, int WN, int MB, int WK>
+__global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split_pair(KParams p1, KParams p2, int first) {
+    __shared__ __attribute__((aligned(128))) char lds[WK * 2 * TileShape<WM, WN, MB>::STAGE];
+    const int b = blockIdx.x;
+    if (b < first) pair_tile<false, TB1, WM, WN, MB, WK>(p1, b, lds);
+    else pair_tile<true, false, WM, WN, MB, WK>(p2, b - first, lds);
+}
+
 // Sums the large tiles' split partials in split order, then applies the
 // epilogue. VEC: four consecutive columns per thread (n, ldc multiples of 4,
 // 16-byte aligned C, residual and partials), four splits' loads in flight.
@@ -1199,6 +1255,31 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
         launch_form<EPI_STORE>(ctx, p, grid, ta, tb, tile);
     }
     check_hip(hipGetLastError(), "gemm launch");
+}
+
+void launch_gemm_pair(Context &ctx, const KParams &p1, const KParams &p2, bool tb1, int tile) {
+    const int64_t g1 = (int64_t)p1.tiles_m * p1.tiles_n * p1.splits, first = (g1 + 7) / 8 * 8;
+    const int64_t g2 = (int64_t)p2.tiles_m * p2.tiles_n * p2.splits;
+    if (first + g2 > 0x7fffffff) fail(MMH_ERR_SHAPE, "gemm: grid too large");
+    const dim3 grid((unsigned)(first + g2));
+#define MMH_GEMM_PAIR(WM, WN, MB, WK)                                                                    \
+    do {                                                                                                 \
+        if (tb1)                                                                                         \
+            hipLaunchKernelGGL((gemm_f32_split_pair<true, WM, WN, MB, WK>), grid, dim3(WM * WN * WK * 64), 0, \
+                               ctx.stream, p1, p2, (int)first);                                          \
+        else                                                                                             \
+            hipLaunchKernelGGL((gemm_f32_split_pair<false, WM, WN, MB, WK>), grid, dim3(WM * WN * WK * 64), 0, \
+                               ctx.stream, p1, p2, (int)first);                                          \
+    } while (0)
+    switch (tile) {
+        case TILE_256: MMH_GEMM_PAIR(2, 4, 4, 1); break;
+        case TILE_256x128: MMH_GEMM_PAIR(4, 2, 2, 1); break;
+        case TILE_128: MMH_GEMM_PAIR(2, 2, 2, 2); break;
+        case TILE_128x64: MMH_GEMM_PAIR(4, 1, 1, 2); break;
+        case TILE_64: MMH_GEMM_PAIR(2, 1, 1, 4); break;
+    }
+#undef MMH_GEMM_PAIR
+    check_hip(hipGetLastError(), "gemm pair launch");
 }
 
 void launch_splitk_reduce(Context &ctx, const KParams &p, int epi) {

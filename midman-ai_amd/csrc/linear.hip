@@ -141,8 +141,8 @@ void check_linear(int32_t form, int64_t rows, int64_t k, int64_t n, int32_t act)
         fail(MMH_ERR_ARGUMENT, "linear: unknown activation " + std::to_string(act));
 }
 
-void product(Context &cx, const float *a, bool ta, const float *b, bool tb, float *c, int64_t m,
-             int64_t k, int64_t n, const LinearTail *tail = nullptr) {
+GemmDesc product(const float *a, bool ta, const float *b, bool tb, float *c, int64_t m, int64_t k,
+                 int64_t n) {
     GemmDesc g;
     g.a = a;
     g.ta = ta;
@@ -156,11 +156,7 @@ void product(Context &cx, const float *a, bool ta, const float *b, bool tb, floa
     g.k = k;
     g.n = n;
     g.split_bytes = kTrainSplitBytes;
-    if (tail) {
-        g.epi = EPI_LINEAR;
-        g.tail = tail;
-    }
-    gemm(cx, g);
+    return g;
 }
 
 }  // namespace
@@ -222,7 +218,10 @@ int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w,
         tail.out = out;
         tail.act = activation;
         tail.drop = d;
-        product(cx, x, false, w, form == MMH_GEMM_NT, nullptr, rows, k, n, &tail);
+        GemmDesc g = product(x, false, w, form == MMH_GEMM_NT, nullptr, rows, k, n);
+        g.epi = EPI_LINEAR;
+        g.tail = &tail;
+        gemm(cx, g);
         return MMH_OK;
     });
 }
@@ -268,9 +267,12 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
             check_hip(hipGetLastError(), "linear dpre launch");
             if (several) launch_sum_rows(cx, sums, strips, n, dbias);
         }
-        if (dx) product(cx, dpre, false, w, !nt, dx, rows, n, k);
-        if (dw && !nt) product(cx, x, true, dpre, false, dw, k, rows, n);
-        if (dw && nt) product(cx, dpre, true, x, false, dw, n, rows, k);
+        const GemmDesc to_x = product(dpre, false, w, !nt, dx, rows, n, k);
+        const GemmDesc to_w = nt ? product(dpre, true, x, false, dw, n, rows, k)
+                                 : product(x, true, dpre, false, dw, k, rows, n);
+        if (dx && dw) gemm_pair(cx, to_x, to_w);
+        else if (dx) gemm(cx, to_x);
+        else if (dw) gemm(cx, to_w);
         return MMH_OK;
     });
 }

@@ -459,7 +459,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     float *z = ws + packed, *part = z + round64(block * ld);
     float *zt = part + round64(block * units * 2), *dxk = all ? dx : zt + kFewRows;
     const float scale = 1.0f / (float)r.kept;
-    // dz of the rows at .. at + rows in z, and their dx
+    // dz of the rows at .. at + rows in zp
     auto logits = [&](float *zp, int64_t at, int64_t rows) {
         GemmDesc g = head_product(h, r.x + at * h.d, rows);
         g.c = zp;
@@ -485,44 +485,52 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
             gemm(cx, g);
             launch_loss_rows<true>(cx, zp, r.targets + at, rows, ld, h.vocab, scale, row_loss + at);
         }
-        if (dx) {  // dz [rows, vocab] . op(W)^T
-            GemmDesc p;
-            p.a = zp;
-            p.b = h.w;
-            p.c = dxk + at * h.d;
-            p.m = rows;
-            p.k = h.vocab;
-            p.n = h.d;
-            p.lda = ld;
-            p.tb = !nt;
-            p.ldb = nt ? h.d : h.vocab;
-            p.ldc = h.d;
-            p.split_bytes = kTrainSplitBytes;
-            gemm(cx, p);
-        }
     };
+    // dx of the rows at .. at + rows: dz [rows, vocab] . op(W)^T
+    auto dx_product = [&](const float *zp, int64_t at, int64_t rows) {
+        GemmDesc p;
+        p.a = zp;
+        p.b = h.w;
+        p.c = dxk + at * h.d;
+        p.m = rows;
+        p.k = h.vocab;
+        p.n = h.d;
+        p.lda = ld;
+        p.tb = !nt;
+        p.ldb = nt ? h.d : h.vocab;
+        p.ldc = h.d;
+        p.split_bytes = kTrainSplitBytes;
+        return p;
+    };
+    // a block's share of dW: x^T dz [d, vocab], or dz^T x [vocab, d]; later blocks are added
+    auto dw_product = [&](int64_t at, int64_t rows) {
+        GemmDesc p;
+        p.a = nt ? z : r.x + at * h.d;
+        p.b = nt ? r.x + at * h.d : z;
+        p.c = dw;
+        p.m = nt ? h.vocab : h.d;
+        p.k = rows;
+        p.n = nt ? h.d : h.vocab;
+        p.ta = true;
+        p.lda = nt ? ld : h.d;
+        p.ldb = nt ? h.d : ld;
+        p.ldc = p.n;
+        p.split_bytes = kTrainSplitBytes;
+        p.epi = at ? EPI_ACCUM : EPI_STORE;
+        return p;
+    };
+    const int64_t weights = h.d * h.vocab;
     for (int64_t at = 0; at < r.kept; at += block) {
-        const int64_t rows = std::min(block, r.kept - at);
-        for (int64_t sub = 0, n; sub < rows; sub += n) {
-            n = part_rows(rows, sub, h.d * h.vocab);
-            logits(z + sub * ld, at + sub, n);
+        const int64_t rows = std::min(block, r.kept - at), most = part_rows(rows, 0, weights);
+        logits(z, at, most);
+        if (most < rows) logits(z + most * ld, at + most, rows - most);
+        if (dx && dw && at == 0) {
+            gemm_pair(cx, dx_product(z, at, most), dw_product(at, rows));
+        } else {
+            if (dx) gemm(cx, dx_product(z, at, most));
+            if (dw) gemm(cx, dw_product(at, rows));
         }
-        if (dw) {  // x^T dz [d, vocab], or dz^T x [vocab, d]; later blocks are added
-            GemmDesc p;
-            p.a = nt ? z : r.x + at * h.d;
-            p.b = nt ? r.x + at * h.d : z;
-            p.c = dw;
-            p.m = nt ? h.vocab : h.d;
-            p.k = rows;
-            p.n = nt ? h.d : h.vocab;
-            p.ta = true;
-            p.lda = nt ? ld : h.d;
-            p.ldb = nt ? h.d : ld;
-            p.ldc = p.n;
-            p.split_bytes = kTrainSplitBytes;
-            p.epi = at ? EPI_ACCUM : EPI_STORE;
-            gemm(cx, p);
-        }
+        if (dx && most < rows) gemm(cx, dx_product(z + most * ld, at + most, rows - most));
     }
     if (!all && dx) {
         hipLaunchKernelGGL(spread_rows_kernel, dim3((unsigned)std::min<int64_t>(h.n, 65536)), dim3(256), 0,

@@ -90,6 +90,8 @@ constexpr GemmTileInfo kGemmTiles[TILE_COUNT] = {
 bool gemm_tile_takes(const KParams &p, int epi, int tile);
 void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool tb, int epi,
                        int tile);
+// An nn or nt product and a tn one in one launch of tiles of one shape, both stored.
+void launch_gemm_pair(Context &ctx, const KParams &p1, const KParams &p2, bool tb1, int tile);
 void launch_splitk_reduce(Context &ctx, const KParams &p, int epi);
 
 }  // namespace mmh

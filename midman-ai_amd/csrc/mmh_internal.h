@@ -191,6 +191,9 @@ struct GemmDesc {
 };
 
 void gemm(Context &ctx, const GemmDesc &d);
+// Two plain products (EPI_STORE, batch 1) that do not depend on each other: a an nn
+// or nt one, b a tn one. In one launch where that is estimated faster than two.
+void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b);
 // Whether gemm() folds the A-row norm and the RoPE of d into its kernel (so a
 // caller can time or schedule them as kernels of their own otherwise).
 struct GemmFusion {

@@ -243,6 +243,35 @@ def test_linear_backward(ctx, i, form):
         near(got[name], value, tol, name)
 
 
+@pytest.mark.parametrize("form", [0, 1])
+@pytest.mark.parametrize("shape", [(40, 33, 70), (512, 384, 1500), (1003, 517, 770), (256, 1500, 5632), (1500, 3000, 768),
+                                   (3000, 256, 2816)])
+def test_backward_values_outside_the_split(ctx, shape, form):
+    """A NaN and an infinity of dout, and values from 2^104 on, reach their row of dx and their column of dW alone, in
+    products that run by themselves and together."""
+    rows, k, n = shape
+    print(f"\n[backward, values outside the split] {shape} {form}", flush=True)
+    x, w, _, dout = operands(rows, k, n, 51)
+    x[np.abs(x) < 1e-3] = 0.5  # (an infinity times 0 would be NaN)
+    w[np.abs(w) < 1e-6] = 0.5
+    clean = dout.copy()
+    bad = [(5, 3), (9, 11)]
+    for r, c in bad:
+        clean[r, c] = 0
+    dout = clean.copy()
+    dout[5, 3], dout[9, 11] = np.nan, np.inf
+    dout[20, 17] = clean[20, 17] = np.float32(2.0) ** 105
+    got = run_backward(ctx, form, x, w, None, dout, "none", 0.0, 0, 0)
+    want = R.linear_backward(x, w, None, clean, "none", 0.0, 0, 0)
+    ok_rows, ok_cols = np.setdiff1d(np.arange(rows), [5, 9]), np.setdiff1d(np.arange(n), [3, 11])
+    near(got["dx"][ok_rows], want["dx"][0][ok_rows], want["dx"][1][ok_rows], "dx")
+    near(got["dw"][:, ok_cols], want["dw"][0][:, ok_cols], want["dw"][1][:, ok_cols], "dw")
+    near(got["dbias"][ok_cols], want["dbias"][0][ok_cols], want["dbias"][1][ok_cols], "dbias")
+    assert np.isnan(got["dx"][5]).all() and np.isnan(got["dw"][:, 3]).all() and np.isnan(got["dbias"][3])
+    assert np.array_equal(got["dx"][9], np.sign(w[:, 11]) * np.float32(np.inf))
+    assert np.array_equal(got["dw"][:, 11], np.sign(x[9]) * np.float32(np.inf)) and got["dbias"][11] == np.inf
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("outs", [("dx",), ("dw",), ("dbias",), ("dw", "dbias"), ("dx", "dw"), ()])
 def test_linear_backward_outputs_and_alignments(ctx, act, outs):
