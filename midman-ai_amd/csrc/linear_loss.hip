@@ -570,7 +570,9 @@ int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const fl
         const Span sx{x, n * d, "x"}, sw{w, d * vocab, "w"}, gx{dx, n * d, "dx"}, gw{dw, d * vocab, "dw"};
         apart(gx, {sx, sw, gw});
         apart(gw, {sx, sw});
-        backward(context(ctx), h, dx, dw, loss_host);
+        if (dx || dw) backward(context(ctx), h, dx, dw, loss_host);
+        else if (loss_host) forward(context(ctx), h, loss_host);
+        else context(ctx);
         return MMH_OK;
     });
 }
