@@ -1503,10 +1503,12 @@ void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b) {
                 for (int j = 0; j < counts[1]; ++j) {
                     const double l1 = steps[0] / kCounts[i] + t.setup, l2 = steps[1] / kCounts[j] + t.setup;
                     const double g1 = (double)(tiles[0] * kCounts[i]), g2 = (double)(tiles[1] * kCounts[j]);
-                    const double full = (g1 * l1 + g2 * l2) / cus * t.full + cost[0][i] + cost[1][j] + 3.0;
+                    // (a launch, and one for the sums of both)
+                    const double more = cost[0][i] + cost[1][j] + 3.0 - (i > 0 && j > 0 ? 4.0 : 0.0);
+                    const double full = (g1 * l1 + g2 * l2) / cus * t.full + more;
                     if (full >= best.us) continue;
-                    const double us = std::max(full, list_end(cus, (int64_t)g1, l1, (int64_t)g2, l2) * t.alone +
-                                                         cost[0][i] + cost[1][j] + 3.0);
+                    const double us =
+                        std::max(full, list_end(cus, (int64_t)g1, l1, (int64_t)g2, l2) * t.alone + more);
                     if (us >= best.us) continue;
                     found = true;
                     best.us = us;
@@ -1534,8 +1536,7 @@ void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b) {
         p[1].partial = partial + floats[0];
     }
     launch_gemm_pair(ctx, p[0], p[1], a.tb, best.tile);
-    for (const KParams &x : p)
-        if (x.splits > 1) launch_splitk_reduce(ctx, x, EPI_STORE);
+    launch_splitk_reduce_pair(ctx, p[0], p[1]);
 }
 
 double mfma_peak_tflops(Context &ctx) {

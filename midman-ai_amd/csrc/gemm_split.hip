@@ -1110,14 +1110,14 @@ __global__ __launch_bounds__(WM *WN *WK * 64, 2) void gemm_f32_split_pair(KParam
 // Sums the large tiles' split partials in split order, then applies the
 // epilogue. VEC: four consecutive columns per thread (n, ldc multiples of 4,
 // 16-byte aligned C, residual and partials), four splits' loads in flight.
+// (block of blocks: the workgroup's place in the launch.)
 template <int EPI, bool VEC>
-__global__ __launch_bounds__(256) void splitk_reduce(const float *__restrict__ partial,
-                                                     float *c, const float *resid, int64_t m,
-                                                     int64_t n, int64_t ldc, int splits) {
+__device__ __forceinline__ void reduce_splits(const float *__restrict__ partial, float *c,
+                                              const float *resid, int64_t m, int64_t n, int64_t ldc,
+                                              int splits, int64_t block, int64_t blocks) {
     const int64_t total = m * n;
     if (VEC) {
-        for (int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; 4 * q < total;
-             q += (int64_t)gridDim.x * blockDim.x) {
+        for (int64_t q = block * 256 + threadIdx.x; 4 * q < total; q += blocks * 256) {
             const int64_t idx = 4 * q;
             float4 acc = *reinterpret_cast<const float4 *>(partial + idx);
             for (int s0 = 1; s0 < splits; s0 += 4) {
@@ -1148,8 +1148,7 @@ __global__ __launch_bounds__(256) void splitk_reduce(const float *__restrict__ p
         }
         return;
     }
-    for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < total;
-         idx += (int64_t)gridDim.x * blockDim.x) {
+    for (int64_t idx = block * 256 + threadIdx.x; idx < total; idx += blocks * 256) {
         float acc = partial[idx];
         for (int s = 1; s < splits; ++s) acc = __fadd_rn(acc, partial[(int64_t)s * total + idx]);
         const int64_t row = idx / n, col = idx - row * n;
@@ -1159,6 +1158,23 @@ __global__ __launch_bounds__(256) void splitk_reduce(const float *__restrict__ p
         else
             *dst = acc;
     }
+}
+
+template <int EPI, bool VEC>
+__global__ __launch_bounds__(256) void splitk_reduce(const float *__restrict__ partial, float *c,
+                                                     const float *resid, int64_t m, int64_t n,
+                                                     int64_t ldc, int splits) {
+    reduce_splits<EPI, VEC>(partial, c, resid, m, n, ldc, splits, blockIdx.x, gridDim.x);
+}
+// The sums of a pair's two products (stored), the first `first` workgroups the first's.
+template <bool VEC1, bool VEC2>
+__global__ __launch_bounds__(256) void splitk_reduce_pair(KParams p1, KParams p2, int first) {
+    const int b = blockIdx.x;
+    if (b < first)
+        reduce_splits<EPI_STORE, VEC1>(p1.partial, p1.c, nullptr, p1.m, p1.n, p1.ldc, p1.splits, b, first);
+    else
+        reduce_splits<EPI_STORE, VEC2>(p2.partial, p2.c, nullptr, p2.m, p2.n, p2.ldc, p2.splits, b - first,
+                                       (int)gridDim.x - first);
 }
 
 // The same for EPI_LINEAR: the sums in split order, then the layer's epilogue,
@@ -1282,6 +1298,17 @@ void launch_gemm_pair(Context &ctx, const KParams &p1, const KParams &p2, bool t
     check_hip(hipGetLastError(), "gemm pair launch");
 }
 
+namespace {
+bool reduce_vec(const KParams &p) {
+    return p.n % 4 == 0 && p.ldc % 4 == 0 && aligned16(p.c) && aligned16(p.partial) &&
+           (!p.resid || aligned16(p.resid));
+}
+unsigned reduce_blocks(const KParams &p, bool vec) {
+    const int64_t items = vec ? p.m * p.n / 4 : p.m * p.n;
+    return (unsigned)std::min<int64_t>((items + 255) / 256, 8192);
+}
+}  // namespace
+
 void launch_splitk_reduce(Context &ctx, const KParams &p, int epi) {
     if (epi == EPI_LINEAR) {
         const int64_t units = p.m * ((p.n + 3) / 4);
@@ -1290,11 +1317,8 @@ void launch_splitk_reduce(Context &ctx, const KParams &p, int epi) {
         check_hip(hipGetLastError(), "split-k linear launch");
         return;
     }
-    const int64_t total = p.m * p.n;
-    const bool vec = p.n % 4 == 0 && p.ldc % 4 == 0 && aligned16(p.c) && aligned16(p.partial) &&
-                     (!p.resid || aligned16(p.resid));
-    const int64_t items = vec ? total / 4 : total;
-    const unsigned blocks = (unsigned)std::min<int64_t>((items + 255) / 256, 8192);
+    const bool vec = reduce_vec(p);
+    const unsigned blocks = reduce_blocks(p, vec);
 #define MMH_SPLITK(E, V)                                                                     \
     hipLaunchKernelGGL((splitk_reduce<E, V>), dim3(blocks), dim3(256), 0, ctx.stream, p.partial, \
                        p.c, p.resid, p.m, p.n, p.ldc, p.splits)
@@ -1304,6 +1328,24 @@ void launch_splitk_reduce(Context &ctx, const KParams &p, int epi) {
         if (vec) MMH_SPLITK(EPI_STORE, true); else MMH_SPLITK(EPI_STORE, false);
     }
 #undef MMH_SPLITK
+    check_hip(hipGetLastError(), "split-k reduce launch");
+}
+
+void launch_splitk_reduce_pair(Context &ctx, const KParams &p1, const KParams &p2) {
+    if (p1.splits == 1 || p2.splits == 1) {
+        for (const KParams *p : {&p1, &p2})
+            if (p->splits > 1) launch_splitk_reduce(ctx, *p, EPI_STORE);
+        return;
+    }
+    const bool v1 = reduce_vec(p1), v2 = reduce_vec(p2);
+    const unsigned first = reduce_blocks(p1, v1), blocks = first + reduce_blocks(p2, v2);
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, ctx.stream, p1, p2, (int)first);
+    };
+    if (v1 && v2) launch(splitk_reduce_pair<true, true>);
+    else if (v1) launch(splitk_reduce_pair<true, false>);
+    else if (v2) launch(splitk_reduce_pair<false, true>);
+    else launch(splitk_reduce_pair<false, false>);
     check_hip(hipGetLastError(), "split-k reduce launch");
 }
 

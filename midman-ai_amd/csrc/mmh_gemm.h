@@ -93,5 +93,7 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
 // An nn or nt product and a tn one in one launch of tiles of one shape, both stored.
 void launch_gemm_pair(Context &ctx, const KParams &p1, const KParams &p2, bool tb1, int tile);
 void launch_splitk_reduce(Context &ctx, const KParams &p, int epi);
+// The split sums of a pair, those there are, in one launch.
+void launch_splitk_reduce_pair(Context &ctx, const KParams &p1, const KParams &p2);
 
 }  // namespace mmh
