@@ -455,12 +455,13 @@ int32_t mmh_dropout_backward(mmh_handle ctx, const float *dout, int64_t n, float
 int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w, const float *bias,
                    const float *residual, int64_t rows, int64_t k, int64_t n, int32_t activation,
                    float p, uint64_t seed, uint64_t offset, float *pre, float *out);
-/* Its backward for dout [rows, n]: dpre = dropout(dout) * act'(pre), dx = dpre
+/* Its backward for dout [rows, n]: dpre = dropout(dout * act'(pre)), dx = dpre
  * op(w)^T, dw = x^T dpre in w's layout, dbias the column sums of dpre (d residual
  * is dout itself). pre as the forward call left it; NULL for MMH_ACT_NONE. Any
  * of dx, dw, dbias may be NULL (not needed), and then w (for dx), x (for dw) too.
- * Outputs are overwritten. The derivative of relu at 0 is 0. dpre takes rows * n
- * floats of the context's workspace where it is not dout itself. */
+ * Outputs are overwritten. The derivative of relu at 0 is 0. A dropped value of
+ * dpre is 0 whatever dout and pre hold there; at a kept one a NaN of either stays.
+ * dpre takes rows * n floats of the context's workspace where it is not dout itself. */
 int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const float *w,
                             const float *pre, const float *dout, int64_t rows, int64_t k, int64_t n,
                             int32_t activation, float p, uint64_t seed, uint64_t offset, float *dx,

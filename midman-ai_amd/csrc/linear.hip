@@ -1,7 +1,7 @@
 // The linear layer with its epilogue, and dropout.
 //
 //   pre = x op(W) + bias,  out = residual + dropout(act(pre))
-//   dpre = dropout(dout) * act'(pre),  dbias = column sums of dpre,
+//   dpre = dropout(dout * act'(pre)),  dbias = column sums of dpre,
 //   dx = dpre op(W)^T,  dW = x^T dpre (or its transpose)
 //
 // Dropout's mask is drawn again wherever it is needed, from the call's key and
@@ -83,7 +83,7 @@ void launch_dropout(Context &ctx, const float *x, const float *residual, int64_t
     check_hip(hipGetLastError(), "dropout launch");
 }
 
-// dpre = dropout(dout) * act'(pre) (written where WRITE) and the column sums of
+// dpre = dropout(dout * act'(pre)) (written where WRITE) and the column sums of
 // a strip of rows of it. A wave walks rows of 256 columns, four per lane: 16-byte
 // accesses, one generator block per four values. Bound by its reads and writes (4096 x
 // 5632: 59 us, 4.7 TB/s).
@@ -102,8 +102,15 @@ __global__ __launch_bounds__(256) void linear_dpre_kernel(const float *dout, con
             float v[4], x[4] = {};
             load4(dout + i, count, v);
             if (act != MMH_ACT_NONE) load4(pre + i, count, x);
-            if (d.on) drop4(d, i, v);
+            // (drawn while the loads are on their way, applied last: a dropped value is 0
+            // whatever dout and pre hold)
+            uint32_t w[4] = {};
+            if (d.on) drop_words4(d, i, w);
             activate_grad4(act, x, v);
+            if (d.on) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = drop_word(d, w[j], v[j]);
+            }
             if (WRITE) store4(dpre + i, count, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] += v[j];

@@ -43,7 +43,7 @@ __device__ __forceinline__ float tanh_arg2(float x) {
 // erfcx is a polynomial in t = 1 / (1 + 0.35 |x| / sqrt 2), fitted here to the
 // least largest relative error over |x| <= 13.15, 1.4e-8 (beyond, e is 0 in f32).
 __device__ __forceinline__ float normal_tail(float x, float &e) {
-    const float ax = fminf(fabsf(x), 15.0f), sq = ax * ax;
+    const float ax = fabsf(x) > 15.0f ? 15.0f : fabsf(x), sq = ax * ax;  // (a NaN stays)
     e = exp_neg(-0.5f * sq);
     e = __builtin_fmaf(e, -0.5f * __builtin_fmaf(ax, ax, -sq), e);
     const float t = reciprocal(__builtin_fmaf(0.247487373f, ax, 1.0f));
@@ -107,10 +107,10 @@ __device__ __forceinline__ void activate4(int act, float (&v)[4]) {
         default: break;
     }
 }
-// dh *= act'(x)
+// dh *= act'(x); a NaN of x stays one in every activation's (relu's slope at 0 is 0)
 __device__ __forceinline__ void activate_grad4(int act, const float (&x)[4], float (&dh)[4]) {
     switch (act) {
-        case MMH_ACT_RELU: MMH_EACH4(dh[j] = x[j] > 0.0f ? dh[j] : 0.0f); break;
+        case MMH_ACT_RELU: MMH_EACH4(dh[j] = x[j] > 0.0f ? dh[j] : x[j] <= 0.0f ? 0.0f : x[j]); break;
         case MMH_ACT_GELU: MMH_EACH4(dh[j] *= gelu_slope(x[j])); break;
         case MMH_ACT_GELU_TANH: MMH_EACH4(dh[j] *= gelu_tanh_slope(x[j])); break;
         case MMH_ACT_SILU: MMH_EACH4(dh[j] *= silu_slope(x[j])); break;
@@ -150,12 +150,12 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint32_t k0, uint32_t k1
 __device__ __forceinline__ float drop_word(const Drop &d, uint32_t word, float x) {
     return word <= d.last ? 0.0f : x * d.scale;
 }
-// Values i .. i + 3 of an array: one block where they are its four words, else
-// two that follow each other.
-__device__ __forceinline__ void drop4(const Drop &d, int64_t i, float (&v)[4]) {
+// The words of values i .. i + 3 of an array: one block where they are its four
+// words, else two that follow each other.
+__device__ __forceinline__ void drop_words4(const Drop &d, int64_t i, uint32_t (&w)[4]) {
     const uint64_t block = d.offset + ((uint64_t)i >> 2);
     const uint4 a = philox(block, d.k0, d.k1);
-    uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
     const int first = (int)(i & 3);
     if (first) {
         const uint4 b = philox(block + 1, d.k0, d.k1);
@@ -163,6 +163,10 @@ __device__ __forceinline__ void drop4(const Drop &d, int64_t i, float (&v)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = first == 1 ? e[j + 1] : first == 2 ? e[j + 2] : e[j + 3];
     }
+}
+__device__ __forceinline__ void drop4(const Drop &d, int64_t i, float (&v)[4]) {
+    uint32_t w[4];
+    drop_words4(d, i, w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = drop_word(d, w[j], v[j]);
 }

@@ -272,6 +272,27 @@ def test_backward_values_outside_the_split(ctx, shape, form):
     assert np.array_equal(got["dw"][:, 11], np.sign(x[9]) * np.float32(np.inf)) and got["dbias"][11] == np.inf
 
 
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_backward_of_infinite_and_missing_values(ctx, act, p):
+    """One row, so that dbias is dpre: NaN and infinities of pre, and of dout, where the mask keeps them and where it drops
+    them (0 there). The slope is 1 at inf and 0 at -inf, a NaN stays one."""
+    n, seed, offset = 96, 31, 5
+    keep = R.kept(n, p, seed, offset)
+    pre = np.resize(np.array([np.nan, np.inf, -np.inf, 0.75], np.float32), n)
+    dout = np.repeat(np.array([1.5, -2.0, np.nan], np.float32), n // 3)
+    x, w = np.ones((1, 3), np.float32), np.ones((3, n), np.float32)
+    got = run_backward(ctx, 0, x, w, pre[None], dout[None], act, p, seed, offset, outs=("dbias",))["dbias"]
+    assert not p or 0 < keep.sum() < n
+    assert (got[~keep] == 0).all()
+    bad = keep & (np.isnan(pre) | (np.isnan(dout) & ((pre > 0) | (act != "relu"))))
+    assert np.isnan(got[bad]).all()
+    scale = np.float32(1.0 / (1.0 - p))
+    for value, slope in ((np.inf, 1.0), (-np.inf, 0.0)):
+        at = keep & (pre == np.float32(value)) & ~np.isnan(dout)
+        assert np.array_equal(got[at], dout[at] * scale * np.float32(slope)), (act, value)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("outs", [("dx",), ("dw",), ("dbias",), ("dw", "dbias"), ("dx", "dw"), ()])
 def test_linear_backward_outputs_and_alignments(ctx, act, outs):
