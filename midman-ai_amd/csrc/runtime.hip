@@ -21,8 +21,9 @@ std::vector<std::unique_ptr<Context>> g_contexts;  // handle = index + 1
 }  // namespace
 
 void check_hip(hipError_t e, const char *what) {
-    if (e != hipSuccess)
-        fail(MMH_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e));
+    if (e == hipSuccess) return;
+    (void)hipGetLastError();  // (kept by the runtime, the next launch check would report it again)
+    fail(MMH_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e));
 }
 
 void *Context::get_scratch(size_t bytes) { return workspace(0, bytes); }

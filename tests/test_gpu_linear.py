@@ -630,6 +630,14 @@ def test_a_refused_call_runs_nothing(ctx):
     assert (dx.numpy() == 3).all() and (dw.numpy() == 4).all() and np.array_equal(X.numpy(), x)
 
 
+def test_a_failed_allocation_fails_no_later_call(ctx):
+    """The runtime keeps the error of an allocation until it is asked for; the next call's launch is not that call."""
+    X = ctx.to_device(np.arange(64, dtype=np.float32))
+    with pytest.raises(mh.DeviceError):
+        ctx.empty((1 << 45,))
+    assert np.array_equal(mh.dropout(ctx, X, 0.0, 1).numpy(), np.arange(64, dtype=np.float32))
+
+
 def test_two_threads_with_a_context_each(ctx):
     """Calls of two threads at once, each on its own context, give what they give alone."""
     import threading
