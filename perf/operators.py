@@ -86,18 +86,15 @@ def draw(rng):
 # ---- inputs --------------------------------------------------------------------
 
 _context = None
-_module = None
 
 
 def _mh():
-    """The library's Python mirror, looked up once."""
-    global _module
-    if _module is None:
-        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-        sys.path.insert(0, os.path.join(root, "midman-ai_amd"))
-        import midman_hip
-        _module = midman_hip
-    return _module
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.path.join(root, "midman-ai_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import midman_hip
+    return midman_hip
 
 
 def _ctx():
