@@ -445,6 +445,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
         if (loss_host) *loss_host = 0.0f;
         if (dx) launch_fill(cx, dx, h.n * h.d, 0.0f);
         if (dw) launch_fill(cx, dw, h.d * h.vocab, 0.0f);
+        check_hip(hipStreamSynchronize(cx.stream), "loss sync");  // (like every other way out)
         return;
     }
     const bool all = r.kept == h.n, nt = h.form == MMH_GEMM_NT;
