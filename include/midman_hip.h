@@ -460,7 +460,8 @@ int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w,
  * is dout itself). pre as the forward call left it; NULL for MMH_ACT_NONE. Any
  * of dx, dw, dbias may be NULL (not needed), and then w (for dx), x (for dw) too.
  * Outputs are overwritten. The derivative of relu at 0 is 0. A dropped value of
- * dpre is 0 whatever dout and pre hold there; at a kept one a NaN of either stays.
+ * dpre is 0 whatever dout and pre hold there; at a kept one a NaN of either stays,
+ * and an infinity of dout times a slope of 0 is a NaN.
  * dpre takes rows * n floats of the context's workspace where it is not dout itself. */
 int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const float *w,
                             const float *pre, const float *dout, int64_t rows, int64_t k, int64_t n,

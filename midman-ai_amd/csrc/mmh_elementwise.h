@@ -107,10 +107,11 @@ __device__ __forceinline__ void activate4(int act, float (&v)[4]) {
         default: break;
     }
 }
-// dh *= act'(x); a NaN of x stays one in every activation's (relu's slope at 0 is 0)
+// dh *= act'(x); a NaN of x or dh stays one in every activation's (relu's slope at 0 is
+// 0, and the product with it is taken: an infinity of dh times 0 is a NaN)
 __device__ __forceinline__ void activate_grad4(int act, const float (&x)[4], float (&dh)[4]) {
     switch (act) {
-        case MMH_ACT_RELU: MMH_EACH4(dh[j] = x[j] > 0.0f ? dh[j] : x[j] <= 0.0f ? 0.0f : x[j]); break;
+        case MMH_ACT_RELU: MMH_EACH4(dh[j] = x[j] > 0.0f ? dh[j] : x[j] <= 0.0f ? dh[j] * 0.0f : x[j]); break;
         case MMH_ACT_GELU: MMH_EACH4(dh[j] *= gelu_slope(x[j])); break;
         case MMH_ACT_GELU_TANH: MMH_EACH4(dh[j] *= gelu_tanh_slope(x[j])); break;
         case MMH_ACT_SILU: MMH_EACH4(dh[j] *= silu_slope(x[j])); break;

@@ -38,3 +38,24 @@ def test_a_loss_of_ignored_rows_alone_waits_for_its_zeros(ctx, grads):
             assert (got == 0).all(), name
     for a in (A, C):
         a.free()
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_relu_backward_is_the_product_with_its_slope(ctx, p, shift):
+    """dout * (pre > 0) by IEEE: a NaN of dout stays one where the slope is 0 too, an infinity becomes one there, finite
+    values become 0; the others' formula (dout times slope) has it the same way, and a dropped value is 0 whatever it was.
+    One row, so that dbias is dpre."""
+    n, seed, offset = 120, 41, 9
+    pre = np.tile(np.array([-2, 0, -0.0, 3, -np.inf, np.inf], np.float32), n // 6)
+    dout = np.repeat(np.array([np.nan, np.inf, -np.inf, 1.5, -2.5], np.float32), n // 5)
+    keep = R.kept(n, p, seed, offset)
+    with np.errstate(invalid="ignore"):
+        want = np.where(keep, dout * (pre > 0).astype(np.float32) * np.float32(1 / (1 - p)), np.float32(0))
+    x, w = np.ones((1, 3), np.float32), np.ones((3, n), np.float32)
+    got = run_backward(ctx, 0, x, w, pre[None], dout[None], "relu", p, seed, offset, shift, outs=("dbias",))["dbias"]
+    assert np.isnan(want).any() and np.array_equal(got, want, equal_nan=True)
+    # a NaN of pre stays one beside any dout
+    got = run_backward(ctx, 0, x, w, np.full((1, n), np.nan, np.float32), dout[None], "relu", p, seed, offset, shift,
+                       outs=("dbias",))["dbias"]
+    assert np.isnan(got[keep]).all() and (got[~keep] == 0).all()
