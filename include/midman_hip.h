@@ -472,8 +472,12 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
  * `ignore` (any value, -1 say) are left out: the mean is over the others, and
  * nothing the row holds is read. With no row left the loss is 0. Other targets
  * outside [0, vocab) are MMH_ERR_INDEX, and nothing runs. However many rows there
- * are, the context's workspace holds the logits of a block of them: 512 MiB of
- * rows, or 128 rows where those are more. Both calls wait for their work (the
+ * are, the context's workspace holds the logits of a block of them (in place of
+ * those, partial sums where the loss alone is asked for): 512 MiB, or 128 rows where
+ * those are more. Beside them it holds the products' split partials (256 MiB at
+ * most), 8 bytes per row of the block and 128 columns for vocabularies above 32768,
+ * and, with any row ignored, the kept rows of x and of dx, packed; per row 8 bytes of
+ * pinned host memory, 16 with any row ignored. Both calls wait for their work (the
  * targets have been read and the loss is there when they return). */
 int32_t mmh_linear_cross_entropy(mmh_handle ctx, int32_t form, const float *x, const float *w,
                                  const int32_t *targets_host, int64_t n, int64_t d, int64_t vocab,

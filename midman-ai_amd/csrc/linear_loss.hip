@@ -20,11 +20,7 @@
 namespace mmh {
 namespace {
 
-// The workspace of a block's logits, and the rows that a block has at least. Twice
-// as large as 256 MiB, since a block's last tiles of rows and what its part adds to
-// dW are paid per block: 817 rows x 1024 x 131071 4510 -> 4020 us, 4096 x 2048 x
-// 32000 7585 -> 7445.
-constexpr int64_t kLogitBytes = int64_t(512) << 20;
+// The rows that a block has at least.
 constexpr int64_t kMinRows = 128;
 // Up to so many rows the loss takes stored logits: the tiles that fold it have
 // 128 rows at least, those of the plain product 32 or 64 (35 rows x 1344 x 153411
@@ -46,14 +42,17 @@ int64_t part_rows(int64_t rows, int64_t at, int64_t weights) {
     return rows - tail;
 }
 
-int64_t block_rows(int64_t n, int64_t row_bytes) {
-    int64_t rows = std::max(kMinRows, kLogitBytes / row_bytes);
-    if (rows >= n) return n;
-    // blocks of one size (the last may be smaller), in whole tiles of 256 rows
-    // where a block has as many
-    const int64_t blocks = (n + rows - 1) / rows;
-    rows = (n + blocks - 1) / blocks;
-    return rows > 256 ? (rows + 255) / 256 * 256 : rows;
+// Rows of a block of n rows of row_bytes each: all, or as many as `bytes` hold, but
+// kMinRows at least. Blocks of one size (the last may be smaller), in whole tiles of
+// 256 rows where a block has as many: rounded up where that still fits, else down
+// where that takes a quarter more blocks at most.
+int64_t block_rows(int64_t n, int64_t row_bytes, int64_t bytes) {
+    const int64_t most = std::max(kMinRows, bytes / row_bytes);
+    if (most >= n) return n;
+    const int64_t blocks = (n + most - 1) / most, rows = (n + blocks - 1) / blocks;
+    if (rows <= 256) return rows;
+    const int64_t down = rows / 256 * 256, up = down == rows ? rows : down + 256;
+    return up <= most ? up : 4 * rows <= 5 * down ? down : rows;
 }
 
 // dx[i] = from[map[i]], a row of zeros where map[i] < 0.
@@ -397,7 +396,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
         return rows > kFewRows && (h.vocab > kRowCols || gemm_ce_tiles(cx, head_product(h, h.x, rows)) > 0);
     };
     const int64_t ld = logit_row(h.vocab);
-    const int64_t block = block_rows(r.kept, folds(r.kept) ? units * 8 : ld * 4);
+    const int64_t block = block_rows(r.kept, folds(r.kept) ? units * 8 : ld * 4, cx.loss_block_bytes);
     // a block's partials, or the logits of one too small for the product to fold them (the last, often)
     auto floats = [&](int64_t rows) { return rows * (folds(rows) ? units * 2 : ld); };
     const int64_t weights = h.d * h.vocab, last = (r.kept - 1) % block + 1;
@@ -450,7 +449,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
     }
     const bool all = r.kept == h.n, nt = h.form == MMH_GEMM_NT;
     const int64_t units = (h.vocab + 127) / 128;
-    const int64_t ld = logit_row(h.vocab), block = block_rows(r.kept, ld * 4);
+    const int64_t ld = logit_row(h.vocab), block = block_rows(r.kept, ld * 4, cx.loss_block_bytes);
     const size_t packed = all ? 0 : round64(r.kept * h.d);
     float *ws = static_cast<float *>(
         cx.workspace(2, (packed * (dx ? 2 : 1) + round64(block * ld) + round64(block * units * 2) + kFewRows) * 4));
@@ -548,6 +547,24 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
 using namespace mmh;
 
 extern "C" {
+
+// For the tests, not part of the C ABI: the rows of a block of n rows of row_bytes
+// within `bytes`; the bytes that a context's blocks take (0: the ordinary ones).
+int32_t mmh_test_loss_block_rows(int64_t n, int64_t row_bytes, int64_t bytes, int64_t *rows) {
+    return guard([&] {
+        need(rows, "rows");
+        positive(n, "n");
+        positive(row_bytes, "row_bytes");
+        *rows = block_rows(n, row_bytes, bytes > 0 ? bytes : kLogitBytes);
+        return MMH_OK;
+    });
+}
+int32_t mmh_test_loss_block_bytes(mmh_handle ctx, int64_t bytes) {
+    return guard([&] {
+        context(ctx).loss_block_bytes = bytes > 0 ? bytes : kLogitBytes;
+        return MMH_OK;
+    });
+}
 
 int32_t mmh_linear_cross_entropy(mmh_handle ctx, int32_t form, const float *x, const float *w,
                                  const int32_t *targets_host, int64_t n, int64_t d, int64_t vocab,

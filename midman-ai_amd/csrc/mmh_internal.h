@@ -60,6 +60,12 @@ __device__ __forceinline__ void lse_merge(float &m, float &s, float m2, float s2
 
 void check_hip(hipError_t e, const char *what);
 
+// What a block of the linear cross entropy's rows takes: its logits, or the partials
+// of the loss alone. Twice as large as 256 MiB, since a block's last tiles of rows
+// and what its part adds to dW are paid per block: 817 rows x 1024 x 131071 4510 ->
+// 4020 us, 4096 x 2048 x 32000 7585 -> 7445.
+constexpr int64_t kLogitBytes = int64_t(512) << 20;
+
 // One device + one stream + growable workspaces.
 struct Context {
     // 0 split-K partials, 1 ids, 2 op temporaries, 3 losses, 4 attention heads
@@ -92,6 +98,8 @@ struct Context {
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
     void *pinned_rows(size_t bytes);
+    // (less in tests of several blocks)
+    int64_t loss_block_bytes = kLogitBytes;
     // Allocations made through mmh_alloc, freed at destroy.
     std::vector<void *> owned;
 

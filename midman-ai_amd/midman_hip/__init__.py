@@ -712,9 +712,9 @@ def _head_args(x, w, targets, form):
 
 def linear_cross_entropy(ctx: Context, x: DeviceArray, w: DeviceArray, targets: np.ndarray,
                          form: str = "nt", ignore: int = -1) -> float:
-    """cross_entropy of the logits x op(w), which are never whole in memory:
-    x [.., d], w [vocab, d] (nt, a tied embedding) or [d, vocab] (nn). Rows whose
-    target is `ignore` are left out of the mean."""
+    """cross_entropy of the logits x op(w), which are not stored (those of 64 rows
+    at most are): x [.., d], w [vocab, d] (nt, a tied embedding) or [d, vocab] (nn).
+    Rows whose target is `ignore` are left out of the mean."""
     f, targets, n, d, vocab = _head_args(x, w, targets, form)
     loss = ctypes.c_float()
     check(lib().mmh_linear_cross_entropy(ctx.handle, f, x.ptr, w.ptr, _ip(targets), n, d, vocab,
@@ -725,7 +725,8 @@ def linear_cross_entropy(ctx: Context, x: DeviceArray, w: DeviceArray, targets: 
 def linear_cross_entropy_backward(ctx: Context, x: DeviceArray, w: DeviceArray, targets: np.ndarray,
                                   form: str = "nt", ignore: int = -1, dx: DeviceArray = None,
                                   dw: DeviceArray = None):
-    """(loss, dx, dw) of linear_cross_entropy for loss gradient 1."""
+    """(loss, dx, dw) of linear_cross_entropy for loss gradient 1. The logits of a
+    block of rows are in memory at a time, 512 MiB or 128 rows of them."""
     f, targets, n, d, vocab = _head_args(x, w, targets, form)
     _fits("linear_cross_entropy_backward: dx", dx, x.shape)
     _fits("linear_cross_entropy_backward: dw", dw, w.shape)

@@ -7,7 +7,7 @@ import pytest
 
 import linear_oracle as R
 import midman_hip as mh
-from test_gpu_linear import run_backward
+from test_gpu_linear import Box, check_loss, empty, head, run_backward, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,99 @@ def test_relu_backward_is_the_product_with_its_slope(ctx, p, shift):
     got = run_backward(ctx, 0, x, w, np.full((1, n), np.nan, np.float32), dout[None], "relu", p, seed, offset, shift,
                        outs=("dbias",))["dbias"]
     assert np.isnan(got[keep]).all() and (got[~keep] == 0).all()
+
+
+def limit_blocks(ctx, limit):
+    f = mh.lib().mmh_test_loss_block_bytes
+    f.argtypes = [ctypes.c_int64, ctypes.c_int64]
+    mh.check(f(ctx.handle, limit))
+
+
+def block_sizes(n, row_bytes, limit):
+    rows = ctypes.c_int64()
+    f = mh.lib().mmh_test_loss_block_rows
+    f.argtypes = [ctypes.c_int64] * 3 + [ctypes.POINTER(ctypes.c_int64)]
+    mh.check(f(n, row_bytes, limit, ctypes.byref(rows)))
+    return [min(rows.value, n - at) for at in range(0, n, rows.value)]
+
+
+# kept rows, rows that the bytes hold, the blocks that this gives
+BLOCKS = [(300, 128, [100, 100, 100]), (257, 128, [86, 86, 85]), (1072, 536, [512, 512, 48]), (514, 257, [256, 256, 2]),
+          (513, 510, [256, 256, 1]), (769, 511, [385, 384]), (1300, 900, [768, 532])]
+
+
+@pytest.mark.parametrize("form", [0, 1])
+@pytest.mark.parametrize("ignored", [0, 37])
+@pytest.mark.parametrize("d,V", [(40, 1003), (33, 8192), (12, 33001)])
+@pytest.mark.parametrize("kept,most,blocks", BLOCKS)
+def test_several_row_blocks(ctx, kept, most, blocks, d, V, ignored, form):
+    """Blocks of equal sizes, ones cut down to whole tiles, a last one of 48 rows, of 2, of 1; the gradients' (logits) and
+    the loss's own (partial sums where the tiles fold it), with every row kept and with some ignored."""
+    print(f"\n[several row blocks] {kept} in {blocks}, d {d} V {V} ignored {ignored} form {form}", flush=True)
+    x, w, t = head(kept + ignored, d, V, seed=kept + V)
+    if ignored:
+        t[np.random.default_rng(ignored).choice(kept + ignored, ignored, replace=False)] = -1
+        x[t < 0] = np.nan
+    want = R.cross_entropy(x if not ignored else np.nan_to_num(x), w, t, blocks=len(blocks))
+    row = (V + 31) // 32 * 32 * 4
+    folds = V > 32768 or V == 8192 and kept > 512  # (256 tiles of 128x128 and more)
+    parts = (V + 127) // 128 * 8 if folds else row
+    assert block_sizes(kept, row, most * row) == block_sizes(kept, parts, most * parts) == blocks
+    X, W = Box(ctx, x), Box(ctx, stored(w, form))
+    dx, dw = empty(ctx, x.shape), empty(ctx, stored(w, form).shape)
+    tp = t.ctypes.data_as(ctypes.POINTER(ctypes.c_int32))
+    loss = ctypes.c_float(np.nan)
+    try:
+        limit_blocks(ctx, most * row)
+        mh.check(mh.lib().mmh_linear_cross_entropy_backward(ctx.handle, form, X.ptr, W.ptr, tp, len(t), d, V, -1, dx.ptr, dw.ptr,
+                                                            ctypes.byref(loss)))
+        got = {"dx": dx.numpy(), "dw": dw.numpy().T if form else dw.numpy(), "loss": loss.value}
+        limit_blocks(ctx, most * parts)
+        mh.check(mh.lib().mmh_linear_cross_entropy(ctx.handle, form, X.ptr, W.ptr, tp, len(t), d, V, -1, ctypes.byref(loss)))
+        got["forward"] = loss.value
+    finally:
+        limit_blocks(ctx, 0)
+    check_loss(got, want)
+    assert (got["dx"][t < 0] == 0).all()
+
+
+@pytest.mark.parametrize("form", [0, 1])
+def test_row_blocks_beside_large_weights(ctx, form):
+    """Blocks whose few rows past the last 256 are a part of their own, in the first block and in later ones."""
+    d, V, kept, most = 1700, 32100, 1600, 560
+    row, parts = (V + 31) // 32 * 32 * 4, (V + 127) // 128 * 8
+    print(f"\n[row blocks beside large weights] {form}", flush=True)
+    assert d * V >= 52 << 20 and block_sizes(kept, row, most * row) == [512, 512, 512, 64]
+    x, w, t = head(kept, d, V, seed=4)
+    want = R.cross_entropy(x, w, t, blocks=4)
+    X, W = ctx.to_device(x), ctx.to_device(stored(w, form))
+    try:
+        limit_blocks(ctx, most * row)
+        loss, dx, dw = mh.linear_cross_entropy_backward(ctx, X, W, t, form=("nn", "nt")[form])
+        limit_blocks(ctx, most * parts)
+        forward = mh.linear_cross_entropy(ctx, X, W, t, form=("nn", "nt")[form])
+    finally:
+        limit_blocks(ctx, 0)
+    dw = dw.numpy().T if form else dw.numpy()
+    check_loss({"loss": loss, "forward": forward, "dx": dx.numpy(), "dw": dw}, want)
+
+
+def test_the_loss_alone_over_more_rows_than_a_block(ctx):
+    """The ordinary workspace holds the partial sums of 65536 rows of 131072 columns. The mean over more rows against that of
+    calls of one block each, both within the bound of a row's term."""
+    n, d, V = 70000, 8, 131072
+    x, w, t = head(n, d, V, seed=5)
+    t[::100] = -1
+    x[::100] = np.nan
+    keep = t >= 0
+    blocks = block_sizes(int(keep.sum()), V // 128 * 8, 0)
+    assert len(blocks) == 2
+    print(f"\n[the loss of blocks of {blocks} rows]", flush=True)
+    X, W = ctx.to_device(x), ctx.to_device(stored(w, 1))
+    whole, parts = mh.linear_cross_entropy(ctx, X, W, t), []
+    for at in range(0, n, 20000):
+        part, ids = ctx.to_device(x[at:at + 20000]), t[at:at + 20000]
+        parts.append(mh.linear_cross_entropy(ctx, part, W, ids) * (ids >= 0).sum())
+        part.free()
+    bound = 2 * R.product_bound(d, np.abs(x[keep]).sum(1).max() * np.abs(w).max()) + (V / 256 + 40) * 2 * R.U + 64 * R.U
+    assert abs(whole - sum(parts) / keep.sum()) <= 2 * bound

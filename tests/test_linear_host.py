@@ -197,3 +197,28 @@ def test_binding_checks_shapes():
         mh.linear_cross_entropy(c, S(4, 8), S(6, 8), np.zeros(3, np.int32))
     with pytest.raises(mh.ShapeError):
         mh.linear_cross_entropy(c, S(4, 8), S(8, 6), np.zeros(4, np.int32))
+
+
+def block_rows(n, row_bytes, limit=0):
+    rows = ctypes.c_int64()
+    f = mh.lib().mmh_test_loss_block_rows
+    f.argtypes = [ctypes.c_int64] * 3 + [ctypes.POINTER(ctypes.c_int64)]
+    assert f(n, row_bytes, limit, ctypes.byref(rows)) == mh.OK
+    return rows.value
+
+
+@pytest.mark.parametrize("limit", [0, 1, 64 << 20, 512 << 20])
+def test_blocks_of_the_loss_keep_to_their_workspace(limit):
+    """A block's rows fit the bytes given (128 rows always do); they are all there are, whole tiles of 256 or of one size, in
+    a quarter more blocks at most than the bytes need."""
+    bytes_ = limit or 512 << 20
+    r = np.random.default_rng(limit)
+    cases = [(8192, 152064 * 4), (1072, 250016 * 4), (514, 522016 * 4), (670, 400000 * 4), (4096, 200000 * 4), (1, 128),
+             (4096, 32000 * 4), (817, 131072 * 4), (33001, 8192), (2 ** 31 - 1, 128), (2 ** 31 - 1, 8), (129, 2 ** 33)]
+    cases += [(int(2 ** r.uniform(0, 24)), 128 * int(2 ** r.uniform(0, 14))) for _ in range(3000)]
+    for n, row_bytes in cases:
+        rows, most = block_rows(n, row_bytes, limit), max(128, bytes_ // row_bytes)
+        assert 1 <= rows <= min(n, most), (n, row_bytes, rows)
+        need = -(-n // most)
+        assert rows == n or rows % 256 == 0 or rows == -(-n // need), (n, row_bytes, rows)
+        assert -(-n // rows) <= 1.25 * need + 1, (n, row_bytes, rows)
