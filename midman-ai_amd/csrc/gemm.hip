@@ -1368,7 +1368,8 @@ void gemm(Context &ctx, const GemmDesc &d) {
 
     // (the small tiles' splits finish EPI_LINEAR in the launch)
     const int epi = splits > 1 && !(d.epi == EPI_LINEAR && !tiled) ? EPI_STORE : d.epi;
-    if (tiles > 0x7fffffff || d.batch > 65535) fail(MMH_ERR_SHAPE, "gemm: grid too large");
+    if (tiles * (ksplit ? 1024 : tiled ? 512 : 256) > 0xffffffffll || d.batch > 65535)
+        fail(MMH_ERR_SHAPE, "gemm: grid too large");
     dim3 grid((unsigned)tiles, (unsigned)d.batch, (unsigned)splits);
     if (ksplit) {
         // The k-contiguous operands (A when !ta, B when tb, the norm weights)
@@ -1506,7 +1507,7 @@ void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b) {
                     // (a launch, and one for the sums of both)
                     const double more = cost[0][i] + cost[1][j] + 3.0 - (i > 0 && j > 0 ? 4.0 : 0.0);
                     const double full = (g1 * l1 + g2 * l2) / cus * t.full + more;
-                    if (full >= best.us) continue;
+                    if (full >= best.us || g1 + g2 + 7 > (double)kMaxTiles) continue;
                     const double us =
                         std::max(full, list_end(cus, (int64_t)g1, l1, (int64_t)g2, l2) * t.alone + more);
                     if (us >= best.us) continue;

@@ -1242,6 +1242,8 @@ bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 // The loss and the rotation need 128 columns in a tile; the SwiGLU backward
 // does not fit the 256x256 tile's registers (its epilogue spills).
 bool gemm_tile_takes(const KParams &p, int epi, int tile) {
+    const GemmTileInfo &t = kGemmTiles[tile];
+    if (((p.m + t.rows - 1) / t.rows) * ((p.n + t.cols - 1) / t.cols) > kMaxTiles) return false;
     if (tile == TILE_256) return epi != EPI_SWIGLU_BWD;
     return (tile != TILE_128x64 && tile != TILE_64) ||
            (epi != EPI_CE && epi != EPI_CE_STORE && !p.rope_cos);
@@ -1276,7 +1278,7 @@ void launch_gemm_tiles(Context &ctx, const KParams &p, dim3 grid, bool ta, bool 
 void launch_gemm_pair(Context &ctx, const KParams &p1, const KParams &p2, bool tb1, int tile) {
     const int64_t g1 = (int64_t)p1.tiles_m * p1.tiles_n * p1.splits, first = (g1 + 7) / 8 * 8;
     const int64_t g2 = (int64_t)p2.tiles_m * p2.tiles_n * p2.splits;
-    if (first + g2 > 0x7fffffff) fail(MMH_ERR_SHAPE, "gemm: grid too large");
+    if (first + g2 > kMaxTiles) fail(MMH_ERR_SHAPE, "gemm: grid too large");
     const dim3 grid((unsigned)(first + g2));
 #define MMH_GEMM_PAIR(WM, WN, MB, WK)                                                                    \
     do {                                                                                                 \

@@ -84,6 +84,8 @@ constexpr GemmTileInfo kGemmTiles[TILE_COUNT] = {
     {256, 256, 1.75f, 2.35f, 7.5f}, {256, 128, 1.0f, 1.29f, 6.0f}, {128, 128, 0.55f, 0.72f, 10.0f},
     {128, 64, 0.42f, 0.43f, 8.0f},  {64, 64, 0.25f, 0.26f, 14.0f},
 };
+// A launch has less than 2^32 threads along x, a tile 512.
+constexpr int64_t kMaxTiles = 0xffffffffll / 512;
 // The tile kernel for p's product in the given form and epilogue; p.tiles_m and
 // p.tiles_n count tiles of the given shape. Splits (grid z) write their sums
 // to p.partial; launch_splitk_reduce adds them in split order.

@@ -7,7 +7,7 @@ import pytest
 
 import linear_oracle as R
 import midman_hip as mh
-from test_gpu_linear import Box, check_loss, empty, head, run_backward, stored
+from test_gpu_linear import Box, check_loss, empty, head, near, run_backward, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,34 @@ def test_the_loss_alone_over_more_rows_than_a_block(ctx):
         part.free()
     bound = 2 * R.product_bound(d, np.abs(x[keep]).sum(1).max() * np.abs(w).max()) + (V / 256 + 40) * 2 * R.U + 64 * R.U
     assert abs(whole - sum(parts) / keep.sum()) <= 2 * bound
+
+
+def test_more_rows_than_the_smallest_tiles_cover(ctx):
+    """A launch has less than 2^32 threads: 2^29 rows and more take larger tiles than 64x64. The rows repeat a pattern, so
+    every output is known from one pass over it."""
+    rows, p = 2 ** 29 + 77, 4099
+    print(f"\n[many rows] {rows}", flush=True)
+    x = np.random.default_rng(1).standard_normal(p).astype(np.float32)
+    w, b = np.full((1, 1), 0.75, np.float32), np.full(1, 0.125, np.float32)
+    try:
+        X, O = ctx.empty((rows, 1)), ctx.empty((rows, 1))
+    except mh.DeviceError:
+        pytest.skip("needs 4.3 GB of free device memory")
+    whole = np.resize(x, rows)[:, None]
+    X.upload(whole)
+    W, B = ctx.to_device(w), ctx.to_device(b)
+
+    def repeats(first, tol):
+        got = O.numpy()[:, 0]
+        near(got[:p], first, tol, "the first rows")
+        assert np.array_equal(got[:rows // p * p].reshape(-1, p), np.broadcast_to(got[:p], (rows // p, p)))
+        assert np.array_equal(got[rows // p * p:], got[:rows % p])
+
+    mh.linear(ctx, X, W, B, activation="silu", out=O)
+    want, tol, _, _ = R.linear(x[:, None], w, b, None, "silu", 0.0, 0, 0)
+    repeats(want[:, 0], tol[:, 0])
+    print("[many rows] dx", flush=True)
+    mh.check(mh.lib().mmh_linear_backward(ctx.handle, 0, None, W.ptr, None, X.ptr, rows, 1, 1, 0, 0.0, 0, 0, O.ptr, None, None))
+    repeats(x.astype(np.float64) * 0.75, 2 * R.U * np.abs(x))
+    for a in (X, O, W, B):
+        a.free()
