@@ -20,8 +20,9 @@
 namespace mmh {
 namespace {
 
-// The rows that a block has at least.
-constexpr int64_t kMinRows = 128;
+// The rows that a block has at least, and at most (narrow vocabularies: a launch has
+// less than 2^32 threads, a row up to 512).
+constexpr int64_t kMinRows = 128, kMaxRows = int64_t(1) << 22;
 // Up to so many rows the loss takes stored logits: the tiles that fold it have
 // 128 rows at least, those of the plain product 32 or 64 (35 rows x 1344 x 153411
 // 367 -> 266 us for the product, 64 rows 372 -> 274, 128 rows 384 -> 341 and 33
@@ -47,7 +48,7 @@ int64_t part_rows(int64_t rows, int64_t at, int64_t weights) {
 // 256 rows where a block has as many: rounded up where that still fits, else down
 // where that takes a quarter more blocks at most.
 int64_t block_rows(int64_t n, int64_t row_bytes, int64_t bytes) {
-    const int64_t most = std::max(kMinRows, bytes / row_bytes);
+    const int64_t most = std::min(kMaxRows, std::max(kMinRows, bytes / row_bytes));
     if (most >= n) return n;
     const int64_t blocks = (n + most - 1) / most, rows = (n + blocks - 1) / blocks;
     if (rows <= 256) return rows;
@@ -265,8 +266,8 @@ void launch_loss_parts(Context &cx, const float *z, const int32_t *targets, int6
 }
 
 __global__ __launch_bounds__(256) void copy_ids_kernel(const int32_t *host, int64_t n, int32_t *dev) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) dev[i] = host[i];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        dev[i] = host[i];
 }
 
 // Floats of a row of stored logits: whole float4s, for the products too.
@@ -332,12 +333,13 @@ void stage_rows(Context &cx, const Head &h, bool device, float *packed, Rows &r)
     }
     int32_t *dev = static_cast<int32_t *>(cx.workspace(1, (size_t)total * 4));
     r.targets = dev;
-    hipLaunchKernelGGL(copy_ids_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, cx.stream, t,
-                       total, dev);
+    hipLaunchKernelGGL(copy_ids_kernel, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 65536)),
+                       dim3(256), 0, cx.stream, t, total, dev);
     check_hip(hipGetLastError(), "targets launch");
     if (r.kept == h.n) return;
     r.map = dev + 2 * pad;
-    launch_embedding(cx, h.x, h.d, dev + pad, r.kept, packed);
+    for (int64_t at = 0; at < r.kept; at += kMaxRows)
+        launch_embedding(cx, h.x, h.d, dev + pad + at, std::min(kMaxRows, r.kept - at), packed + at * h.d);
     r.x = packed;
 }
 

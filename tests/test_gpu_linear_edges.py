@@ -186,3 +186,33 @@ def test_more_rows_than_the_smallest_tiles_cover(ctx):
     repeats(x.astype(np.float64) * 0.75, 2 * R.U * np.abs(x))
     for a in (X, O, W, B):
         a.free()
+
+
+@pytest.mark.parametrize("ignored", [False, True])
+def test_the_loss_of_very_many_rows(ctx, ignored):
+    """2^26 rows of a narrow vocabulary, whose partial sums would all fit one block but not one launch. The rows repeat a
+    pattern of 4096: the mean is the pattern's, a row's gradient its own divided by the repetitions (a power of two)."""
+    p, times, V = 4096, 2 ** 14, 100
+    n = p * times
+    print(f"\n[very many rows] {n} {ignored}", flush=True)
+    x, w, t = head(p, 1, V, seed=6)
+    if ignored:
+        t[5::17] = -1
+    want = R.cross_entropy(x, w, t)
+    try:
+        X, dX = ctx.empty((n, 1)), ctx.empty((n, 1))
+    except mh.DeviceError:
+        pytest.skip("needs 0.6 GB of free device memory")
+    X.upload(np.tile(x, (times, 1)))
+    W = ctx.to_device(w)
+    ids = np.tile(t, times)
+    loss = mh.linear_cross_entropy(ctx, X, W, ids, form="nn")
+    check_loss({"loss": loss}, want)
+    value = ctypes.c_float()
+    mh.check(mh.lib().mmh_linear_cross_entropy_backward(
+        ctx.handle, 0, X.ptr, W.ptr, ids.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), n, 1, V, -1, dX.ptr, None,
+        ctypes.byref(value)))
+    got = dX.numpy().reshape(times, p)
+    check_loss({"loss": value.value, "dx": got[0][:, None] * np.float32(times)}, want)
+    assert np.array_equal(got, np.broadcast_to(got[0], (times, p)))
+    X.free(), dX.free()

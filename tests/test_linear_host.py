@@ -209,7 +209,7 @@ def block_rows(n, row_bytes, limit=0):
 
 @pytest.mark.parametrize("limit", [0, 1, 64 << 20, 512 << 20])
 def test_blocks_of_the_loss_keep_to_their_workspace(limit):
-    """A block's rows fit the bytes given (128 rows always do); they are all there are, whole tiles of 256 or of one size, in
+    """A block's rows fit the bytes given (128 rows always do) and a launch (2^22 rows); they are all there are, whole tiles of 256 or of one size, in
     a quarter more blocks at most than the bytes need."""
     bytes_ = limit or 512 << 20
     r = np.random.default_rng(limit)
@@ -217,7 +217,7 @@ def test_blocks_of_the_loss_keep_to_their_workspace(limit):
              (4096, 32000 * 4), (817, 131072 * 4), (33001, 8192), (2 ** 31 - 1, 128), (2 ** 31 - 1, 8), (129, 2 ** 33)]
     cases += [(int(2 ** r.uniform(0, 24)), 128 * int(2 ** r.uniform(0, 14))) for _ in range(3000)]
     for n, row_bytes in cases:
-        rows, most = block_rows(n, row_bytes, limit), max(128, bytes_ // row_bytes)
+        rows, most = block_rows(n, row_bytes, limit), min(2 ** 22, max(128, bytes_ // row_bytes))
         assert 1 <= rows <= min(n, most), (n, row_bytes, rows)
         need = -(-n // most)
         assert rows == n or rows % 256 == 0 or rows == -(-n // need), (n, row_bytes, rows)
