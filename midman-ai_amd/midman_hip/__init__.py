@@ -702,11 +702,18 @@ def linear_backward(ctx: Context, x: DeviceArray, w: DeviceArray, dout: DeviceAr
     return dx, dw, dbias
 
 
-def _head_args(x, w, targets, form):
+def _head_args(x, w, targets, form, ignore):
     f, _, n, d, vocab = _linear_args(x, w, form, "none")
-    targets = np.ascontiguousarray(targets, dtype=np.int32)
-    if targets.size != n:
-        raise ShapeError(ERR_SHAPE, f"linear_cross_entropy: {n} rows but {targets.size} targets")
+    given = np.asarray(targets)
+    if given.size != n:
+        raise ShapeError(ERR_SHAPE, f"linear_cross_entropy: {n} rows but {given.size} targets")
+    with np.errstate(invalid="ignore"):
+        targets = np.ascontiguousarray(given, dtype=np.int32)
+    # (a value that wrapped would be another class)
+    if targets is not given and not np.array_equal(targets.ravel(), given.ravel()):
+        raise IndexOutOfRange(ERR_INDEX, "linear_cross_entropy: a target is no 32-bit class")
+    if not -1 << 31 <= ignore < 1 << 31:
+        raise ArgumentError(ERR_ARGUMENT, f"linear_cross_entropy: ignore must fit 32 bits, got {ignore}")
     return f, targets, n, d, vocab
 
 
@@ -715,7 +722,7 @@ def linear_cross_entropy(ctx: Context, x: DeviceArray, w: DeviceArray, targets: 
     """cross_entropy of the logits x op(w), which are not stored (those of 64 rows
     at most are): x [.., d], w [vocab, d] (nt, a tied embedding) or [d, vocab] (nn).
     Rows whose target is `ignore` are left out of the mean."""
-    f, targets, n, d, vocab = _head_args(x, w, targets, form)
+    f, targets, n, d, vocab = _head_args(x, w, targets, form, ignore)
     loss = ctypes.c_float()
     check(lib().mmh_linear_cross_entropy(ctx.handle, f, x.ptr, w.ptr, _ip(targets), n, d, vocab,
                                          ignore, ctypes.byref(loss)))
@@ -727,7 +734,7 @@ def linear_cross_entropy_backward(ctx: Context, x: DeviceArray, w: DeviceArray, 
                                   dw: DeviceArray = None):
     """(loss, dx, dw) of linear_cross_entropy for loss gradient 1. The logits of a
     block of rows are in memory at a time, 512 MiB or 128 rows of them."""
-    f, targets, n, d, vocab = _head_args(x, w, targets, form)
+    f, targets, n, d, vocab = _head_args(x, w, targets, form, ignore)
     _fits("linear_cross_entropy_backward: dx", dx, x.shape)
     _fits("linear_cross_entropy_backward: dw", dw, w.shape)
     dx, dw = dx or ctx.empty(x.shape), dw or ctx.empty(w.shape)

@@ -222,3 +222,19 @@ def test_blocks_of_the_loss_keep_to_their_workspace(limit):
         need = -(-n // most)
         assert rows == n or rows % 256 == 0 or rows == -(-n // need), (n, row_bytes, rows)
         assert -(-n // rows) <= 1.25 * need + 1, (n, row_bytes, rows)
+
+
+def test_binding_refuses_targets_that_do_not_fit_32_bits():
+    c, x, w = NoContext(), Shaped(3, 8), Shaped(6, 8)
+    calls = (lambda t, **a: mh.linear_cross_entropy(c, x, w, t, **a),
+             lambda t, **a: mh.linear_cross_entropy_backward(c, x, w, t, dx=x, dw=w, **a))
+    for f in calls:
+        for bad in (np.array([0, 2 ** 32 + 1, 2]), np.array([0, 2 ** 32 - 1, 2], np.uint32), np.array([0.0, 1.5, 2.0]),
+                    np.array([0.0, np.nan, 2.0]), np.array([0, 1, -2 ** 40])):
+            with pytest.raises(mh.IndexOutOfRange):
+                f(bad)
+        with pytest.raises(mh.ArgumentError, match="ignore"):
+            f([0, 1, 2], ignore=2 ** 32 - 1)
+        for good in ([0, 1, 5], np.array([0, -1, 5]), np.array([0, 1, 5], np.uint8), np.array([[0], [1], [5]], np.int32)):
+            with pytest.raises(mh.ArgumentError, match="invalid context|overlaps"):
+                f(good)
