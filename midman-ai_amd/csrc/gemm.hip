@@ -1521,14 +1521,25 @@ void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b) {
         tiled = found;
     }
     if (!tiled) {
+        if (a.plan) {
+            std::fill(a.plan, a.plan + 4, 0);
+            return;
+        }
         gemm(ctx, a);
         gemm(ctx, b);
         return;
     }
     KParams p[2];
     int64_t floats[2];
+    for (int i = 0; i < 2; ++i) p[i] = plain_params(*d[i], kGemmTiles[best.tile], splits[i]);
+    if (a.plan) {
+        a.plan[0] = kGemmTiles[best.tile].rows;
+        a.plan[1] = kGemmTiles[best.tile].cols;
+        a.plan[2] = p[0].splits;
+        a.plan[3] = p[1].splits;
+        return;
+    }
     for (int i = 0; i < 2; ++i) {
-        p[i] = plain_params(*d[i], kGemmTiles[best.tile], splits[i]);
         floats[i] = p[i].splits > 1 ? ((int64_t)p[i].splits * p[i].m * p[i].n + 63) / 64 * 64 : 0;
     }
     if (floats[0] + floats[1] > 0) {

@@ -166,6 +166,12 @@ GemmDesc product(const float *a, bool ta, const float *b, bool tb, float *c, int
     g.split_bytes = kTrainSplitBytes;
     return g;
 }
+GemmDesc dx_product(bool nt, const float *dpre, const float *w, float *dx, int64_t rows, int64_t k, int64_t n) {
+    return product(dpre, false, w, !nt, dx, rows, n, k);
+}
+GemmDesc dw_product(bool nt, const float *x, const float *dpre, float *dw, int64_t rows, int64_t k, int64_t n) {
+    return nt ? product(dpre, true, x, false, dw, n, rows, k) : product(x, true, dpre, false, dw, k, rows, n);
+}
 
 }  // namespace
 }  // namespace mmh
@@ -173,6 +179,31 @@ GemmDesc product(const float *a, bool ta, const float *b, bool tb, float *c, int
 using namespace mmh;
 
 extern "C" {
+
+// For the tests, not part of the C ABI: the tile (rows, columns) and the K splits of
+// mmh_linear for arrays at `at` (forward), or the tile and the splits of dx and dw
+// that mmh_linear_backward takes in one launch, zeros where it takes two.
+int32_t mmh_test_linear_plan(mmh_handle ctx, int32_t form, float *at, int64_t rows, int64_t k, int64_t n,
+                             int32_t backward, int32_t *plan) {
+    return guard([&] {
+        need(plan, "plan");
+        check_linear(form, rows, k, n, MMH_ACT_NONE);
+        Context &cx = context(ctx);
+        const bool nt = form == MMH_GEMM_NT;
+        LinearTail tail;
+        tail.out = at;
+        GemmDesc g = backward ? dx_product(nt, at, at, at, rows, k, n) : product(at, false, at, nt, nullptr, rows, k, n);
+        g.plan = plan;
+        if (backward) {
+            gemm_pair(cx, g, dw_product(nt, at, at, at, rows, k, n));
+        } else {
+            g.epi = EPI_LINEAR;
+            g.tail = &tail;
+            gemm(cx, g);
+        }
+        return MMH_OK;
+    });
+}
 
 int32_t mmh_dropout(mmh_handle ctx, const float *x, const float *residual, int64_t n, float p,
                     uint64_t seed, uint64_t offset, float *out) {
@@ -275,9 +306,8 @@ int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const 
             check_hip(hipGetLastError(), "linear dpre launch");
             if (several) launch_sum_rows(cx, sums, strips, n, dbias);
         }
-        const GemmDesc to_x = product(dpre, false, w, !nt, dx, rows, n, k);
-        const GemmDesc to_w = nt ? product(dpre, true, x, false, dw, n, rows, k)
-                                 : product(x, true, dpre, false, dw, k, rows, n);
+        const GemmDesc to_x = dx_product(nt, dpre, w, dx, rows, k, n);
+        const GemmDesc to_w = dw_product(nt, x, dpre, dw, rows, k, n);
         if (dx && dw) gemm_pair(cx, to_x, to_w);
         else if (dx) gemm(cx, to_x);
         else if (dw) gemm(cx, to_w);

@@ -201,6 +201,7 @@ struct GemmDesc {
 void gemm(Context &ctx, const GemmDesc &d);
 // Two plain products (EPI_STORE, batch 1) that do not depend on each other: a an nn
 // or nt one, b a tn one. In one launch where that is estimated faster than two.
+// a.plan receives the pair's tile and both products' splits, zeros for two launches.
 void gemm_pair(Context &ctx, const GemmDesc &a, const GemmDesc &b);
 // Whether gemm() folds the A-row norm and the RoPE of d into its kernel (so a
 // caller can time or schedule them as kernels of their own otherwise).

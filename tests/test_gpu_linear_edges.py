@@ -1,13 +1,14 @@
 """GPU checks of what the linear layer's operators promise at their edges: what a call has done when it returns, values that
-are not finite."""
+are not finite, several row blocks, very many rows, every tile that the products take, the activations' digits."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
 
 import linear_oracle as R
 import midman_hip as mh
-from test_gpu_linear import Box, check_loss, empty, head, near, run_backward, stored
+from test_gpu_linear import Box, check_loss, empty, head, near, operands, run_backward, run_linear, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -103,8 +104,8 @@ def test_several_row_blocks(ctx, kept, most, blocks, d, V, ignored, form):
     loss = ctypes.c_float(np.nan)
     try:
         limit_blocks(ctx, most * row)
-        mh.check(mh.lib().mmh_linear_cross_entropy_backward(ctx.handle, form, X.ptr, W.ptr, tp, len(t), d, V, -1, dx.ptr, dw.ptr,
-                                                            ctypes.byref(loss)))
+        mh.check(mh.lib().mmh_linear_cross_entropy_backward(ctx.handle, form, X.ptr, W.ptr, tp, len(t), d, V, -1, dx.ptr,
+                                                            dw.ptr, ctypes.byref(loss)))
         got = {"dx": dx.numpy(), "dw": dw.numpy().T if form else dw.numpy(), "loss": loss.value}
         limit_blocks(ctx, most * parts)
         mh.check(mh.lib().mmh_linear_cross_entropy(ctx.handle, form, X.ptr, W.ptr, tp, len(t), d, V, -1, ctypes.byref(loss)))
@@ -216,3 +217,117 @@ def test_the_loss_of_very_many_rows(ctx, ignored):
     check_loss({"loss": value.value, "dx": got[0][:, None] * np.float32(times)}, want)
     assert np.array_equal(got, np.broadcast_to(got[0], (times, p)))
     X.free(), dX.free()
+
+
+# (form, rows, k, n, tile rows and columns, K splits) of mmh_linear on 256 CUs: every tile, whole and split
+FORWARD_PLANS = [
+    (0, 1, 1, 1, (32, 32, 1)), (0, 1, 536, 1, (32, 32, 2)), (0, 68, 1817, 3274, (128, 128, 8)),
+    (0, 177, 2534, 599, (64, 64, 8)), (0, 395, 1, 8778, (256, 128, 1)), (0, 397, 1126, 8553, (256, 256, 3)),
+    (0, 576, 1, 11456, (128, 128, 1)), (0, 1192, 107, 9803, (256, 256, 1)), (0, 2436, 3342, 33, (128, 64, 12)),
+    (0, 3205, 381, 220, (64, 64, 1)), (0, 10174, 1124, 90, (256, 128, 5)), (0, 11388, 1, 290, (128, 64, 1)),
+    (1, 1, 1, 1, (32, 32, 1)), (1, 1, 225, 1, (32, 32, 2)), (1, 68, 1817, 3274, (128, 128, 8)),
+    (1, 177, 2534, 599, (64, 64, 8)), (1, 395, 1, 8778, (256, 128, 1)), (1, 397, 1126, 8553, (256, 256, 3)),
+    (1, 576, 1, 11456, (128, 128, 1)), (1, 1192, 107, 9803, (256, 256, 1)), (1, 2436, 3342, 33, (128, 64, 12)),
+    (1, 3205, 381, 220, (64, 64, 1)), (1, 10174, 1124, 90, (256, 128, 5)), (1, 11388, 1, 290, (128, 64, 1))]
+# the same with the splits of dx and dw, for the tiles that mmh_linear_backward takes for both in one launch: neither, either
+# and both of them split, and for both the rows of either a multiple of four floats or not (the sums' 16-byte form)
+BACKWARD_PLANS = [
+    (0, 412, 667, 994, (64, 64, 1, 1)), (0, 5398, 57, 874, (64, 64, 1, 8)), (0, 531, 279, 1817, (64, 64, 2, 1)),
+    (0, 4552, 22, 2718, (64, 64, 3, 6)), (0, 3741, 21, 3592, (64, 64, 2, 2)), (0, 2514, 52, 2134, (64, 64, 3, 4)),
+    (0, 1152, 192, 1216, (64, 64, 2, 2)), (0, 177, 2534, 599, (128, 64, 1, 1)), (0, 4036, 250, 273, (128, 64, 1, 8)),
+    (0, 214, 382, 3293, (128, 64, 8, 1)), (0, 1124, 315, 759, (128, 64, 2, 3)), (0, 168, 7170, 230, (128, 128, 1, 1)),
+    (0, 2404, 1109, 102, (128, 128, 1, 8)), (0, 70, 1086, 3562, (128, 128, 8, 1)), (0, 2980, 78, 1185, (128, 128, 4, 8)),
+    (0, 164, 9477, 233, (256, 128, 1, 1)), (0, 386, 8409, 85, (256, 128, 1, 3)), (0, 144, 2534, 817, (256, 128, 6, 1)),
+    (0, 3010, 129, 1543, (256, 128, 4, 8)), (0, 305, 11253, 335, (256, 256, 1, 1)),
+    (0, 1830, 4527, 138, (256, 256, 1, 6)), (0, 395, 4679, 1691, (256, 256, 3, 1)),
+    (0, 7406, 137, 2947, (256, 256, 4, 8)), (1, 412, 667, 994, (64, 64, 1, 1)), (1, 5398, 57, 874, (64, 64, 1, 8)),
+    (1, 270, 722, 1390, (64, 64, 2, 1)), (1, 2548, 43, 2854, (64, 64, 3, 3)), (1, 4921, 63, 976, (64, 64, 2, 6)),
+    (1, 4108, 56, 1295, (64, 64, 2, 6)), (1, 1152, 64, 3776, (64, 64, 6, 2)), (1, 177, 2534, 599, (128, 64, 1, 1)),
+    (1, 4036, 250, 273, (128, 64, 1, 8)), (1, 214, 382, 3293, (128, 64, 8, 1)), (1, 1124, 315, 759, (128, 64, 3, 4)),
+    (1, 148, 7122, 259, (128, 128, 1, 1)), (1, 2404, 1109, 102, (128, 128, 1, 8)), (1, 171, 1009, 1570, (128, 128, 6, 1)),
+    (1, 2980, 78, 1185, (128, 128, 4, 8)), (1, 157, 9065, 191, (256, 128, 1, 1)), (1, 733, 4402, 86, (256, 128, 1, 4)),
+    (1, 144, 2534, 817, (256, 128, 6, 1)), (1, 3299, 78, 3227, (256, 128, 8, 8)), (1, 305, 11253, 335, (256, 256, 1, 1)),
+    (1, 1830, 4527, 138, (256, 256, 1, 6)), (1, 341, 3231, 2633, (256, 256, 4, 1)),
+    (1, 7406, 137, 2947, (256, 256, 4, 8))]
+
+
+def plan(ctx, form, rows, k, n, backward):
+    out, x = (ctypes.c_int32 * 4)(), ctx.empty((4,))
+    f = mh.lib().mmh_test_linear_plan
+    f.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p] + [ctypes.c_int64] * 3 + [
+        ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]
+    mh.check(f(ctx.handle, form, x.ptr, rows, k, n, backward, out))
+    x.free()
+    return tuple(out)
+
+
+def on_256_cus(ctx):
+    if ctx.device_info()[1] != 256:
+        pytest.skip("the plans are those of 256 CUs")
+
+
+@pytest.mark.parametrize("form,rows,k,n,want", FORWARD_PLANS)
+def test_linear_on_every_tile(ctx, form, rows, k, n, want):
+    on_256_cus(ctx)
+    assert plan(ctx, form, rows, k, n, 0)[:3] == want
+    print(f"\n[linear] {form} {rows} {k} {n} {want}", flush=True)
+    x, w, b, res = operands(rows, k, n, rows + n)
+    out, pre = run_linear(ctx, form, x, w, b, res, "gelu", 0.25, 3, 4, True)
+    value, tol, want_pre, pre_tol = R.linear(x, w, b, res, "gelu", 0.25, 3, 4)
+    near(out, value, tol, "out")
+    near(pre, want_pre, pre_tol, "pre")
+
+
+@pytest.mark.parametrize("form,rows,k,n,want", BACKWARD_PLANS)
+def test_linear_backward_on_every_pair_of_tiles(ctx, form, rows, k, n, want):
+    on_256_cus(ctx)
+    assert plan(ctx, form, rows, k, n, 1) == want
+    print(f"\n[linear_backward] {form} {rows} {k} {n} {want}", flush=True)
+    x, w, _, dout = operands(rows, k, n, rows + k)
+    pre = np.random.default_rng(k).standard_normal((rows, n)).astype(np.float32)
+    assert x.shape == (rows, k) and w.shape == (k, n) and dout.shape == pre.shape == (rows, n)
+    got = run_backward(ctx, form, x, w, pre, dout, "silu", 0.1, 5, 6)
+    for name, (value, tol) in R.linear_backward(x, w, pre, dout, "silu", 0.1, 5, 6).items():
+        near(got[name], value, tol, name)
+
+
+def test_products_that_are_not_joined(ctx):
+    """Small products and ones that two launches are estimated to take less time for."""
+    on_256_cus(ctx)
+    for form, rows, k, n in ((0, 64, 64, 176), (1, 64, 64, 176), (0, 4096, 1024, 2816), (1, 4096, 1024, 2816)):
+        assert plan(ctx, form, rows, k, n, 1) == (0, 0, 0, 0)
+
+
+def exact_activations(x):
+    """{activation: (value, slope, the exponent whose rounding its far tail shows)} in 64 bits, by forms that do not cancel."""
+    tail = 0.5 * np.vectorize(math.erfc)(np.abs(x) / math.sqrt(2.0))  # Phi(-|x|)
+    cdf = np.where(x < 0, tail, 1.0 - tail)
+
+    def sigmoid(y):
+        e = np.exp(-np.abs(y))
+        return np.where(y < 0, e, 1.0) / (1.0 + e)
+
+    y = 2.0 * R.C0 * (x + R.C1 * x ** 3)
+    return {"gelu": (x * cdf, cdf + x * np.exp(-0.5 * x * x) / math.sqrt(2.0 * math.pi), 0.0),
+            "silu": (x * sigmoid(x), sigmoid(x) * (1.0 + x * sigmoid(-x)), 0.0),
+            "gelu_tanh": (x * sigmoid(y),
+                          sigmoid(y) + x * sigmoid(y) * sigmoid(-y) * 2.0 * R.C0 * (1.0 + 3.0 * R.C1 * x * x), np.abs(y))}
+
+
+def test_activations_keep_their_digits(ctx):
+    """Relative to the value itself, far tails too. In u = 2^-24: an exponential of a carried argument is off by 5 (the
+    hardware's 2, three roundings); gelu's tail adds its polynomial's fit (1), argument (2), steps (2) and two products: 12,
+    and 1 - tail and a product to that: 14; a sigmoid's small side is the exponential (4), over 1 + it (4), a product each:
+    10; gelu_tanh's argument, six roundings, is 6 |y| more of it. The slopes, at most 1.13, are sums of such terms: 16 u.
+    An exponential below 2^-126 is 0."""
+    r = np.random.default_rng(7)
+    v = np.concatenate([np.linspace(-13, 13, 400001), r.standard_normal(100000), 10.0 ** r.uniform(-30, 0, 20000),
+                        -10.0 ** r.uniform(-30, 0, 20000)]).astype(np.float32)
+    n, one = len(v), np.ones((1, 1), np.float32)
+    for act, (value, slope, y) in exact_activations(v.astype(np.float64)).items():
+        out, pre = run_linear(ctx, 0, one, v[None], None, None, act, 0.0, 0, 0, True)
+        assert np.array_equal(pre[0], v)
+        bound = {"gelu": 14, "silu": 10, "gelu_tanh": 10 + 6 * y}[act]
+        near(out[0], value, bound * R.U * np.abs(value) + 2 * R.TINY * np.abs(v), act)
+        got = run_backward(ctx, 0, one, v[None], v[None], np.ones((1, n), np.float32), act, 0.0, 0, 0, outs=("dbias",))
+        near(got["dbias"], slope, np.full(n, 16 * R.U), act + " slope")
