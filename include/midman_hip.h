@@ -462,7 +462,8 @@ int32_t mmh_linear(mmh_handle ctx, int32_t form, const float *x, const float *w,
  * Outputs are overwritten. The derivative of relu at 0 is 0. A dropped value of
  * dpre is 0 whatever dout and pre hold there; at a kept one a NaN of either stays,
  * and an infinity of dout times a slope of 0 is a NaN.
- * dpre takes rows * n floats of the context's workspace where it is not dout itself. */
+ * The context's workspace holds dpre (rows * n floats) where it is not dout itself,
+ * the bias gradient's partial sums, and up to 256 MiB of the products' (mmh_linear: 128). */
 int32_t mmh_linear_backward(mmh_handle ctx, int32_t form, const float *x, const float *w,
                             const float *pre, const float *dout, int64_t rows, int64_t k, int64_t n,
                             int32_t activation, float p, uint64_t seed, uint64_t offset, float *dx,

@@ -4,10 +4,10 @@
 //
 // The loss alone folds into the head's product (EPI_CE: a maximum and a sum per
 // row and 128 columns) and stores no logits; the gradients take blocks of rows,
-// whose logits become dz in place in a workspace of kLogitBytes, however many rows
-// there are. (Dropping them and forming them again for dx and dW would cost a
-// fourth product, a third of the time.) A pass over them reads and writes each
-// row once: up to kRowCols columns from registers; for wider rows the product
+// whose logits become dz in place in a workspace of kLogitBytes (or kMinRows rows),
+// however many rows there are. (Dropping them and forming them again for dx and dW
+// would cost a fourth product, a third of the time.) A pass over them reads and
+// writes each row once: up to kRowCols columns from registers; for wider rows the product
 // leaves the same partials beside the logits (three passes over such rows instead:
 // 817 x 1024 x 131071 4650 us, 4500 so). Rows whose target is `ignore` are left out
 // before the first product, so nothing they hold (infinities, NaN) reaches a sum.
@@ -46,7 +46,9 @@ int64_t part_rows(int64_t rows, int64_t at, int64_t weights) {
 // Rows of a block of n rows of row_bytes each: all, or as many as `bytes` hold, but
 // kMinRows at least. Blocks of one size (the last may be smaller), in whole tiles of
 // 256 rows where a block has as many: rounded up where that still fits, else down
-// where that takes a quarter more blocks at most.
+// where that takes a quarter more blocks at most (8192 x 1024 x 152064 with 768 rows
+// 42.2 ms, with 820 45.1; 514 x 768 x 522000 with 256 10.0, with 257 10.5; where it
+// takes more the two are even: 670 x 1024 x 400000 with 256 or 335 11.9).
 int64_t block_rows(int64_t n, int64_t row_bytes, int64_t bytes) {
     const int64_t most = std::min(kMaxRows, std::max(kMinRows, bytes / row_bytes));
     if (most >= n) return n;
