@@ -490,6 +490,96 @@ int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const fl
                                           int64_t d, int64_t vocab, int32_t ignore, float *dx,
                                           float *dw, float *loss_host);
 
+/* ---- Scoring and distilling --------------------------------------------------
+ * No counterpart in the reference, whose only score is the mean cross entropy.
+ * logits [n, vocab] f32, contiguous at any 4-byte alignment; targets on the host
+ * (MMH_ERR_INDEX, and nothing runs, for one outside [0, vocab) that is not
+ * `ignore`, any value, -1 say). A row whose target is `ignore` is left out, and
+ * nothing it holds is read. Sums are f32. A logit of -inf is a masked token: its
+ * probability is 0, and so is its gradient. A row whose largest logit is not finite
+ * (nothing but -inf, a +inf, a NaN) has no distribution: its log probabilities,
+ * entropy, loss and gradients are NaN. An output that overlaps another buffer of
+ * the call is MMH_ERR_ARGUMENT, except that dlogits may be logits. */
+
+/* Per row, each where it is wanted (else NULL): logprobs [n], the log probability
+ * of the row's target; entropy [n], -sum p ln p; and the k largest logits' ids and
+ * log probabilities, top_ids and top_logprobs [n, k] (k = 0: none, up to 256 and to
+ * vocab), the largest first, lower ids first among equals (-0 equals 0, and a NaN
+ * counts as +inf). targets_host may be NULL where logprobs is: no row is left out
+ * then. A row left out has 0, 0, ids -1 and log probabilities -inf. */
+int32_t mmh_token_logprobs(mmh_handle ctx, const float *logits, const int32_t *targets_host,
+                           int64_t n, int64_t vocab, int32_t ignore, int64_t k, float *logprobs,
+                           float *entropy, int32_t *top_ids, float *top_logprobs);
+/* Its backward for dlogprobs [n] and dentropy [n] (each may be NULL, zeros):
+ * dlogits [n, vocab] = dlogprob (onehot - p) - dentropy p (ln p + entropy),
+ * overwritten, zeros in rows left out. targets_host may be NULL where dlogprobs is. */
+int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits,
+                                    const int32_t *targets_host, int64_t n, int64_t vocab,
+                                    int32_t ignore, const float *dlogprobs, const float *dentropy,
+                                    float *dlogits);
+/* The distillation loss against a teacher's k largest logits (1 to 256) per row,
+ * teacher_ids and teacher_logits [n, k] on the device, as mmh_token_logprobs leaves
+ * them (log probabilities differ from logits by a row's constant, which cancels).
+ * With q the softmax of the row's teacher logits / temperature and p_T the softmax of
+ * the row's logits / temperature over the whole vocabulary, a row's loss is
+ *   alpha temperature^2 sum_j q_j (ln q_j - ln p_T[id_j]) + (1 - alpha) cross entropy,
+ * and the loss their mean over the rows that are not left out (0 with none). The
+ * cross entropy is of the row's target at temperature 1; with alpha = 1 targets_host
+ * may be NULL. A slot whose id is negative or whose logit is -inf is empty; a row of
+ * empty slots has no first term. An id in several slots has all their shares.
+ * temperature in [0.001, 1000], alpha in [0, 1]. An id of vocab or more is
+ * MMH_ERR_INDEX, found by the kernels. The call waits for its work. */
+int32_t mmh_distillation(mmh_handle ctx, const float *logits, const int32_t *targets_host,
+                         int64_t n, int64_t vocab, int32_t ignore, const int32_t *teacher_ids,
+                         const float *teacher_logits, int64_t k, float temperature, float alpha,
+                         float *loss_host);
+/* The same with dlogits [n, vocab] for loss gradient 1, overwritten, zeros in rows
+ * left out; loss_host may be NULL. After MMH_ERR_INDEX for a teacher's id dlogits
+ * holds no defined values. */
+int32_t mmh_distillation_backward(mmh_handle ctx, const float *logits, const int32_t *targets_host,
+                                  int64_t n, int64_t vocab, int32_t ignore,
+                                  const int32_t *teacher_ids, const float *teacher_logits,
+                                  int64_t k, float temperature, float alpha, float *dlogits,
+                                  float *loss_host);
+
+/* ---- Rotary positions in other forms ------------------------------------------
+ * Beside mmh_rope_tables and mmh_apply_rope (half layout, the whole head, positions
+ * 0..t-1, unscaled). */
+
+#define MMH_ROTARY_HALF 0        /* pairs (i, i + width/2) */
+#define MMH_ROTARY_INTERLEAVED 1 /* pairs (2i, 2i + 1) */
+
+#define MMH_ROTARY_NONE 0   /* w_i = theta^(-2i/width) */
+#define MMH_ROTARY_LINEAR 1 /* w_i / factor */
+#define MMH_ROTARY_BASE 2   /* theta times factor^(width/(width-2)) (width 2: theta) */
+#define MMH_ROTARY_PARTS 3  /* w_i (r + (1 - r) / factor), r = (turns - low) / (high - low) \
+                               within [0, 1], turns = trained w_i / 2 pi */
+
+/* cos and sin tables [positions, width/2]: amplitude * cos and sin of position * w_i,
+ * formed in f64, rounded to f32. factor is read by every scaling but
+ * MMH_ROTARY_NONE; trained (a length in tokens), low and high by MMH_ROTARY_PARTS
+ * alone. Within a rounding of mmh_rope_tables, whose bits are the reference's. */
+int32_t mmh_rotary_tables(mmh_handle ctx, int64_t width, int64_t positions, float theta,
+                          int32_t scaling, float factor, int64_t trained, float low, float high,
+                          float amplitude, float *cos_dev, float *sin_dev);
+/* q [b, h, t, hd] and k [b, hkv, t, hd] (either may be NULL, its heads and output are
+ * then not looked at) with the pairs of each head's first `width` columns (even, 2 to
+ * hd) rotated, (x0 c - x1 s, x1 c + x0 s), each product and sum rounded, and the other
+ * columns as they are. positions_host [b, t]: the row of the tables (of `table` rows)
+ * for each token, MMH_ERR_INDEX and nothing runs where it has none; NULL: 0..t-1.
+ * f32, contiguous at any 4-byte alignment. q_out may be q and k_out k; other overlaps
+ * are MMH_ERR_ARGUMENT. */
+int32_t mmh_rotary(mmh_handle ctx, int32_t layout, const float *q, const float *k,
+                   const int32_t *positions_host, int64_t b, int64_t h, int64_t hkv, int64_t t,
+                   int64_t hd, int64_t width, int64_t table, const float *cos_dev,
+                   const float *sin_dev, float *q_out, float *k_out);
+/* Its backward: the gradients dq, dk of the rotated heads turned back (s negated). */
+int32_t mmh_rotary_backward(mmh_handle ctx, int32_t layout, const float *dq, const float *dk,
+                            const int32_t *positions_host, int64_t b, int64_t h, int64_t hkv,
+                            int64_t t, int64_t hd, int64_t width, int64_t table,
+                            const float *cos_dev, const float *sin_dev, float *dq_out,
+                            float *dk_out);
+
 /* ---- Checkpoints: midman-checkpoint (safetensors.rs, params.rs) -----------
  * TensorFile (safetensors.rs:68-330): named F32 tensors + string metadata,
  * read with the reference's validation (8-byte length, <= 100 MB header of

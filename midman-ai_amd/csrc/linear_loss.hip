@@ -16,6 +16,7 @@
 #include "mmh_args.h"
 #include "mmh_elementwise.h"
 #include "mmh_internal.h"
+#include "mmh_loss.h"
 
 namespace mmh {
 namespace {
@@ -365,28 +366,6 @@ GemmDesc head_product(const Head &h, const float *x, int64_t rows) {
 
 size_t round64(int64_t floats) { return ((size_t)floats + 63) / 64 * 64; }
 
-// A call that fails after its first launch still waits for its kernels: they use
-// the pinned memory that the next call writes.
-struct Drain {
-    Context &cx;
-    bool done = false;
-    ~Drain() {
-        if (!done) (void)hipStreamSynchronize(cx.stream);
-    }
-};
-
-// Waits for the call's kernels. The row terms lie in pinned memory, and their mean
-// is taken here, in f64 and in eight sums of a fixed order: a launch of its own
-// would take longer than the sum of a few thousand.
-float mean_loss(Drain &drain, const float *rows, int64_t n) {
-    drain.done = true;
-    check_hip(hipStreamSynchronize(drain.cx.stream), "loss sync");
-    double sum[8] = {};
-    for (int64_t i = 0; i < n; ++i) sum[i & 7] += (double)rows[i];
-    const double total = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
-    return (float)(total / (double)n);
-}
-
 void forward(Context &cx, const Head &h, float *loss_host) {
     Rows r;
     r.kept = kept_rows(h);
@@ -438,7 +417,7 @@ void forward(Context &cx, const Head &h, float *loss_host) {
             }
         }
     }
-    *loss_host = mean_loss(drain, r.loss, r.kept);
+    *loss_host = mean_loss(drain, r.loss, r.kept, r.kept);
 }
 
 void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host) {
@@ -541,7 +520,7 @@ void backward(Context &cx, const Head &h, float *dx, float *dw, float *loss_host
                            cx.stream, dxk, r.map, h.n, h.d, dx);
         check_hip(hipGetLastError(), "gradient rows launch");
     }
-    const float loss = mean_loss(drain, r.loss, r.kept);  // (waits: the pinned targets have been read)
+    const float loss = mean_loss(drain, r.loss, r.kept, r.kept);  // (waits: the pinned targets have been read)
     if (loss_host) *loss_host = loss;
 }
 

@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -145,6 +145,16 @@ _SIGNATURES = {
     "mmh_linear_cross_entropy": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 3 + [_i32, _f32p],
     "mmh_linear_cross_entropy_backward": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 3 + [_i32, _vp, _vp,
                                                                                      _f32p],
+    "mmh_token_logprobs": [_h, _vp, _i32p, _i64, _i64, _i32, _i64] + [_vp] * 4,
+    "mmh_token_logprobs_backward": [_h, _vp, _i32p, _i64, _i64, _i32] + [_vp] * 3,
+    "mmh_distillation": [_h, _vp, _i32p, _i64, _i64, _i32, _vp, _vp, _i64, ctypes.c_float,
+                         ctypes.c_float, _f32p],
+    "mmh_distillation_backward": [_h, _vp, _i32p, _i64, _i64, _i32, _vp, _vp, _i64, ctypes.c_float,
+                                  ctypes.c_float, _vp, _f32p],
+    "mmh_rotary_tables": [_h, _i64, _i64, ctypes.c_float, _i32, ctypes.c_float, _i64]
+                         + [ctypes.c_float] * 3 + [_vp, _vp],
+    "mmh_rotary": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 7 + [_vp] * 4,
+    "mmh_rotary_backward": [_h, _i32, _vp, _vp, _i32p] + [_i64] * 7 + [_vp] * 4,
     "mmh_tensorfile_create": [ctypes.POINTER(_h)],
     "mmh_tensorfile_parse": [ctypes.c_char_p, ctypes.c_uint64, ctypes.POINTER(_h)],
     "mmh_tensorfile_push": [_h, ctypes.c_char_p, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64),
@@ -743,6 +753,185 @@ def linear_cross_entropy_backward(ctx: Context, x: DeviceArray, w: DeviceArray, 
                                                   vocab, ignore, dx.ptr, dw.ptr,
                                                   ctypes.byref(loss)))
     return loss.value, dx, dw
+
+
+# ---- scoring and distilling (scoring.hip) ------------------------------------------------
+
+class TokenScores(NamedTuple):
+    """What token_logprobs gives per row: DeviceArrays, None where not asked for."""
+    logprobs: Optional[DeviceArray]
+    entropy: Optional[DeviceArray]
+    top_ids: Optional[DeviceArray]
+    top_logprobs: Optional[DeviceArray]
+
+
+def _host_ids(what, given, n):
+    """Ids for the C ABI: n int32 values, contiguous, none of them wrapped."""
+    given = np.asarray(given)
+    if given.size != n:
+        raise ShapeError(ERR_SHAPE, f"{what}: {n} are needed but {given.size} are given")
+    with np.errstate(invalid="ignore"):
+        ids = np.ascontiguousarray(given, dtype=np.int32)
+    if ids is not given and not np.array_equal(ids.ravel(), given.ravel()):
+        raise IndexOutOfRange(ERR_INDEX, f"{what}: a value does not fit 32 bits")
+    return ids
+
+
+def _scored(what, logits, targets, ignore):
+    """(targets or None, n, vocab) of logits [.., vocab]."""
+    if logits.dtype != np.float32 or not logits.shape:
+        raise ShapeError(ERR_SHAPE, f"{what}: logits must be f32 [.., vocab]")
+    if not -1 << 31 <= ignore < 1 << 31:
+        raise ArgumentError(ERR_ARGUMENT, f"{what}: ignore must fit 32 bits, got {ignore}")
+    vocab = logits.shape[-1]
+    n = logits.size // max(1, vocab)
+    return None if targets is None else _host_ids(what + ": targets", targets, n), n, vocab
+
+
+def _typed(what, a, shape, dtype=np.float32):
+    _fits(what, a, shape)
+    if a is not None and a.dtype != dtype:
+        raise ArgumentError(ERR_ARGUMENT, f"{what} must be {np.dtype(dtype).name}, got {a.dtype.name}")
+
+
+def token_logprobs(ctx: Context, logits: DeviceArray, targets: np.ndarray = None, k: int = 0,
+                   ignore: int = -1, entropy: bool = True) -> TokenScores:
+    """Per row of logits [.., vocab]: the log probability of its target, the entropy,
+    and the ids and log probabilities of the k most likely tokens ([.., k], the first
+    is the likeliest, lower ids first among equals). Rows whose target is `ignore`
+    are left out: 0, 0, -1 and -inf."""
+    t, n, vocab = _scored("token_logprobs", logits, targets, ignore)
+    rows = logits.shape[:-1]
+    if not 0 <= k <= min(vocab, 256):
+        raise ShapeError(ERR_SHAPE, f"token_logprobs: k must be 0 to {min(vocab, 256)}, got {k}")
+    s = TokenScores(None if t is None else ctx.empty(rows), ctx.empty(rows) if entropy else None,
+                    ctx.empty(rows + (k,), np.int32) if k else None,
+                    ctx.empty(rows + (k,)) if k else None)
+    check(lib().mmh_token_logprobs(ctx.handle, logits.ptr, None if t is None else _ip(t), n, vocab,
+                                   ignore, k, *[_ptr(a) for a in s]))
+    return s
+
+
+def token_logprobs_backward(ctx: Context, logits: DeviceArray, targets: np.ndarray = None,
+                            dlogprobs: DeviceArray = None, dentropy: DeviceArray = None,
+                            ignore: int = -1, out: DeviceArray = None):
+    """dlogits of token_logprobs' log probabilities and entropies for their gradients
+    (each may be None: zeros). out may be logits."""
+    t, n, vocab = _scored("token_logprobs_backward", logits, targets, ignore)
+    _typed("token_logprobs_backward: dlogprobs", dlogprobs, logits.shape[:-1])
+    _typed("token_logprobs_backward: dentropy", dentropy, logits.shape[:-1])
+    _typed("token_logprobs_backward: out", out, logits.shape)
+    out = out or ctx.empty(logits.shape)
+    check(lib().mmh_token_logprobs_backward(ctx.handle, logits.ptr, None if t is None else _ip(t),
+                                            n, vocab, ignore, _ptr(dlogprobs), _ptr(dentropy),
+                                            out.ptr))
+    return out
+
+
+def _distill_args(what, logits, teacher_ids, teacher_logits, targets, ignore):
+    t, n, vocab = _scored(what, logits, targets, ignore)
+    if len(teacher_ids.shape) != len(logits.shape):
+        raise ShapeError(ERR_SHAPE, f"{what}: teacher_ids {teacher_ids.shape} do not fit logits {logits.shape}")
+    k = teacher_ids.shape[-1]
+    _typed(what + ": teacher_ids", teacher_ids, logits.shape[:-1] + (k,), np.int32)
+    _typed(what + ": teacher_logits", teacher_logits, teacher_ids.shape)
+    return [logits.ptr, None if t is None else _ip(t), n, vocab, ignore, teacher_ids.ptr,
+            teacher_logits.ptr, k], t
+
+
+def distillation(ctx: Context, logits: DeviceArray, teacher_ids: DeviceArray,
+                 teacher_logits: DeviceArray, targets: np.ndarray = None, temperature: float = 1.0,
+                 alpha: float = 1.0, ignore: int = -1) -> float:
+    """alpha temperature^2 KL(teacher || model at that temperature) + (1 - alpha) cross
+    entropy of the targets, the mean over rows whose target is not `ignore`. The
+    teacher's k largest logits or log probabilities per row ([.., k], int32 ids and f32,
+    as token_logprobs gives them) are its whole distribution; a negative id is an empty
+    slot."""
+    args, _keep = _distill_args("distillation", logits, teacher_ids, teacher_logits, targets, ignore)
+    loss = ctypes.c_float()
+    check(lib().mmh_distillation(ctx.handle, *args, temperature, alpha, ctypes.byref(loss)))
+    return loss.value
+
+
+def distillation_backward(ctx: Context, logits: DeviceArray, teacher_ids: DeviceArray,
+                          teacher_logits: DeviceArray, targets: np.ndarray = None,
+                          temperature: float = 1.0, alpha: float = 1.0, ignore: int = -1,
+                          out: DeviceArray = None):
+    """(loss, dlogits) of distillation for loss gradient 1. out may be logits."""
+    args, _keep = _distill_args("distillation_backward", logits, teacher_ids, teacher_logits, targets,
+                                ignore)
+    _typed("distillation_backward: out", out, logits.shape)
+    out = out or ctx.empty(logits.shape)
+    loss = ctypes.c_float()
+    check(lib().mmh_distillation_backward(ctx.handle, *args, temperature, alpha, out.ptr,
+                                          ctypes.byref(loss)))
+    return loss.value, out
+
+
+# ---- rotary positions in other forms (rotary.hip) ----------------------------------------
+
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+class ScaledRotaryTables:
+    """cos and sin tables for `positions` positions of heads that rotate their first
+    `width` columns, formed on the device; the frequencies scaled for a longer context:
+    "linear" divides them by factor, "base" raises theta by factor^(width/(width-2)),
+    "parts" divides those that turn less than `low` times in the `trained` length, keeps
+    those that turn more than `high` times and blends between."""
+
+    def __init__(self, ctx: Context, width: int, positions: int, theta: float = 10000.0,
+                 scaling: str = "none", factor: float = 1.0, trained: int = 0, low: float = 1.0,
+                 high: float = 32.0, amplitude: float = 1.0):
+        if scaling not in ROTARY_SCALINGS:
+            raise ArgumentError(ERR_ARGUMENT, f"rotary tables: unknown scaling {scaling!r}")
+        if width < 2 or width % 2 or positions < 1:
+            raise ShapeError(ERR_SHAPE, f"rotary tables: no tables of {positions} positions for width {width}")
+        self.width, self.positions = width, positions
+        self.cos = ctx.empty((positions, width // 2))
+        self.sin = ctx.empty((positions, width // 2))
+        check(lib().mmh_rotary_tables(ctx.handle, width, positions, theta, ROTARY_SCALINGS[scaling],
+                                      factor, trained, low, high, amplitude, self.cos.ptr,
+                                      self.sin.ptr))
+
+
+def _rotary(name, ctx, q, k, tables, layout, positions, q_out, k_out):
+    if layout not in ROTARY_LAYOUTS:
+        raise ArgumentError(ERR_ARGUMENT, f"{name}: unknown layout {layout!r}")
+    given = [a for a in (q, k) if a is not None]
+    if not given or any(len(a.shape) != 4 for a in given):
+        raise ShapeError(ERR_SHAPE, f"{name}: q and k are [b, heads, t, hd], one of them at least")
+    b, _, t, hd = given[0].shape
+    for what, a, out in (("q", q, q_out), ("k", k, k_out)):
+        if a is not None:
+            _typed(f"{name}: {what}", a, (b, a.shape[1], t, hd))
+            _typed(f"{name}: {what}_out", out, a.shape)
+    table, half = tables.cos.shape
+    at = None if positions is None else _host_ids(name + ": positions", positions, b * t)
+    q_out = (q_out or ctx.empty(q.shape)) if q is not None else None
+    k_out = (k_out or ctx.empty(k.shape)) if k is not None else None
+    check(getattr(lib(), "mmh_" + name)(ctx.handle, ROTARY_LAYOUTS[layout], _ptr(q), _ptr(k),
+                                        None if at is None else _ip(at), b, q.shape[1] if q else 0,
+                                        k.shape[1] if k else 0, t, hd, 2 * half, table,
+                                        tables.cos.ptr, tables.sin.ptr, _ptr(q_out), _ptr(k_out)))
+    return q_out, k_out
+
+
+def rotary(ctx: Context, q: Optional[DeviceArray], k: Optional[DeviceArray], tables,
+           layout: str = "half", positions: np.ndarray = None, q_out: DeviceArray = None,
+           k_out: DeviceArray = None):
+    """(q, k) [b, heads, t, hd] with the first columns of each head, twice the tables'
+    width of them, rotated at positions [b, t] (None: 0..t-1); the other columns as
+    they are. tables: RotaryTables or ScaledRotaryTables. q_out may be q and k_out k."""
+    return _rotary("rotary", ctx, q, k, tables, layout, positions, q_out, k_out)
+
+
+def rotary_backward(ctx: Context, dq: Optional[DeviceArray], dk: Optional[DeviceArray], tables,
+                    layout: str = "half", positions: np.ndarray = None,
+                    dq_out: DeviceArray = None, dk_out: DeviceArray = None):
+    """rotary's gradients (dq, dk) for those of its outputs."""
+    return _rotary("rotary_backward", ctx, dq, dk, tables, layout, positions, dq_out, dk_out)
 
 
 # ---- checkpoints: midman-checkpoint ----------------------------------------------------
