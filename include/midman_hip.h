@@ -527,8 +527,9 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits,
  * cross entropy is of the row's target at temperature 1; with alpha = 1 targets_host
  * may be NULL. A slot whose id is negative or whose logit is -inf is empty; a row of
  * empty slots has no first term. An id in several slots has all their shares.
- * temperature in [0.001, 1000], alpha in [0, 1]. An id of vocab or more is
- * MMH_ERR_INDEX, found by the kernels. The call waits for its work. */
+ * temperature in [0.001, 1000], alpha in [0, 1] (at 0 the teacher is not looked at).
+ * An id of vocab or more is MMH_ERR_INDEX, found by the kernels. The call waits for
+ * its work. */
 int32_t mmh_distillation(mmh_handle ctx, const float *logits, const int32_t *targets_host,
                          int64_t n, int64_t vocab, int32_t ignore, const int32_t *teacher_ids,
                          const float *teacher_logits, int64_t k, float temperature, float alpha,

@@ -22,85 +22,144 @@
 namespace mmh {
 namespace {
 
-// A launch has less than 2^32 threads, a row up to 512.
-constexpr int64_t kMaxRows = int64_t(1) << 22;
+// A launch has less than 2^32 threads, a row's workgroup up to 1024.
+constexpr int64_t kMaxRows = int64_t(1) << 21;
 // Alternatives of a row, and slots of a teacher's, at most.
 constexpr int64_t kMaxTop = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+// (exp(-200) is 0 in f32: a masked token's difference has this in its place, so that
+// its product with that 0 is one)
+constexpr float kFar = -200.0f;
 
-// A row's sums in progress: m the largest logit (-inf: none yet), a the sum of
-// exp((z - m) rate) without one term of m itself, u the sum of exp(z - m) (z - m)
-// (SUMS_ENTROPY) or a at rate 1 (SUMS_BOTH).
-enum Sums : int { SUMS_ONE = 0, SUMS_ENTROPY = 1, SUMS_BOTH = 2 };
-struct RowSums {
-    float m, a, u;
-};
-
-// exp(d rate), d <= 0.
-__device__ __forceinline__ float exp_at(float d, float rate) { return exp_neg(d * rate); }
-
-// (A NaN counts as +inf, which leaves a row without a distribution: see finish.)
-__device__ __forceinline__ float logit(float z) { return z != z ? INFINITY : z; }
-
-template <int SUMS>
-__device__ __forceinline__ void merge(RowSums &x, const RowSums &y, float rate) {
-    if (y.m == -INFINITY) return;
-    if (x.m == -INFINITY) {
-        x = y;
-        return;
-    }
-    RowSums big = x, small = y;
-    if (y.m > x.m) {
-        big = y;
-        small = x;
-    }
-    const float d = fmaxf(small.m - big.m, -1e30f), w = exp_at(d, rate);
-    x.m = big.m;
-    x.a = big.a + (1.0f + small.a) * w;
-    if (SUMS == SUMS_ENTROPY) x.u = big.u + (small.u + d * (1.0f + small.a)) * w;
-    if (SUMS == SUMS_BOTH) x.u = big.u + (1.0f + small.u) * exp_at(d, 1.0f);
-}
-
-// A row whose largest logit is not finite (nothing but -inf, an infinity or a NaN) has
-// no distribution: its sums are NaN, and so is what is formed from them.
-__device__ __forceinline__ void finish(RowSums &x) {
-    if (!(fabsf(x.m) < INFINITY)) x.a = x.u = __builtin_nanf("");
-}
-
-template <int NT, int SUMS>
-__device__ __forceinline__ RowSums block_sums(RowSums x, float rate, RowSums *lds) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const RowSums y{__shfl_xor(x.m, off, 64), __shfl_xor(x.a, off, 64), __shfl_xor(x.u, off, 64)};
-        // (both lanes take the sums in one order: their results are the same)
-        const bool low = (threadIdx.x & off) == 0;
-        RowSums l = low ? x : y;
-        merge<SUMS>(l, low ? y : x, rate);
-        x = l;
-    }
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = lds[0];
-    for (int i = 1; i < NT / 64; ++i) merge<SUMS>(x, lds[i], rate);
-    finish(x);
-    return x;
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
 }
 
-template <int NT, int SUMS>
-__device__ __forceinline__ RowSums row_sums(const float *z, int64_t v, float rate, RowSums *lds) {
-    RowSums x{-INFINITY, 0.0f, 0.0f};
-    for (int64_t j = threadIdx.x; j < v; j += NT) {
-        const RowSums y{logit(z[j]), 0.0f, 0.0f};
-        merge<SUMS>(x, y, rate);
+// ---- a stretch of a row in registers ------------------------------------------
+// NT threads hold NV strips of 4 NT columns, thread t of strip i the columns 4 (t +
+// NT i) and three on; what lies past the stretch's `cols` is -inf. Rows begin at any
+// 4-byte address, at which gfx950 moves 16 bytes as well. Loads of whole float4s are
+// unconditional (from the last one past the end), so all of them are in flight at once.
+template <int NT, int NV>
+__device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e)[NV][4]) {
+    const int tid = threadIdx.x;
+    if (cols >= 4) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) __builtin_memcpy(e[i], z + min(4 * (tid + NT * i), cols - 4), 16);
     }
-    return block_sums<NT, SUMS>(x, rate, lds);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (4 * NT * (i + 1) <= cols) continue;
+        const int c = 4 * (tid + NT * i);
+        if (c + 4 <= cols) continue;
+        // (a float4 at the end: its last columns, from the load at cols - 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[i][j] = c + j < cols ? z[c + j] : -INFINITY;
+    }
+}
+template <int NT, int NV>
+__device__ __forceinline__ void store_stretch(float *out, int cols, const float (&e)[NV][4]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = 4 * (threadIdx.x + NT * i);
+        store4(out + c, max(0, min(4, cols - c)), e[i]);
+    }
 }
 
-// Values in the order of their logits, lower ids first among equals: a number that
-// is larger for what comes first.
+// ---- a row's sums ---------------------------------------------------------------
+// Of exp((z - m) rate), m the largest logit: `count` of the terms are 1 (z = m), a is
+// the sum of the others, and u the sum of exp(z - m) (z - m) (KIND_SCORES) or of the
+// others' terms at rate 1 (KIND_BOTH). A wave has one m, its lanes share count.
+enum Kind : int { KIND_SCORES = 0, KIND_ONE = 1, KIND_BOTH = 2 };
+struct RowSums {
+    float m, count, a, u;
+};
+__device__ __forceinline__ RowSums no_sums() { return RowSums{-INFINITY, 0.0f, 0.0f, 0.0f}; }
+
+// Adds a stretch to a wave's running sums (per lane but for m and count). A NaN stays in a.
+template <int KIND, int NV>
+__device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4], float k) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = fmaxf(top, fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])));
+    top = wave_max(top);
+    if (top > s.m) {
+        // what is there is scaled to the new largest logit; its ones are ordinary terms
+        const float one = (threadIdx.x & 63) == 0 ? s.count : 0.0f;
+        if (s.m > -INFINITY) {
+            const float d = s.m - top, w = __builtin_amdgcn_exp2f(d * k);
+            if (KIND == KIND_SCORES) s.u = (s.u + fmaxf(d, kFar) * (s.a + one)) * w;
+            if (KIND == KIND_BOTH) s.u = (s.u + one) * __builtin_amdgcn_exp2f(d * kLog2e);
+            s.a = (s.a + one) * w;
+        }
+        s.m = top;
+        s.count = 0.0f;
+    }
+    const float m = s.m == -INFINITY ? 0.0f : s.m;  // (nothing but -inf: terms of 0)
+    int ones = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float d = e[i][j] - m;
+            const float x = __builtin_amdgcn_exp2f(d * k);
+            const bool one = d == 0.0f;
+            ones += __popcll(__ballot(one));
+            s.a += one ? 0.0f : x;
+            if (KIND == KIND_SCORES) s.u = __builtin_fmaf(x, fmaxf(d, kFar), s.u);
+            if (KIND == KIND_BOTH) s.u += one ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
+        }
+    s.count += s.m == -INFINITY ? 0.0f : (float)ones;
+}
+// The wave's sums in every lane; a NaN among its logits makes m one.
+__device__ __forceinline__ RowSums wave_sums(RowSums s) {
+    s.a = wave_sum(s.a);
+    s.u = wave_sum(s.u);
+    if (s.a != s.a) s.m = s.a;
+    return s;
+}
+// One of n sums of the parts of a row. Those of a row whose largest logit is not finite
+// (nothing but -inf, an infinity or a NaN) are NaN: inf - inf is one.
+template <int KIND>
+__device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, float k) {
+    RowSums s = no_sums();
+    for (int i = 0; i < n; ++i) s.m = fmaxf(s.m, parts[i].m);
+    for (int i = 0; i < n; ++i) {
+        const RowSums p = parts[i];
+        const float d = p.m - s.m;
+        if (d == 0.0f) {
+            s.count += p.count;
+            s.a += p.a;
+            s.u += p.u;
+        } else {
+            const float w = __builtin_amdgcn_exp2f(d * k), all = p.a + p.count;
+            s.a += all * w;
+            if (KIND == KIND_SCORES) s.u += (p.u + fmaxf(d, kFar) * all) * w;
+            if (KIND == KIND_BOTH) s.u += (p.u + p.count) * __builtin_amdgcn_exp2f(d * kLog2e);
+        }
+    }
+    return s;
+}
+// S - 1: the sum without one of the largest logits' terms.
+__device__ __forceinline__ float rest_of(const RowSums &s) { return s.a + (s.count - 1.0f); }
+
+// Values in the order of their logits: a larger number for a larger one, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float z) {
-    const uint32_t b = __float_as_uint(z + 0.0f);  // (-0 as 0)
+    const uint32_t b = __float_as_uint(z + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t order) {
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// (for the order of alternatives a NaN counts as +inf)
+__device__ __forceinline__ float ranked(float z) { return z != z ? INFINITY : z; }
 
 struct ScoreArgs {
     const float *logits;
@@ -129,17 +188,26 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoreArgs p) {
         }
         return;
     }
-    const RowSums s = row_sums<256, SUMS_ENTROPY>(z, p.vocab, 1.0f, lds);
-    const float rest = log1pf(s.a);
-    if (tid == 0 && p.logprobs) p.logprobs[row] = (logit(z[t]) - s.m) - rest;
-    if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + s.a);
+    RowSums s = no_sums();
+    for (int64_t c = 0; c < p.vocab; c += 4096) {
+        float e[4][4];
+        load_stretch<256, 4>(z + c, (int)min((int64_t)4096, p.vocab - c), e);
+        add_stretch<KIND_SCORES>(s, e, kLog2e);
+    }
+    s = wave_sums(s);
+    if ((tid & 63) == 0) lds[tid >> 6] = s;
+    __syncthreads();
+    s = join_sums<KIND_SCORES>(lds, 4, kLog2e);
+    const float a = rest_of(s), rest = log1pf(a);
+    if (tid == 0 && p.logprobs) p.logprobs[row] = (z[t] - s.m) - rest;
+    if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
     unsigned long long last = ~0ull;
     for (int j = 0; j < p.k; ++j) {
         if (tid == 0) best = 0;
         __syncthreads();
         unsigned long long mine = 0;
         for (int64_t i = tid; i < p.vocab; i += 256) {
-            const unsigned long long key = (unsigned long long)order_of(logit(z[i])) << 32 | (uint32_t)~(uint32_t)i;
+            const unsigned long long key = (unsigned long long)order_of(ranked(z[i])) << 32 | (uint32_t)~(uint32_t)i;
             if (key < last && key > mine) mine = key;
         }
         atomicMax(&best, mine);
@@ -148,107 +216,178 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoreArgs p) {
         const int32_t id = (int32_t) ~(uint32_t)last;
         if (tid == 0) {
             p.top_ids[row * p.k + j] = id;
-            p.top_logprobs[row * p.k + j] = (logit(z[id]) - s.m) - rest;
+            p.top_logprobs[row * p.k + j] = (z[id] - s.m) - rest;
         }
         __syncthreads();
     }
 }
 
-// dlogits of the log probabilities and entropies. dlogits may be the logits.
-__global__ __launch_bounds__(256) void scores_grad_kernel(const float *logits, const int32_t *targets, int64_t v,
-                                                          int32_t ignore, const float *dlogprobs,
-                                                          const float *dentropy, float *dlogits) {
-    __shared__ RowSums lds[4];
-    const int64_t row = blockIdx.x;
-    const float *z = logits + row * v;
-    float *out = dlogits + row * v;
-    const int64_t t = targets ? targets[row] : -1;
-    if (targets && t == ignore) {
-        for (int64_t j = threadIdx.x; j < v; j += 256) out[j] = 0.0f;
-        return;
-    }
-    const RowSums s = row_sums<256, SUMS_ENTROPY>(z, v, 1.0f, lds);
-    const float total = 1.0f + s.a, rest = log1pf(s.a), h = rest - s.u / total;
-    const float dl = dlogprobs ? dlogprobs[row] : 0.0f, dh = dentropy ? dentropy[row] : 0.0f;
-    for (int64_t j = threadIdx.x; j < v; j += 256) {
-        const float d = fmaxf(logit(z[j]) - s.m, -1e4f), p = exp_neg(d) / total;
-        const float g = p * (-dl - dh * ((d - rest) + h));
-        out[j] = j == t ? dl + g : g;
-    }
-}
-
-struct DistillArgs {
+// ---- gradients of a row's logits, and the distillation loss -----------------------
+// Every gradient here is exp(d rate) times a line in d (KIND_SCORES) or a constant,
+// KIND_BOTH with a second exponential at rate 1, less a weight at a few tokens: the
+// teacher's slots and the target.
+struct RowArgs {
     const float *logits;
     const int32_t *targets;  // or null
     int64_t vocab;
     int32_t ignore;
+    float *out;              // dlogits, which may be the logits; null: the loss alone
+    const float *dlogprobs, *dentropy;  // KIND_SCORES, each may be null
+    // distillation
     const int32_t *ids;
     const float *teacher;
     int k;
     float temperature, alpha, scale;  // scale: 1 / the rows that count
+    float rate;                       // of the first exponential: 1 / temperature, or 1 (KIND_SCORES, alpha 0)
     float *row_loss;                  // [rows], 0 for a row that is left out
-    int32_t *wrong;                   // receives an id beyond the vocabulary
-    float *dlogits;
+    int32_t *wrong;                   // receives 1 for a teacher's id beyond the vocabulary
 };
 
-// The row's loss and (dlogits) its gradient. dlogits may be the logits.
-__global__ __launch_bounds__(256) void distill_kernel(DistillArgs p) {
-    __shared__ RowSums lds[4];
-    __shared__ float q[kMaxTop], term[kMaxTop], zid[kMaxTop];
-    __shared__ int32_t id[kMaxTop];
+// What the threads of a row share after its sums are known.
+struct RowShared {
+    RowSums parts[16];
+    int32_t id[kMaxTop + 1];
+    float weight[kMaxTop + 1], z[kMaxTop + 1];
+};
+
+// The teacher's softmax over the slots in LDS (values in weight), by one wave: weight
+// becomes soft q. Returns sum_j q_j (ln q_j - (d_j rate - rest)).
+__device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate, float soft, float m, float rest) {
+    const int lane = threadIdx.x & 63;
+    float t[kMaxTop / 64], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMaxTop / 64; ++i) {
+        t[i] = lane + 64 * i < k ? sh.weight[lane + 64 * i] : -INFINITY;
+        top = fmaxf(top, ranked(t[i]));
+    }
+    top = wave_max(top);
+    // (a row of empty slots has no teacher: every share 0)
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxTop / 64; ++i) {
+        t[i] = (t[i] - base) * rate;
+        sum += __builtin_amdgcn_exp2f(t[i] * kLog2e);
+    }
+    sum = wave_sum(sum);
+    const float f = top == -INFINITY ? 0.0f : 1.0f / sum, log_sum = logf(sum);
+    float kl = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxTop / 64; ++i) {
+        const int j = lane + 64 * i;
+        if (j >= k) break;
+        const float q = __builtin_amdgcn_exp2f(t[i] * kLog2e) * f;
+        if (q != 0.0f) kl += q * ((t[i] - log_sum) - ((sh.z[j] - m) * rate - rest));
+        sh.weight[j] = soft * q;
+    }
+    return wave_sum(kl);
+}
+
+template <int NT, int NV, int KIND>
+__global__ __launch_bounds__(NT) void rows_kernel(RowArgs p) {
+    constexpr int kCols = 4 * NT * NV;
+    __shared__ RowShared sh;
     const int64_t row = blockIdx.x, v = p.vocab;
     const float *z = p.logits + row * v;
-    float *out = p.dlogits ? p.dlogits + row * v : nullptr;
-    const int tid = threadIdx.x;
-    const int64_t t = p.targets ? p.targets[row] : -1;
+    float *out = p.out ? p.out + row * v : nullptr;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int stretches = (int)((v + kCols - 1) / kCols);
+    auto cols_of = [&](int i) { return (int)min((int64_t)kCols, v - (int64_t)i * kCols); };
+    const int32_t t = p.targets ? p.targets[row] : -1;
     if (p.targets && t == p.ignore) {
-        if (tid == 0) p.row_loss[row] = 0.0f;
+        if (KIND != KIND_SCORES && tid == 0) p.row_loss[row] = 0.0f;
         if (out)
-            for (int64_t j = tid; j < v; j += 256) out[j] = 0.0f;
+            for (int64_t j = tid; j < v; j += NT) out[j] = 0.0f;
         return;
     }
-    const float rate = 1.0f / p.temperature;
-    const RowSums s = row_sums<256, SUMS_BOTH>(z, v, rate, lds);
-    const float zt = t >= 0 ? logit(z[t]) : 0.0f;
-    if (tid < p.k) {
-        const int32_t i = p.ids[row * p.k + tid];
-        const bool ok = i >= 0 && i < v;
-        if (i >= v) *p.wrong = 1;
-        id[tid] = ok ? i : -1;
-        q[tid] = ok ? logit(p.teacher[row * p.k + tid]) : -INFINITY;
-        zid[tid] = ok ? logit(z[i]) : 0.0f;
+    // slots 0 .. k - 1 the teacher's, slot k the target
+    const int k = KIND == KIND_SCORES ? 0 : p.k;
+    for (int j = tid; j <= k; j += NT) {
+        int32_t id = j < k ? p.ids[row * k + j] : t;
+        if (j < k && id >= v) *p.wrong = 1;
+        if (id >= v) id = -1;
+        sh.id[j] = id;
+        sh.z[j] = id >= 0 ? z[id] : 0.0f;
+        if (KIND != KIND_SCORES && j < k) sh.weight[j] = id >= 0 ? p.teacher[row * k + j] : -INFINITY;
+    }
+    const float rate = p.rate, kx = rate * kLog2e;
+    float e[NV][4];
+    RowSums s = no_sums();
+    for (int i = 0; i < stretches; ++i) {
+        load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
+        add_stretch<KIND>(s, e, kx);
+    }
+    s = wave_sums(s);
+    if ((tid & 63) == 0) sh.parts[wave] = s;
+    __syncthreads();
+    s = join_sums<KIND>(sh.parts, NT / 64, kx);
+    const float a = rest_of(s), total = 1.0f + a;
+    float f0, f1 = 0.0f, hit;  // dense gradient, and what the target's has beside it
+    if constexpr (KIND == KIND_SCORES) {
+        const float rest = log1pf(a), h = rest - s.u / total;
+        const float dl = p.dlogprobs ? p.dlogprobs[row] : 0.0f, dh = p.dentropy ? p.dentropy[row] : 0.0f;
+        f0 = (-dl - dh * (h - rest)) / total;
+        f1 = -dh / total;
+        hit = -dl;
+    } else {
+        const float soft = p.alpha * p.temperature * p.scale, hard = (1.0f - p.alpha) * p.scale;
+        const float rest1 = s.u + (s.count - 1.0f);  // (KIND_BOTH)
+        f0 = (KIND == KIND_BOTH ? soft : soft + hard) / total;
+        if (KIND == KIND_BOTH) f1 = hard / (1.0f + rest1);
+        hit = hard;
+        if (wave == 0) {
+            const float kl = teacher_terms(sh, k, rate, soft, s.m, log1pf(a));
+            float loss = 0.0f;
+            if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
+            if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(KIND == KIND_BOTH ? rest1 : a) - (sh.z[k] - s.m));
+            // (without a distribution the loss is NaN, also where no term above has met it)
+            if (a != a) loss = a;
+            if (tid == 0) p.row_loss[row] = loss;
+        }
+        if (!out) return;
+    }
+    auto dense = [&](float x) {
+        const float d = x - s.m;
+        if (KIND == KIND_SCORES) return __builtin_amdgcn_exp2f(d * kx) * __builtin_fmaf(fmaxf(d, kFar), f1, f0);
+        const float g = __builtin_amdgcn_exp2f(d * kx) * f0;
+        return KIND == KIND_BOTH ? __builtin_fmaf(__builtin_amdgcn_exp2f(d * kLog2e), f1, g) : g;
+    };
+    // (the last stretch first: it is still here)
+    for (int i = stretches - 1; i >= 0; --i) {
+        if (i < stretches - 1) load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
+#pragma unroll
+        for (int r = 0; r < NV; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[r][j] = dense(e[r][j]);
+        store_stretch<NT, NV>(out + (int64_t)i * kCols, cols_of(i), e);
     }
     __syncthreads();
-    float top = -INFINITY;
-    for (int j = 0; j < p.k; ++j) top = fmaxf(top, q[j]);
-    float sum = 0.0f;
-    if (top > -INFINITY)
-        for (int j = 0; j < p.k; ++j) sum += exp_neg((q[j] - top) * rate);
-    __syncthreads();
-    if (tid < p.k) {
-        const float u = (q[tid] - top) * rate, share = top > -INFINITY ? exp_neg(u) / sum : 0.0f;
-        q[tid] = share;
-        term[tid] = share == 0.0f ? 0.0f : share * ((u - logf(sum)) - ((zid[tid] - s.m) * rate - log1pf(s.a)));
+    // The few tokens' own values: an id's first slot takes the shares of all its slots.
+    for (int j = tid; j <= k; j += NT) {
+        const int32_t id = sh.id[j];
+        if (id < 0) continue;
+        float w = 0.0f;
+        bool first = true;
+        for (int i = 0; i <= k; ++i)
+            if (sh.id[i] == id) {
+                first = first && i >= j;
+                w += i < k ? sh.weight[i] : hit;
+            }
+        if (first) out[id] = dense(sh.z[j]) - w;
     }
-    __syncthreads();
-    if (tid == 0) {
-        float kl = 0.0f;
-        for (int j = 0; j < p.k; ++j) kl += term[j];
-        float loss = 0.0f;
-        if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
-        if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(s.u) - (zt - s.m));
-        p.row_loss[row] = loss;
-    }
-    if (!out) return;
-    const float soft = p.alpha * p.temperature * p.scale, hard = (1.0f - p.alpha) * p.scale;
-    for (int64_t j = tid; j < v; j += 256) {
-        const float d = fmaxf(logit(z[j]) - s.m, -1e30f);
-        float g = exp_neg(d * rate) / (1.0f + s.a) * soft + exp_neg(d) / (1.0f + s.u) * hard;
-        for (int i = 0; i < p.k; ++i)
-            if (id[i] == j) g -= soft * q[i];
-        if (j == t) g -= hard;
-        out[j] = g;
-    }
+}
+
+template <int KIND>
+void launch_rows(Context &cx, const RowArgs &p, int64_t rows) {
+    auto launch = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, cx.stream, p);
+    };
+    if (p.vocab <= 1024) launch(rows_kernel<256, 1, KIND>, 256);
+    else if (p.vocab <= 4096) launch(rows_kernel<256, 4, KIND>, 256);
+    else if (p.vocab <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
+    else if (p.vocab <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
+    else launch(rows_kernel<512, 16, KIND>, 512);
+    check_hip(hipGetLastError(), "rows launch");
 }
 
 void check_logits(const char *what, const float *logits, const int32_t *targets, int64_t n, int64_t vocab,
@@ -292,12 +431,13 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
     const int64_t kept = d.targets ? d.n - std::count(d.targets, d.targets + d.n, d.ignore) : d.n;
     int32_t *pinned = static_cast<int32_t *>(cx.pinned_rows((size_t)(2 * d.n + 16) * 4));
     Drain drain{cx};
-    DistillArgs p;
+    RowArgs p{};
     p.vocab = d.vocab;
     p.ignore = d.ignore;
-    p.k = (int)d.k;
+    p.k = d.alpha > 0.0f ? (int)d.k : 0;  // (the teacher has no share at alpha 0)
     p.temperature = d.temperature;
     p.alpha = d.alpha;
+    p.rate = d.alpha > 0.0f ? 1.0f / d.temperature : 1.0f;
     p.scale = 1.0f / (float)std::max<int64_t>(1, kept);
     p.wrong = pinned;
     *pinned = 0;
@@ -311,9 +451,10 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
         p.ids = d.ids + at * d.k;
         p.teacher = d.teacher + at * d.k;
         p.row_loss = rows + at;
-        p.dlogits = dlogits ? dlogits + at * d.vocab : nullptr;
-        hipLaunchKernelGGL(distill_kernel, dim3((unsigned)n), dim3(256), 0, cx.stream, p);
-        check_hip(hipGetLastError(), "distillation launch");
+        p.out = dlogits ? dlogits + at * d.vocab : nullptr;
+        // (with one temperature, or one term, one exponential serves both)
+        if (d.alpha > 0.0f && d.alpha < 1.0f && d.temperature != 1.0f) launch_rows<KIND_BOTH>(cx, p, n);
+        else launch_rows<KIND_ONE>(cx, p, n);
     }
     const float mean = mean_loss(drain, rows, d.n, std::max<int64_t>(1, kept));
     if (*(volatile int32_t *)p.wrong)
@@ -387,10 +528,16 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits, const i
         const int32_t *targets = targets_host ? cx.stage_ids(targets_host, n, 1) : nullptr;
         for (int64_t at = 0; at < n; at += kMaxRows) {
             const int64_t rows = std::min(kMaxRows, n - at);
-            hipLaunchKernelGGL(scores_grad_kernel, dim3((unsigned)rows), dim3(256), 0, cx.stream, logits + at * vocab,
-                               targets ? targets + at : nullptr, vocab, ignore, dlogprobs ? dlogprobs + at : nullptr,
-                               dentropy ? dentropy + at : nullptr, dlogits + at * vocab);
-            check_hip(hipGetLastError(), "token_logprobs gradient launch");
+            RowArgs p{};
+            p.logits = logits + at * vocab;
+            p.targets = targets ? targets + at : nullptr;
+            p.vocab = vocab;
+            p.ignore = ignore;
+            p.dlogprobs = dlogprobs ? dlogprobs + at : nullptr;
+            p.dentropy = dentropy ? dentropy + at : nullptr;
+            p.rate = 1.0f;
+            p.out = dlogits + at * vocab;
+            launch_rows<KIND_SCORES>(cx, p, rows);
         }
         return MMH_OK;
     });
