@@ -31,6 +31,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // its product with that 0 is one)
 constexpr float kFar = -200.0f;
 
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
@@ -64,8 +66,23 @@ __device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e
         for (int j = 0; j < 4; ++j) e[i][j] = c + j < cols ? z[c + j] : -INFINITY;
     }
 }
+// `stream`: past the caches, for outputs that they would not hold until they are read.
 template <int NT, int NV>
-__device__ __forceinline__ void store_stretch(float *out, int cols, const float (&e)[NV][4]) {
+__device__ __forceinline__ void store_stretch(float *out, int cols, bool stream, const float (&e)[NV][4]) {
+    if (stream) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = 4 * (threadIdx.x + NT * i);
+            if (c + 4 <= cols) {
+                float4u x;
+                __builtin_memcpy(&x, e[i], 16);
+                __builtin_nontemporal_store(x, reinterpret_cast<float4u *>(out + c));
+            } else {
+                store4(out + c, max(0, cols - c), e[i]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = 4 * (threadIdx.x + NT * i);
@@ -125,14 +142,15 @@ __device__ __forceinline__ RowSums wave_sums(RowSums s) {
     if (s.a != s.a) s.m = s.a;
     return s;
 }
-// One of n sums of the parts of a row. Those of a row whose largest logit is not finite
-// (nothing but -inf, an infinity or a NaN) are NaN: inf - inf is one.
+// The sums of n parts of a row together. (A part of nothing but -inf adds nothing; inf -
+// inf is NaN.)
 template <int KIND>
 __device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, float k) {
     RowSums s = no_sums();
     for (int i = 0; i < n; ++i) s.m = fmaxf(s.m, parts[i].m);
     for (int i = 0; i < n; ++i) {
         const RowSums p = parts[i];
+        if (p.m == -INFINITY) continue;
         const float d = p.m - s.m;
         if (d == 0.0f) {
             s.count += p.count;
@@ -145,6 +163,17 @@ __device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, float 
             if (KIND == KIND_BOTH) s.u += (p.u + p.count) * __builtin_amdgcn_exp2f(d * kLog2e);
         }
     }
+    return s;
+}
+// (as wave_sums: a NaN shows in m, so that it is not taken for a part of -inf)
+__device__ __forceinline__ RowSums with_nan(RowSums s) {
+    if (s.a != s.a) s.m = s.a;
+    return s;
+}
+// A whole row's: one whose largest logit is not finite (nothing but -inf, an infinity or
+// a NaN) has no distribution, and what is formed from NaN sums is NaN.
+__device__ __forceinline__ RowSums row_sums(RowSums s) {
+    if (!(fabsf(s.m) < INFINITY)) s.a = s.u = __builtin_nanf("");
     return s;
 }
 // S - 1: the sum without one of the largest logits' terms.
@@ -197,7 +226,7 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoreArgs p) {
     s = wave_sums(s);
     if ((tid & 63) == 0) lds[tid >> 6] = s;
     __syncthreads();
-    s = join_sums<KIND_SCORES>(lds, 4, kLog2e);
+    s = row_sums(join_sums<KIND_SCORES>(lds, 4, kLog2e));
     const float a = rest_of(s), rest = log1pf(a);
     if (tid == 0 && p.logprobs) p.logprobs[row] = (z[t] - s.m) - rest;
     if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
@@ -241,6 +270,12 @@ struct RowArgs {
     float rate;                       // of the first exponential: 1 / temperature, or 1 (KIND_SCORES, alpha 0)
     float *row_loss;                  // [rows], 0 for a row that is left out
     int32_t *wrong;                   // receives 1 for a teacher's id beyond the vocabulary
+    bool stream;
+    // a row over several workgroups (parts_kernel, parts_grad_kernel)
+    int64_t part;     // columns of a part, a multiple of 4
+    int parts;
+    RowSums *sums;    // [rows, parts]
+    float *slot_z;    // [rows, k + 1]
 };
 
 // What the threads of a row share after its sums are known.
@@ -283,111 +318,278 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate,
     return wave_sum(kl);
 }
 
-template <int NT, int NV, int KIND>
-__global__ __launch_bounds__(NT) void rows_kernel(RowArgs p) {
-    constexpr int kCols = 4 * NT * NV;
-    __shared__ RowShared sh;
-    const int64_t row = blockIdx.x, v = p.vocab;
-    const float *z = p.logits + row * v;
-    float *out = p.out ? p.out + row * v : nullptr;
-    const int tid = threadIdx.x, wave = tid >> 6;
-    const int stretches = (int)((v + kCols - 1) / kCols);
-    auto cols_of = [&](int i) { return (int)min((int64_t)kCols, v - (int64_t)i * kCols); };
-    const int32_t t = p.targets ? p.targets[row] : -1;
-    if (p.targets && t == p.ignore) {
-        if (KIND != KIND_SCORES && tid == 0) p.row_loss[row] = 0.0f;
-        if (out)
-            for (int64_t j = tid; j < v; j += NT) out[j] = 0.0f;
-        return;
-    }
-    // slots 0 .. k - 1 the teacher's, slot k the target
-    const int k = KIND == KIND_SCORES ? 0 : p.k;
-    for (int j = tid; j <= k; j += NT) {
+// The slots 0 .. k - 1 of a row, the teacher's, and slot k, its target, whose columns
+// are at .. at + cols - 1: each slot's logit to z_of (LDS or memory).
+template <int NT>
+__device__ __forceinline__ void read_slots(const RowArgs &p, int64_t row, int k, int32_t t, RowShared &sh) {
+    for (int j = threadIdx.x; j <= k; j += NT) {
         int32_t id = j < k ? p.ids[row * k + j] : t;
-        if (j < k && id >= v) *p.wrong = 1;
-        if (id >= v) id = -1;
+        if (j < k && id >= p.vocab) *p.wrong = 1;
+        if (id >= p.vocab) id = -1;
         sh.id[j] = id;
-        sh.z[j] = id >= 0 ? z[id] : 0.0f;
-        if (KIND != KIND_SCORES && j < k) sh.weight[j] = id >= 0 ? p.teacher[row * k + j] : -INFINITY;
+        if (j < k) sh.weight[j] = id >= 0 ? p.teacher[row * k + j] : -INFINITY;
     }
-    const float rate = p.rate, kx = rate * kLog2e;
-    float e[NV][4];
-    RowSums s = no_sums();
-    for (int i = 0; i < stretches; ++i) {
-        load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
-        add_stretch<KIND>(s, e, kx);
+}
+
+// A row that is left out. Its part of the output is zeros.
+template <int NT>
+__device__ __forceinline__ void left_out(const RowArgs &p, int64_t row, int64_t at, int64_t cols) {
+    if (p.row_loss && at == 0 && threadIdx.x == 0) p.row_loss[row] = 0.0f;
+    if (!p.out) return;
+    float *out = p.out + row * p.vocab + at;
+    const float zero[4] = {};
+    for (int64_t j = 4 * (int64_t)threadIdx.x; j < cols; j += 4 * NT) store4(out + j, (int)min((int64_t)4, cols - j), zero);
+}
+
+// A row's dense gradient exp2((z - m) k) (f0 + f1 (z - m)) (KIND_SCORES; KIND_ONE: f1 =
+// 0; KIND_BOTH: f1 times the second exponential instead), and what its target has less.
+struct Dense {
+    float m, kx, f0, f1, hit;
+    template <int KIND>
+    __device__ __forceinline__ float at(float x) const {
+        const float d = x - m;
+        if (KIND == KIND_SCORES) return __builtin_amdgcn_exp2f(d * kx) * __builtin_fmaf(fmaxf(d, kFar), f1, f0);
+        const float g = __builtin_amdgcn_exp2f(d * kx) * f0;
+        return KIND == KIND_BOTH ? __builtin_fmaf(__builtin_amdgcn_exp2f(d * kLog2e), f1, g) : g;
     }
-    s = wave_sums(s);
-    if ((tid & 63) == 0) sh.parts[wave] = s;
-    __syncthreads();
-    s = join_sums<KIND>(sh.parts, NT / 64, kx);
+};
+
+// From the row's sums, by every thread; wave 0 turns the teacher's slots into shares,
+// and its lane 0 writes the row's loss where `loss`.
+template <int KIND>
+__device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int k, const RowSums &s, bool loss_too,
+                                              RowShared &sh) {
     const float a = rest_of(s), total = 1.0f + a;
-    float f0, f1 = 0.0f, hit;  // dense gradient, and what the target's has beside it
+    Dense g{s.m, p.rate * kLog2e, 0.0f, 0.0f, 0.0f};
     if constexpr (KIND == KIND_SCORES) {
         const float rest = log1pf(a), h = rest - s.u / total;
         const float dl = p.dlogprobs ? p.dlogprobs[row] : 0.0f, dh = p.dentropy ? p.dentropy[row] : 0.0f;
-        f0 = (-dl - dh * (h - rest)) / total;
-        f1 = -dh / total;
-        hit = -dl;
+        g.f0 = (-dl - dh * (h - rest)) / total;
+        g.f1 = -dh / total;
+        g.hit = -dl;
     } else {
         const float soft = p.alpha * p.temperature * p.scale, hard = (1.0f - p.alpha) * p.scale;
         const float rest1 = s.u + (s.count - 1.0f);  // (KIND_BOTH)
-        f0 = (KIND == KIND_BOTH ? soft : soft + hard) / total;
-        if (KIND == KIND_BOTH) f1 = hard / (1.0f + rest1);
-        hit = hard;
-        if (wave == 0) {
-            const float kl = teacher_terms(sh, k, rate, soft, s.m, log1pf(a));
+        g.f0 = (KIND == KIND_BOTH ? soft : soft + hard) / total;
+        if (KIND == KIND_BOTH) g.f1 = hard / (1.0f + rest1);
+        g.hit = hard;
+        if (threadIdx.x < 64) {
+            const float kl = teacher_terms(sh, k, p.rate, soft, s.m, log1pf(a));
             float loss = 0.0f;
             if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
             if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(KIND == KIND_BOTH ? rest1 : a) - (sh.z[k] - s.m));
             // (without a distribution the loss is NaN, also where no term above has met it)
             if (a != a) loss = a;
-            if (tid == 0) p.row_loss[row] = loss;
+            if (loss_too && threadIdx.x == 0) p.row_loss[row] = loss;
         }
-        if (!out) return;
     }
-    auto dense = [&](float x) {
-        const float d = x - s.m;
-        if (KIND == KIND_SCORES) return __builtin_amdgcn_exp2f(d * kx) * __builtin_fmaf(fmaxf(d, kFar), f1, f0);
-        const float g = __builtin_amdgcn_exp2f(d * kx) * f0;
-        return KIND == KIND_BOTH ? __builtin_fmaf(__builtin_amdgcn_exp2f(d * kLog2e), f1, g) : g;
-    };
+    return g;
+}
+
+// The few tokens' own values, for columns at .. at + cols - 1, after the dense ones: an
+// id's first slot takes the shares of all its slots.
+template <int NT, int KIND>
+__device__ __forceinline__ void patch(float *out, int64_t at, int64_t cols, int k, const Dense &g, const RowShared &sh) {
+    for (int j = threadIdx.x; j <= k; j += NT) {
+        const int32_t id = sh.id[j];
+        if (id < at || id >= at + cols) continue;
+        float w = 0.0f;
+        bool first = true;
+        for (int i = 0; i <= k; ++i)
+            if (sh.id[i] == id) {
+                first = first && i >= j;
+                w += i < k ? sh.weight[i] : g.hit;
+            }
+        if (first) out[id] = g.at<KIND>(sh.z[j]) - w;
+    }
+}
+
+template <int NT, int NV, int KIND>
+__global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
+    constexpr int kCols = 4 * NT * NV;
+    __shared__ RowShared sh;
+    const int64_t row = blockIdx.x, v = p.vocab;
+    const float *z = p.logits + row * v;
+    const int tid = threadIdx.x;
+    const int stretches = (int)((v + kCols - 1) / kCols);
+    auto cols_of = [&](int i) { return (int)min((int64_t)kCols, v - (int64_t)i * kCols); };
+    const int32_t t = p.targets ? p.targets[row] : -1;
+    if (p.targets && t == p.ignore) return left_out<NT>(p, row, 0, v);
+    const int k = KIND == KIND_SCORES ? 0 : p.k;
+    read_slots<NT>(p, row, k, t, sh);
+    for (int j = tid; j <= k; j += NT) sh.z[j] = sh.id[j] >= 0 ? z[sh.id[j]] : 0.0f;  // (a thread's own slots)
+    float e[NV][4];
+    RowSums s = no_sums();
+    for (int i = 0; i < stretches; ++i) {
+        load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
+        add_stretch<KIND>(s, e, p.rate * kLog2e);
+    }
+    s = wave_sums(s);
+    if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
+    __syncthreads();
+    s = row_sums(join_sums<KIND>(sh.parts, NT / 64, p.rate * kLog2e));
+    const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
+    if (!p.out) return;
+    float *out = p.out + row * v;
     // (the last stretch first: it is still here)
     for (int i = stretches - 1; i >= 0; --i) {
         if (i < stretches - 1) load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
 #pragma unroll
         for (int r = 0; r < NV; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[r][j] = dense(e[r][j]);
-        store_stretch<NT, NV>(out + (int64_t)i * kCols, cols_of(i), e);
+            for (int j = 0; j < 4; ++j) e[r][j] = g.at<KIND>(e[r][j]);
+        store_stretch<NT, NV>(out + (int64_t)i * kCols, cols_of(i), p.stream, e);
     }
     __syncthreads();
-    // The few tokens' own values: an id's first slot takes the shares of all its slots.
-    for (int j = tid; j <= k; j += NT) {
-        const int32_t id = sh.id[j];
-        if (id < 0) continue;
-        float w = 0.0f;
-        bool first = true;
-        for (int i = 0; i <= k; ++i)
-            if (sh.id[i] == id) {
-                first = first && i >= j;
-                w += i < k ? sh.weight[i] : hit;
-            }
-        if (first) out[id] = dense(sh.z[j]) - w;
+    patch<NT, KIND>(out, 0, v, k, g, sh);
+}
+
+// A row over several workgroups, one part of at most 4 NT NV columns each: first the
+// parts' sums and the slots' logits (dlogits may be the logits, which the second
+// launch overwrites), then the gradient.
+template <int NT, int NV, int KIND>
+__global__ __launch_bounds__(NT, 4) void parts_kernel(RowArgs p) {
+    __shared__ RowSums parts[NT / 64];
+    const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * p.part, v = p.vocab;
+    const int32_t t = p.targets ? p.targets[row] : -1;
+    if (p.targets && t == p.ignore) return;
+    const float *z = p.logits + row * v;
+    const int cols = (int)min(p.part, v - at), k = KIND == KIND_SCORES ? 0 : p.k;
+    for (int j = threadIdx.x; j <= k; j += NT) {
+        const int32_t id = j < k ? p.ids[row * k + j] : t;
+        if (id >= at && id < at + cols) p.slot_z[row * (k + 1) + j] = z[id];
+    }
+    float e[NV][4];
+    RowSums s = no_sums();
+    load_stretch<NT, NV>(z + at, cols, e);
+    add_stretch<KIND>(s, e, p.rate * kLog2e);
+    s = wave_sums(s);
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) p.sums[row * p.parts + blockIdx.x] = with_nan(join_sums<KIND>(parts, NT / 64, p.rate * kLog2e));
+}
+
+template <int NT, int NV, int KIND>
+__global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
+    __shared__ RowShared sh;
+    const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * p.part, v = p.vocab;
+    const int cols = (int)min(p.part, v - at);
+    const int32_t t = p.targets ? p.targets[row] : -1;
+    if (p.targets && t == p.ignore) return left_out<NT>(p, row, at, cols);
+    const float *z = p.logits + row * v;
+    const int k = KIND == KIND_SCORES ? 0 : p.k, tid = threadIdx.x;
+    const float kx = p.rate * kLog2e;
+    float e[NV][4];
+    if (p.out) load_stretch<NT, NV>(z + at, cols, e);
+    read_slots<NT>(p, row, k, t, sh);
+    for (int j = tid; j <= k; j += NT) sh.z[j] = sh.id[j] >= 0 ? p.slot_z[row * (k + 1) + j] : 0.0f;
+    // (one wave joins the parts' sums, in one order in every part)
+    if (tid < 64) {
+        RowSums s = no_sums();
+        for (int j = tid; j < p.parts; j += 64) {
+            const RowSums two[2] = {s, p.sums[row * p.parts + j]};
+            s = with_nan(join_sums<KIND>(two, 2, kx));
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            const RowSums o{__shfl_xor(s.m, off, 64), __shfl_xor(s.count, off, 64), __shfl_xor(s.a, off, 64), __shfl_xor(s.u, off, 64)};
+            const RowSums two[2] = {tid & off ? o : s, tid & off ? s : o};
+            s = with_nan(join_sums<KIND>(two, 2, kx));
+        }
+        if (tid == 0) sh.parts[0] = s;
+    }
+    __syncthreads();
+    const RowSums s = row_sums(sh.parts[0]);
+    const Dense g = coefficients<KIND>(p, row, k, s, blockIdx.x == 0, sh);
+    if (!p.out) return;
+    float *out = p.out + row * v;
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[r][j] = g.at<KIND>(e[r][j]);
+    store_stretch<NT, NV>(out + at, cols, p.stream, e);
+    __syncthreads();
+    patch<NT, KIND>(out, at, cols, k, g, sh);
+}
+
+// Outputs from this size on pass the caches by (what the GPU's last cache holds).
+constexpr int64_t kStreamBytes = int64_t(256) << 20;
+// Rows of up to kRowCols columns stay in one workgroup's registers.
+constexpr int64_t kRowCols = 32768;
+constexpr int kPartThreads = 256, kPartStrips = 8;
+constexpr int64_t kPartCols = 4 * kPartThreads * kPartStrips;
+// Rows by their parts in one pair of launches (their sums' workspace; a grid's y).
+constexpr int64_t kPartRows = 4096;
+
+// n rows from `row` on.
+RowArgs rows_from(RowArgs p, int64_t row) {
+    p.logits += row * p.vocab;
+    if (p.targets) p.targets += row;
+    if (p.out) p.out += row * p.vocab;
+    if (p.dlogprobs) p.dlogprobs += row;
+    if (p.dentropy) p.dentropy += row;
+    if (p.ids) p.ids += row * p.k;
+    if (p.teacher) p.teacher += row * p.k;
+    if (p.row_loss) p.row_loss += row;
+    return p;
+}
+
+template <int KIND>
+void launch_whole(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
+    for (int64_t at = first; at < end; at += kMaxRows) {
+        const RowArgs p = rows_from(all, at);
+        const int64_t rows = std::min(kMaxRows, end - at);
+        auto launch = [&](auto kernel, int threads) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, cx.stream, p);
+        };
+        if (p.vocab <= 1024) launch(rows_kernel<256, 1, KIND>, 256);
+        else if (p.vocab <= 4096) launch(rows_kernel<256, 4, KIND>, 256);
+        else if (p.vocab <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
+        else if (p.vocab <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
+        else if (p.vocab <= kRowCols) launch(rows_kernel<512, 16, KIND>, 512);
+        else launch(rows_kernel<1024, 8, KIND>, 1024);
+        check_hip(hipGetLastError(), "rows launch");
     }
 }
 
 template <int KIND>
-void launch_rows(Context &cx, const RowArgs &p, int64_t rows) {
-    auto launch = [&](auto kernel, int threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, cx.stream, p);
-    };
-    if (p.vocab <= 1024) launch(rows_kernel<256, 1, KIND>, 256);
-    else if (p.vocab <= 4096) launch(rows_kernel<256, 4, KIND>, 256);
-    else if (p.vocab <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
-    else if (p.vocab <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
-    else launch(rows_kernel<512, 16, KIND>, 512);
-    check_hip(hipGetLastError(), "rows launch");
+void launch_parts(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
+    const int64_t v = all.vocab, n = end - first, slots = KIND == KIND_SCORES ? 1 : all.k + 1;
+    // parts for two workgroups per CU, of 1024 columns at least
+    const int64_t want = std::max((v + kPartCols - 1) / kPartCols, std::min((v + 1023) / 1024, 2 * cx.cu_count / n));
+    const int64_t part = ((v + want - 1) / want + 3) / 4 * 4, parts = (v + part - 1) / part;
+    const int64_t block = std::min({n, kPartRows, std::max<int64_t>(1, (int64_t(1) << 23) / parts)});
+    const size_t sums = (size_t)(block * parts) * sizeof(RowSums);
+    char *ws = static_cast<char *>(cx.workspace(2, sums + (size_t)(block * slots) * 4));
+    for (int64_t at = first; at < end; at += block) {
+        RowArgs p = rows_from(all, at);
+        p.part = part;
+        p.parts = (int)parts;
+        p.sums = reinterpret_cast<RowSums *>(ws);
+        p.slot_z = reinterpret_cast<float *>(ws + sums);
+        const unsigned rows = (unsigned)std::min(block, end - at);
+        hipLaunchKernelGGL((parts_kernel<kPartThreads, kPartStrips, KIND>), dim3((unsigned)parts, rows), dim3(kPartThreads), 0, cx.stream, p);
+        check_hip(hipGetLastError(), "row parts launch");
+        hipLaunchKernelGGL((parts_grad_kernel<kPartThreads, kPartStrips, KIND>), dim3(p.out ? (unsigned)parts : 1u, rows),
+                           dim3(kPartThreads), 0, cx.stream, p);
+        check_hip(hipGetLastError(), "row parts launch");
+    }
+}
+
+// Rows in one workgroup's registers each, whole. Wider ones take a workgroup that fills a CU
+// and reads them twice; those past the last round of one for every CU go by parts.
+// targets_host: of the n rows, where some may be left out.
+template <int KIND>
+void launch_rows(Context &cx, RowArgs p, int64_t n, const int32_t *targets_host) {
+    p.stream = n * p.vocab * 4 >= kStreamBytes;
+    if (p.vocab <= kRowCols) return launch_whole<KIND>(cx, p, 0, n);
+    int64_t kept = n;
+    if (targets_host) kept -= std::count(targets_host, targets_host + n, p.ignore);
+    int64_t rest = kept % cx.cu_count, first = n;
+    for (; rest > 0; --first)
+        if (!targets_host || targets_host[first - 1] != p.ignore) --rest;
+    if (first > 0) launch_whole<KIND>(cx, p, 0, first);
+    if (first < n) launch_parts<KIND>(cx, p, first, n);
 }
 
 void check_logits(const char *what, const float *logits, const int32_t *targets, int64_t n, int64_t vocab,
@@ -444,18 +646,15 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
     float *rows = reinterpret_cast<float *>(pinned + 16);
     int32_t *targets = pinned + 16 + d.n;
     if (d.targets) std::copy(d.targets, d.targets + d.n, targets);
-    for (int64_t at = 0; at < d.n; at += kMaxRows) {
-        const int64_t n = std::min(kMaxRows, d.n - at);
-        p.logits = d.logits + at * d.vocab;
-        p.targets = d.targets ? targets + at : nullptr;
-        p.ids = d.ids + at * d.k;
-        p.teacher = d.teacher + at * d.k;
-        p.row_loss = rows + at;
-        p.out = dlogits ? dlogits + at * d.vocab : nullptr;
-        // (with one temperature, or one term, one exponential serves both)
-        if (d.alpha > 0.0f && d.alpha < 1.0f && d.temperature != 1.0f) launch_rows<KIND_BOTH>(cx, p, n);
-        else launch_rows<KIND_ONE>(cx, p, n);
-    }
+    p.logits = d.logits;
+    p.targets = d.targets ? targets : nullptr;
+    p.ids = d.ids;
+    p.teacher = d.teacher;
+    p.row_loss = rows;
+    p.out = dlogits;
+    // (with one temperature, or one term, one exponential serves both)
+    if (d.alpha > 0.0f && d.alpha < 1.0f && d.temperature != 1.0f) launch_rows<KIND_BOTH>(cx, p, d.n, d.targets);
+    else launch_rows<KIND_ONE>(cx, p, d.n, d.targets);
     const float mean = mean_loss(drain, rows, d.n, std::max<int64_t>(1, kept));
     if (*(volatile int32_t *)p.wrong)
         fail(MMH_ERR_INDEX, "distillation: a teacher's id is out of range for " + std::to_string(d.vocab));
@@ -526,19 +725,16 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits, const i
         apart(sd, {sl, se});
         Context &cx = context(ctx);
         const int32_t *targets = targets_host ? cx.stage_ids(targets_host, n, 1) : nullptr;
-        for (int64_t at = 0; at < n; at += kMaxRows) {
-            const int64_t rows = std::min(kMaxRows, n - at);
-            RowArgs p{};
-            p.logits = logits + at * vocab;
-            p.targets = targets ? targets + at : nullptr;
-            p.vocab = vocab;
-            p.ignore = ignore;
-            p.dlogprobs = dlogprobs ? dlogprobs + at : nullptr;
-            p.dentropy = dentropy ? dentropy + at : nullptr;
-            p.rate = 1.0f;
-            p.out = dlogits + at * vocab;
-            launch_rows<KIND_SCORES>(cx, p, rows);
-        }
+        RowArgs p{};
+        p.logits = logits;
+        p.targets = targets;
+        p.vocab = vocab;
+        p.ignore = ignore;
+        p.dlogprobs = dlogprobs;
+        p.dentropy = dentropy;
+        p.rate = 1.0f;
+        p.out = dlogits;
+        launch_rows<KIND_SCORES>(cx, p, n, targets_host);
         return MMH_OK;
     });
 }

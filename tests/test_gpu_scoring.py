@@ -281,6 +281,30 @@ def test_distillation(ctx, i):
             near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
 
 
+@pytest.mark.parametrize("v", [700, 5000, 30000, 40000, 140000])
+def test_gradients_of_masked_rows(ctx, v):
+    # few tokens left, whole stretches and parts of a row masked
+    n = 5
+    z, y, r = drawn(n, v, v)
+    for i, left in enumerate(([0, 1], [v - 1], [v // 2, v - 2, 3], range(0, v, 5), range(v // 3, v // 3 + 40))):
+        keep = np.zeros(v, bool)
+        keep[list(left)] = True
+        z[i, ~keep] = -np.inf if i != 2 else np.finfo(np.float32).min
+        y[i] = list(left)[0]
+    dl, dh = r.standard_normal(n).astype(np.float32), r.standard_normal(n).astype(np.float32)
+    g = run_logprobs_bwd(ctx, z, y, dl, dh)
+    near(g, *R.token_logprobs_backward(z, y, dl, dh), "dlogits")
+    assert (g[z < -1e30] == 0).all()
+    ids = np.tile(y[:, None], (1, 3))
+    ids[:, 2] = -1
+    teacher = r.standard_normal((n, 3)).astype(np.float32)
+    for temperature, alpha in ((1.0, 0.5), (2.0, 0.5), (0.001, 0.5), (1000.0, 1.0)):
+        loss, g = run_distill(ctx, z, y, ids, teacher, temperature, alpha)
+        row, tol, want, g_tol = R.distillation(z, y, ids, teacher, temperature, alpha, n)
+        near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
+        near(g, want, g_tol, "dlogits")
+
+
 def test_slots_of_every_kind(ctx):
     v = 5000
     z, y, r = drawn(9, v, 4)
