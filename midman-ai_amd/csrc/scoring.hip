@@ -50,8 +50,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 // 4-byte address, at which gfx950 moves 16 bytes as well. Loads of whole float4s are
 // unconditional (from the last one past the end), so all of them are in flight at once.
 template <int NT, int NV>
-__device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e)[NV][4]) {
-    const int tid = threadIdx.x;
+__device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e)[NV][4], int tid = threadIdx.x) {
     if (cols >= 4) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) __builtin_memcpy(e[i], z + min(4 * (tid + NT * i), cols - 4), 16);
@@ -66,77 +65,101 @@ __device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e
         for (int j = 0; j < 4; ++j) e[i][j] = c + j < cols ? z[c + j] : -INFINITY;
     }
 }
-// `stream`: past the caches, for outputs that they would not hold until they are read.
-template <int NT, int NV>
-__device__ __forceinline__ void store_stretch(float *out, int cols, bool stream, const float (&e)[NV][4]) {
-    if (stream) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = 4 * (threadIdx.x + NT * i);
-            if (c + 4 <= cols) {
-                float4u x;
-                __builtin_memcpy(&x, e[i], 16);
-                __builtin_nontemporal_store(x, reinterpret_cast<float4u *>(out + c));
-            } else {
-                store4(out + c, max(0, cols - c), e[i]);
-            }
-        }
-        return;
-    }
+// f of a stretch to `out`, each strip on its way as soon as it is formed. `stream`: past
+// the caches, for outputs that they would not hold until they are read. (A branch for
+// both ways at the stores alone would hold them back until all is formed: 4096 x 32000
+// 227 -> 237 us.)
+template <bool STREAM, int NT, int NV, class F>
+__device__ __forceinline__ void write_strips(float *out, int cols, const float (&e)[NV][4], int tid, F &&f) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = 4 * (threadIdx.x + NT * i);
-        store4(out + c, max(0, min(4, cols - c)), e[i]);
+        const int c = 4 * (tid + NT * i);
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = f(e[i][j]);
+        if (c + 4 <= cols) {
+            float4u x;
+            __builtin_memcpy(&x, v, 16);
+            if (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<float4u *>(out + c));
+            else *reinterpret_cast<float4u *>(out + c) = x;
+        } else {
+            store4(out + c, max(0, cols - c), v);
+        }
     }
+}
+template <int NT, int NV, class F>
+__device__ __forceinline__ void write_stretch(float *out, int cols, bool stream, const float (&e)[NV][4], int tid, F &&f) {
+    if (stream) write_strips<true, NT, NV>(out, cols, e, tid, f);
+    else write_strips<false, NT, NV>(out, cols, e, tid, f);
 }
 
 // ---- a row's sums ---------------------------------------------------------------
 // Of exp((z - m) rate), m the largest logit: `count` of the terms are 1 (z = m), a is
 // the sum of the others, and u the sum of exp(z - m) (z - m) (KIND_SCORES) or of the
-// others' terms at rate 1 (KIND_BOTH). A wave has one m, its lanes share count.
+// others' terms at rate 1 (KIND_BOTH). A wave's lanes have one m.
 enum Kind : int { KIND_SCORES = 0, KIND_ONE = 1, KIND_BOTH = 2 };
 struct RowSums {
     float m, count, a, u;
 };
 __device__ __forceinline__ RowSums no_sums() { return RowSums{-INFINITY, 0.0f, 0.0f, 0.0f}; }
 
-// Adds a stretch to a wave's running sums (per lane but for m and count). A NaN stays in a.
+// Adds a stretch to a wave's running sums (per lane but for m). A NaN stays in a. The
+// wave's largest logit lies in one group of strips as a rule: only there are its terms
+// told from the others, by a branch that the whole wave takes.
 template <int KIND, int NV>
 __device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4], float k) {
-    float top = -INFINITY;
+    constexpr int G = NV < 16 ? (NV + 3) / 4 : 4;
+    float top = -INFINITY, group[NV / G];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) top = fmaxf(top, fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])));
+    for (int g = 0; g < NV / G; ++g) {
+        group[g] = -INFINITY;
+#pragma unroll
+        for (int i = g * G; i < (g + 1) * G; ++i)
+            group[g] = fmaxf(group[g], fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])));
+        top = fmaxf(top, group[g]);
+    }
     top = wave_max(top);
     if (top > s.m) {
         // what is there is scaled to the new largest logit; its ones are ordinary terms
-        const float one = (threadIdx.x & 63) == 0 ? s.count : 0.0f;
         if (s.m > -INFINITY) {
             const float d = s.m - top, w = __builtin_amdgcn_exp2f(d * k);
-            if (KIND == KIND_SCORES) s.u = (s.u + fmaxf(d, kFar) * (s.a + one)) * w;
-            if (KIND == KIND_BOTH) s.u = (s.u + one) * __builtin_amdgcn_exp2f(d * kLog2e);
-            s.a = (s.a + one) * w;
+            if (KIND == KIND_SCORES) s.u = (s.u + fmaxf(d, kFar) * (s.a + s.count)) * w;
+            if (KIND == KIND_BOTH) s.u = (s.u + s.count) * __builtin_amdgcn_exp2f(d * kLog2e);
+            s.a = (s.a + s.count) * w;
         }
         s.m = top;
         s.count = 0.0f;
     }
     const float m = s.m == -INFINITY ? 0.0f : s.m;  // (nothing but -inf: terms of 0)
-    int ones = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float d = e[i][j] - m;
-            const float x = __builtin_amdgcn_exp2f(d * k);
-            const bool one = d == 0.0f;
-            ones += __popcll(__ballot(one));
-            s.a += one ? 0.0f : x;
-            if (KIND == KIND_SCORES) s.u = __builtin_fmaf(x, fmaxf(d, kFar), s.u);
-            if (KIND == KIND_BOTH) s.u += one ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
+    auto add = [&](float z, bool look) __attribute__((always_inline)) {
+        const float d = z - m;
+        float x = __builtin_amdgcn_exp2f(d * k), x1 = KIND == KIND_BOTH ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.0f;
+        if (look) {
+            // (selected by arithmetic: a selection would become a branch around the exponentials)
+            const float one = d == 0.0f ? 1.0f : 0.0f;
+            s.count += one;
+            x -= one;
+            x1 -= one;
         }
-    s.count += s.m == -INFINITY ? 0.0f : (float)ones;
+        s.a += x;
+        if (KIND == KIND_SCORES) s.u = __builtin_fmaf(x, fmaxf(d, kFar), s.u);
+        if (KIND == KIND_BOTH) s.u += x1;
+    };
+#pragma unroll
+    for (int g = 0; g < NV / G; ++g) {
+        if (__any(group[g] == m)) {
+            asm volatile("");  // (stays a branch of its own)
+#pragma unroll
+            for (int c = 0; c < 4 * G; ++c) add(e[g * G + c / 4][c % 4], true);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4 * G; ++c) add(e[g * G + c / 4][c % 4], false);
+        }
+    }
 }
 // The wave's sums in every lane; a NaN among its logits makes m one.
 __device__ __forceinline__ RowSums wave_sums(RowSums s) {
+    s.count = wave_sum(s.count);
     s.a = wave_sum(s.a);
     s.u = wave_sum(s.u);
     if (s.a != s.a) s.m = s.a;
@@ -318,18 +341,46 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate,
     return wave_sum(kl);
 }
 
-// The slots 0 .. k - 1 of a row, the teacher's, and slot k, its target, whose columns
-// are at .. at + cols - 1: each slot's logit to z_of (LDS or memory).
+// The slots of a row on their way to LDS: 0 .. k - 1 the teacher's, slot k its target.
+// Their loads go out with the target's, before it is known whether the row counts.
 template <int NT>
-__device__ __forceinline__ void read_slots(const RowArgs &p, int64_t row, int k, int32_t t, RowShared &sh) {
-    for (int j = threadIdx.x; j <= k; j += NT) {
-        int32_t id = j < k ? p.ids[row * k + j] : t;
-        if (j < k && id >= p.vocab) *p.wrong = 1;
-        if (id >= p.vocab) id = -1;
-        sh.id[j] = id;
-        if (j < k) sh.weight[j] = id >= 0 ? p.teacher[row * k + j] : -INFINITY;
+struct Slots {
+    static constexpr int N = (kMaxTop + NT) / NT;
+    int32_t id[N];
+    float weight[N], z[N];
+    __device__ __forceinline__ void load(const RowArgs &p, int64_t row, int k) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = threadIdx.x + NT * i;
+            id[i] = j < k ? p.ids[row * k + j] : -1;
+            weight[i] = j < k ? p.teacher[row * k + j] : 0.0f;
+        }
     }
-}
+    // z_of(slot, id): the id's logit
+    template <class F>
+    __device__ __forceinline__ void gather(const RowArgs &p, int k, int32_t t, F &&z_of) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = threadIdx.x + NT * i;
+            if (j == k) id[i] = t;
+            if (id[i] >= p.vocab) {
+                *p.wrong = 1;
+                id[i] = -1;
+            }
+            z[i] = id[i] < 0 ? 0.0f : z_of(j, id[i]);
+        }
+    }
+    __device__ __forceinline__ void store(int k, RowShared &sh) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = threadIdx.x + NT * i;
+            if (j > k) break;
+            sh.id[j] = id[i] < 0 ? -1 : id[i];
+            sh.weight[j] = id[i] < 0 ? -INFINITY : weight[i];
+            sh.z[j] = z[i];
+        }
+    }
+};
 
 // A row that is left out. Its part of the output is zeros.
 template <int NT>
@@ -404,41 +455,113 @@ __device__ __forceinline__ void patch(float *out, int64_t at, int64_t cols, int 
     }
 }
 
+// A row of up to 4 NT NV columns in a workgroup's registers: read once.
 template <int NT, int NV, int KIND>
 __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
-    constexpr int kCols = 4 * NT * NV;
     __shared__ RowShared sh;
-    const int64_t row = blockIdx.x, v = p.vocab;
-    const float *z = p.logits + row * v;
-    const int tid = threadIdx.x;
-    const int stretches = (int)((v + kCols - 1) / kCols);
-    auto cols_of = [&](int i) { return (int)min((int64_t)kCols, v - (int64_t)i * kCols); };
+    const int64_t row = blockIdx.x;
+    const int v = (int)p.vocab, tid = threadIdx.x;
+    const float *z = p.logits + row * p.vocab;
+    const int k = KIND == KIND_SCORES ? 0 : p.k;
+    Slots<NT> slots;
+    slots.load(p, row, k);
     const int32_t t = p.targets ? p.targets[row] : -1;
     if (p.targets && t == p.ignore) return left_out<NT>(p, row, 0, v);
-    const int k = KIND == KIND_SCORES ? 0 : p.k;
-    read_slots<NT>(p, row, k, t, sh);
-    for (int j = tid; j <= k; j += NT) sh.z[j] = sh.id[j] >= 0 ? z[sh.id[j]] : 0.0f;  // (a thread's own slots)
+    slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
     float e[NV][4];
     RowSums s = no_sums();
-    for (int i = 0; i < stretches; ++i) {
-        load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
-        add_stretch<KIND>(s, e, p.rate * kLog2e);
-    }
+    load_stretch<NT, NV>(z, v, e);
+    slots.store(k, sh);
+    add_stretch<KIND>(s, e, p.rate * kLog2e);
     s = wave_sums(s);
     if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
     __syncthreads();
     s = row_sums(join_sums<KIND>(sh.parts, NT / 64, p.rate * kLog2e));
     const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
     if (!p.out) return;
+    float *out = p.out + row * p.vocab;
+    // (addresses formed anew: kept from the loads they would take the row's registers)
+    int me = tid;
+    asm volatile("" : "+v"(me));
+    write_stretch<NT, NV>(out, v, p.stream, e, me, [&](float x) { return g.at<KIND>(x); });
+    __syncthreads();
+    patch<NT, KIND>(out, 0, v, k, g, sh);
+}
+
+// Wider rows, of 2048 R columns at least: 512 threads have a CU's registers, and hold the
+// row's last R strips there and L before them in LDS (98304 and 32768 columns of f32 with
+// 48 and 16). Only what comes before those is read twice. (`some`, 8 strips at a time, is
+// what passes through.)
+template <int R, int L, int KIND>
+__global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
+    constexpr int NT = 512, S = 8, kSome = 4 * NT * S;
+    static_assert(L % S == 0, "whole passes");
+    __shared__ RowShared sh;
+    __shared__ __attribute__((aligned(16))) float held[L ? L * NT * 4 : 4];
+    const int64_t row = blockIdx.x, v = p.vocab;
+    const float *z = p.logits + row * v;
+    const int tid = threadIdx.x;
+    const int k = KIND == KIND_SCORES ? 0 : p.k;
+    Slots<NT> slots;
+    slots.load(p, row, k);
+    const int32_t t = p.targets ? p.targets[row] : -1;
+    if (p.targets && t == p.ignore) return left_out<NT>(p, row, 0, v);
+    slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
+    slots.store(k, sh);
+    const float kx = p.rate * kLog2e;
+    RowSums s = no_sums();
+    // the row from behind: R strips, L strips, and passes of S before them
+    const int64_t in_lds = v - 4 * NT * R, before = max((int64_t)0, in_lds - 4 * NT * L);
+    const int passes = (int)((before + kSome - 1) / kSome);
+    {
+        float some[S][4];
+        for (int i = 0; i < passes; ++i) {
+            load_stretch<NT, S>(z + (int64_t)i * kSome, (int)min((int64_t)kSome, before - (int64_t)i * kSome), some);
+            add_stretch<KIND>(s, some, kx);
+        }
+#pragma unroll 1
+        for (int i = 0; i < L / S; ++i) {
+            const int64_t at = before + (int64_t)i * kSome;
+            load_stretch<NT, S>(z + at, (int)max((int64_t)0, min((int64_t)kSome, in_lds - at)), some);
+            add_stretch<KIND>(s, some, kx);
+#pragma unroll
+            for (int r = 0; r < S; ++r) __builtin_memcpy(__builtin_assume_aligned(&held[((i * S + r) * NT + tid) * 4], 16), some[r], 16);
+        }
+    }
+    const uint32_t lane_at = 16u * (uint32_t)tid;
+    float e[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        __builtin_memcpy(e[r], reinterpret_cast<const char *>(z + in_lds) + 16 * NT * r + lane_at, 16);
+        __builtin_amdgcn_sched_barrier(0);  // (one address at a time: no registers for more)
+    }
+    add_stretch<KIND>(s, e, kx);
+    s = wave_sums(s);
+    if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
+    __syncthreads();
+    s = row_sums(join_sums<KIND>(sh.parts, NT / 64, kx));
+    const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
+    if (!p.out) return;
     float *out = p.out + row * v;
-    // (the last stretch first: it is still here)
-    for (int i = stretches - 1; i >= 0; --i) {
-        if (i < stretches - 1) load_stretch<NT, NV>(z + (int64_t)i * kCols, cols_of(i), e);
+    // (the addresses from here on are formed anew: kept from the first pass they would
+    // take the registers that hold the row)
+    int me = tid;
+    asm volatile("" : "+v"(me));
+    auto turn = [&](float x) { return g.at<KIND>(x); };
+    write_stretch<NT, R>(out + in_lds, 4 * NT * R, p.stream, e, me, turn);
+#pragma unroll 1
+    for (int i = 0; i < L / S; ++i) {
+        float some[S][4];
 #pragma unroll
-        for (int r = 0; r < NV; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) e[r][j] = g.at<KIND>(e[r][j]);
-        store_stretch<NT, NV>(out + (int64_t)i * kCols, cols_of(i), p.stream, e);
+        for (int r = 0; r < S; ++r) __builtin_memcpy(some[r], __builtin_assume_aligned(&held[((i * S + r) * NT + me) * 4], 16), 16);
+        const int64_t at = before + (int64_t)i * kSome;
+        write_stretch<NT, S>(out + at, (int)max((int64_t)0, min((int64_t)kSome, in_lds - at)), p.stream, some, me, turn);
+    }
+    for (int i = passes - 1; i >= 0; --i) {
+        float some[S][4];
+        const int cols = (int)min((int64_t)kSome, before - (int64_t)i * kSome);
+        load_stretch<NT, S>(z + (int64_t)i * kSome, cols, some, me);
+        write_stretch<NT, S>(out + (int64_t)i * kSome, cols, p.stream, some, me, turn);
     }
     __syncthreads();
     patch<NT, KIND>(out, 0, v, k, g, sh);
@@ -481,8 +604,10 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     const float kx = p.rate * kLog2e;
     float e[NV][4];
     if (p.out) load_stretch<NT, NV>(z + at, cols, e);
-    read_slots<NT>(p, row, k, t, sh);
-    for (int j = tid; j <= k; j += NT) sh.z[j] = sh.id[j] >= 0 ? p.slot_z[row * (k + 1) + j] : 0.0f;
+    Slots<NT> slots;
+    slots.load(p, row, k);
+    slots.gather(p, k, t, [&](int j, int32_t) { return p.slot_z[row * (k + 1) + j]; });
+    slots.store(k, sh);
     // (one wave joins the parts' sums, in one order in every part)
     if (tid < 64) {
         RowSums s = no_sums();
@@ -503,11 +628,7 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     const Dense g = coefficients<KIND>(p, row, k, s, blockIdx.x == 0, sh);
     if (!p.out) return;
     float *out = p.out + row * v;
-#pragma unroll
-    for (int r = 0; r < NV; ++r)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) e[r][j] = g.at<KIND>(e[r][j]);
-    store_stretch<NT, NV>(out + at, cols, p.stream, e);
+    write_stretch<NT, NV>(out + at, cols, p.stream, e, tid, [&](float x) { return g.at<KIND>(x); });
     __syncthreads();
     patch<NT, KIND>(out, at, cols, k, g, sh);
 }
@@ -547,7 +668,9 @@ void launch_whole(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
         else if (p.vocab <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
         else if (p.vocab <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
         else if (p.vocab <= kRowCols) launch(rows_kernel<512, 16, KIND>, 512);
-        else launch(rows_kernel<1024, 8, KIND>, 1024);
+        else if (p.vocab <= 65536) launch(wide_rows_kernel<16, 16, KIND>, 512);
+        else if (p.vocab <= 98304) launch(wide_rows_kernel<32, 16, KIND>, 512);
+        else launch(wide_rows_kernel<48, 16, KIND>, 512);
         check_hip(hipGetLastError(), "rows launch");
     }
 }
@@ -585,7 +708,7 @@ void launch_rows(Context &cx, RowArgs p, int64_t n, const int32_t *targets_host)
     if (p.vocab <= kRowCols) return launch_whole<KIND>(cx, p, 0, n);
     int64_t kept = n;
     if (targets_host) kept -= std::count(targets_host, targets_host + n, p.ignore);
-    int64_t rest = kept % cx.cu_count, first = n;
+    int64_t rest = kept < 64 ? kept : 0, first = n;
     for (; rest > 0; --first)
         if (!targets_host || targets_host[first - 1] != p.ignore) --rest;
     if (first > 0) launch_whole<KIND>(cx, p, 0, first);
