@@ -199,6 +199,23 @@ __device__ __forceinline__ RowSums row_sums(RowSums s) {
     if (!(fabsf(s.m) < INFINITY)) s.a = s.u = __builtin_nanf("");
     return s;
 }
+// The sums of a row's n parts, by one wave: in every lane, in one order.
+template <int KIND>
+__device__ __forceinline__ RowSums wave_join(const RowSums *parts, int n, float k) {
+    const int lane = threadIdx.x & 63;
+    RowSums s = no_sums();
+    for (int j = lane; j < n; j += 64) {
+        const RowSums two[2] = {s, parts[j]};
+        s = with_nan(join_sums<KIND>(two, 2, k));
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const RowSums o{__shfl_xor(s.m, off, 64), __shfl_xor(s.count, off, 64), __shfl_xor(s.a, off, 64), __shfl_xor(s.u, off, 64)};
+        const RowSums two[2] = {lane & off ? o : s, lane & off ? s : o};
+        s = with_nan(join_sums<KIND>(two, 2, k));
+    }
+    return s;
+}
 // S - 1: the sum without one of the largest logits' terms.
 __device__ __forceinline__ float rest_of(const RowSums &s) { return s.a + (s.count - 1.0f); }
 
@@ -213,6 +230,11 @@ __device__ __forceinline__ float value_of(uint32_t order) {
 // (for the order of alternatives a NaN counts as +inf)
 __device__ __forceinline__ float ranked(float z) { return z != z ? INFINITY : z; }
 
+// ---- log probabilities, entropies and the most likely tokens -------------------------
+// The k largest of a stretch, without sorting it: the k-th largest of the threads'
+// maxima is no larger than the k-th largest logit, and only what is above it (a little
+// more than k logits as a rule) goes to a list in LDS, where each entry's place is the
+// number of larger ones.
 struct ScoreArgs {
     const float *logits;
     const int32_t *targets;  // device, or null
@@ -222,55 +244,326 @@ struct ScoreArgs {
     float *logprobs, *entropy;
     int32_t *top_ids;
     float *top_logprobs;
+    // rows over several workgroups: what a part leaves
+    int64_t part;         // columns of a part, a multiple of 4
+    int parts;
+    RowSums *sums;        // [rows, parts]
+    uint64_t *best;       // [rows, parts, k], the largest first
 };
 
-__global__ __launch_bounds__(256) void scores_kernel(ScoreArgs p) {
-    __shared__ RowSums lds[4];
-    __shared__ unsigned long long best;
-    const int64_t row = blockIdx.x;
+constexpr int kList = 1024;  // entries of the list; kMaxTop at least
+// An entry: larger for what comes first, the larger logit or the lower column.
+__device__ __forceinline__ uint64_t entry_of(float z, uint32_t col) { return (uint64_t)order_of(z) << 32 | (uint32_t)~col; }
+
+struct TopShared {
+    uint32_t maxima[1024];  // of the threads, as orders
+    uint64_t list[kList];
+    int32_t count[16];
+    int32_t n;              // entries of the list
+    float above;            // logits above it are in the list
+};
+
+// The number, over the workgroup, of logits above t.
+template <int NT, int NV>
+__device__ __forceinline__ int count_above(const float (&e)[NV][4], float t, TopShared &sh) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n += e[i][j] > t ? 1 : 0;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0;
+    for (int i = 0; i < NT / 64; ++i) n += sh.count[i];
+    return n;
+}
+
+// The k largest of a stretch (no NaN; -inf past its `cols`) to place(rank, entry), by
+// every thread of the workgroup; fewer where it has fewer columns.
+template <int NT, int NV, class F>
+__device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32_t first, int k, TopShared &sh, F &&place) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t lowest = order_of(-INFINITY);
+    k = min(k, cols);
+    float mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) mine = fmaxf(mine, fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])));
+    sh.maxima[tid] = order_of(mine);
+    __syncthreads();
+    if (tid < 64) {
+        // A value that k threads' maxima reach, and a quarter more at most where they differ:
+        // halving the range of orders.
+        uint32_t m[NT / 64], lo = lowest, hi = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            m[i] = sh.maxima[lane + 64 * i];
+            hi = max(hi, m[i]);
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, off, 64));
+        hi += 1;  // (lo is reached by k maxima or is the lowest, hi by none)
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(m[i] >= mid));
+            if (n < k) hi = mid;
+            else lo = mid;
+            if (n >= k && n <= k + k / 4) break;
+        }
+        if (tid == 0) {
+            sh.above = value_of(lo);
+            sh.n = 0;
+        }
+    }
+    __syncthreads();
+    float above = sh.above;
+    auto collect = [&] {
+        if (mine > above) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!(fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])) > above)) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (e[i][j] > above) {
+                        const int at = atomicAdd(&sh.n, 1);
+                        if (at < kList) sh.list[at] = entry_of(e[i][j], first + 4 * (tid + NT * i) + j);
+                    }
+            }
+        }
+        __syncthreads();
+    };
+    collect();
+    int n = sh.n;
+    if (n > kList) {
+        // Many of the largest logits are a few threads': the halving goes on over all of them,
+        // until what is above fits, or above and below are neighbours.
+        uint32_t lo = order_of(above), hi = 0;
+        for (int i = 0; i < NT; ++i) hi = max(hi, sh.maxima[i]);  // (more than kList above lo, none above hi)
+        while (n > kList && hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int c = count_above<NT, NV>(e, value_of(mid), sh);
+            if (c < k) hi = mid;
+            else lo = mid, n = c;
+        }
+        above = value_of(n > kList ? hi : lo);
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        collect();
+        n = sh.n;
+    }
+    if (n < k) {
+        // Fewer than k are above it, so it is the k-th largest logit itself: the lowest columns
+        // that hold it fill the list, strip by strip.
+        int have = n;
+        for (int i = 0; i < NV && have < k; ++i) {
+            float x[4];
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+                if (c == i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = e[c][j];
+                }
+            const int c0 = 4 * (tid + NT * i);
+            int before = have, here = 0;
+            uint64_t hit[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hit[j] = __ballot(x[j] == above && c0 + j < cols);
+                here += __popcll(hit[j]);
+            }
+            __syncthreads();
+            if (lane == 0) sh.count[tid >> 6] = here;
+            __syncthreads();
+            for (int w = 0; w < NT / 64; ++w) {
+                if (w < tid >> 6) before += sh.count[w];
+                have += sh.count[w];
+            }
+            // (columns run through the lanes, four to each)
+            const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) before += __popcll(hit[j] & below);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (hit[j] >> lane & 1) {
+                    if (before < k) sh.list[before] = entry_of(x[j], first + c0 + j);
+                    ++before;
+                }
+        }
+        __syncthreads();
+        n = k;
+    }
+    for (int i = tid; i < n; i += NT) {
+        const uint64_t me = sh.list[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += sh.list[j] > me ? 1 : 0;
+        if (rank < k) place(rank, me);
+    }
+}
+
+__device__ __forceinline__ void score_left_out(const ScoreArgs &p, int64_t row, int threads) {
+    if (threadIdx.x == 0 && p.logprobs) p.logprobs[row] = 0.0f;
+    if (threadIdx.x == 0 && p.entropy) p.entropy[row] = 0.0f;
+    for (int j = threadIdx.x; j < p.k; j += threads) {
+        p.top_ids[row * p.k + j] = -1;
+        p.top_logprobs[row * p.k + j] = -INFINITY;
+    }
+}
+
+// A row of up to 4 NT NV columns (PARTS: a part of one) in a workgroup's registers.
+template <int NT, int NV, bool PARTS>
+__global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
+    __shared__ RowSums lds[NT / 64];
+    __shared__ TopShared sh;
+    const int64_t row = PARTS ? blockIdx.y : blockIdx.x, at = PARTS ? (int64_t)blockIdx.x * p.part : 0;
     const float *z = p.logits + row * p.vocab;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, cols = (int)(PARTS ? min(p.part, p.vocab - at) : p.vocab);
     const int32_t t = p.targets ? p.targets[row] : 0;
     if (p.targets && t == p.ignore) {
-        if (tid == 0 && p.logprobs) p.logprobs[row] = 0.0f;
-        if (tid == 0 && p.entropy) p.entropy[row] = 0.0f;
-        for (int j = tid; j < p.k; j += 256) {
-            p.top_ids[row * p.k + j] = -1;
-            p.top_logprobs[row * p.k + j] = -INFINITY;
-        }
+        if (!PARTS) score_left_out(p, row, NT);
         return;
     }
+    float e[NV][4];
+    const float zt = !PARTS && p.logprobs && tid == 0 ? z[t] : 0.0f;
+    load_stretch<NT, NV>(z + at, cols, e);
     RowSums s = no_sums();
-    for (int64_t c = 0; c < p.vocab; c += 4096) {
-        float e[4][4];
-        load_stretch<256, 4>(z + c, (int)min((int64_t)4096, p.vocab - c), e);
-        add_stretch<KIND_SCORES>(s, e, kLog2e);
-    }
+    add_stretch<KIND_SCORES>(s, e, kLog2e);
     s = wave_sums(s);
     if ((tid & 63) == 0) lds[tid >> 6] = s;
     __syncthreads();
-    s = row_sums(join_sums<KIND_SCORES>(lds, 4, kLog2e));
+    s = join_sums<KIND_SCORES>(lds, NT / 64, kLog2e);
+    const bool odd = s.a != s.a;
+    float rest = 0.0f;
+    if constexpr (PARTS) {
+        if (tid == 0) p.sums[row * p.parts + blockIdx.x] = with_nan(s);
+    } else {
+        s = row_sums(s);
+        const float a = rest_of(s);
+        rest = log1pf(a);
+        if (tid == 0 && p.logprobs) p.logprobs[row] = (zt - s.m) - rest;
+        if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
+    }
+    if (p.k == 0) return;
+    if (odd) {
+        // (for the order of alternatives a NaN counts as +inf)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[i][j] = e[i][j] != e[i][j] ? INFINITY : e[i][j];
+    }
+    const float m = s.m;
+    top_of<NT, NV>(e, cols, (uint32_t)at, p.k, sh, [&](int rank, uint64_t entry) {
+        if constexpr (PARTS) {
+            p.best[(row * p.parts + blockIdx.x) * p.k + rank] = entry;
+        } else {
+            p.top_ids[row * p.k + rank] = (int32_t) ~(uint32_t)entry;
+            p.top_logprobs[row * p.k + rank] = (value_of((uint32_t)(entry >> 32)) - m) - rest;
+        }
+    });
+}
+
+// The parts of a row together: their sums, and of their lists the k that come first, each
+// entry's place the number of larger ones in its own list and, by halving, in the others.
+constexpr int kJoinEntries = 4096;
+__global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
+    __shared__ RowSums all;
+    __shared__ uint64_t held[kJoinEntries];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, k = p.k, entries = p.parts * k;
+    const int32_t t = p.targets ? p.targets[row] : 0;
+    if (p.targets && t == p.ignore) return score_left_out(p, row, 256);
+    const uint64_t *best = p.best + row * p.parts * k;
+    const bool in_lds = entries <= kJoinEntries;
+    if (in_lds)
+        for (int i = tid; i < entries; i += 256) held[i] = best[i];
+    if (tid < 64) {
+        const RowSums s = wave_join<KIND_SCORES>(p.sums + row * p.parts, p.parts, kLog2e);
+        if (tid == 0) all = s;
+    }
+    __syncthreads();
+    const RowSums s = row_sums(all);
     const float a = rest_of(s), rest = log1pf(a);
-    if (tid == 0 && p.logprobs) p.logprobs[row] = (z[t] - s.m) - rest;
+    if (tid == 0 && p.logprobs) p.logprobs[row] = (p.logits[row * p.vocab + t] - s.m) - rest;
     if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
-    unsigned long long last = ~0ull;
-    for (int j = 0; j < p.k; ++j) {
-        if (tid == 0) best = 0;
-        __syncthreads();
-        unsigned long long mine = 0;
-        for (int64_t i = tid; i < p.vocab; i += 256) {
-            const unsigned long long key = (unsigned long long)order_of(ranked(z[i])) << 32 | (uint32_t)~(uint32_t)i;
-            if (key < last && key > mine) mine = key;
+    // (a part of fewer columns has a shorter list)
+    const int last = (int)min((int64_t)k, p.vocab - (int64_t)(p.parts - 1) * p.part), full = (int)min((int64_t)k, p.part);
+    auto place = [&](const uint64_t *lists) __attribute__((always_inline)) {
+        for (int i = tid; i < entries; i += 256) {
+            const int q = i / k;
+            int rank = i - q * k;
+            if (rank >= (q == p.parts - 1 ? last : full)) continue;
+            const uint64_t me = lists[i];
+            for (int o = 0; o < p.parts && rank < k; ++o) {
+                if (o == q) continue;
+                const uint64_t *list = lists + (int64_t)o * k;
+                int lo = 0, hi = o == p.parts - 1 ? last : full;  // larger ones: lo at least, hi at most
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (list[mid] > me) lo = mid + 1;
+                    else hi = mid;
+                }
+                rank += lo;
+            }
+            if (rank >= k) continue;
+            p.top_ids[row * k + rank] = (int32_t) ~(uint32_t)me;
+            p.top_logprobs[row * k + rank] = (value_of((uint32_t)(me >> 32)) - s.m) - rest;
         }
-        atomicMax(&best, mine);
-        __syncthreads();
-        last = best;
-        const int32_t id = (int32_t) ~(uint32_t)last;
-        if (tid == 0) {
-            p.top_ids[row * p.k + j] = id;
-            p.top_logprobs[row * p.k + j] = (z[id] - s.m) - rest;
-        }
-        __syncthreads();
+    };
+    if (in_lds) place(held);
+    else place(best);
+}
+
+// Columns of a part at most, and the bytes that the parts' lists may take.
+constexpr int64_t kScoreCols = 32768, kScoreBytes = int64_t(64) << 20;
+
+template <bool PARTS>
+void launch_scores(Context &cx, const ScoreArgs &p, dim3 grid, int64_t cols) {
+    auto launch = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, cx.stream, p); };
+    if (cols <= 1024) launch(scores_kernel<256, 1, PARTS>, 256);
+    else if (cols <= 4096) launch(scores_kernel<256, 4, PARTS>, 256);
+    else if (cols <= 8192) launch(scores_kernel<512, 4, PARTS>, 512);
+    else if (cols <= 16384) launch(scores_kernel<512, 8, PARTS>, 512);
+    else launch(scores_kernel<512, 16, PARTS>, 512);
+    check_hip(hipGetLastError(), "token_logprobs launch");
+}
+
+ScoreArgs rows_from(ScoreArgs p, int64_t row) {
+    p.logits += row * p.vocab;
+    if (p.targets) p.targets += row;
+    if (p.logprobs) p.logprobs += row;
+    if (p.entropy) p.entropy += row;
+    if (p.top_ids) p.top_ids += row * p.k;
+    if (p.top_logprobs) p.top_logprobs += row * p.k;
+    return p;
+}
+
+void scores(Context &cx, const ScoreArgs &all, int64_t n) {
+    const int64_t v = all.vocab;
+    if (v <= kScoreCols) {
+        for (int64_t at = 0; at < n; at += kMaxRows)
+            launch_scores<false>(cx, rows_from(all, at), dim3((unsigned)std::min(kMaxRows, n - at)), v);
+        return;
+    }
+    // parts for two workgroups per CU, of 4096 columns at least
+    const int64_t want = std::max((v + kScoreCols - 1) / kScoreCols, std::min((v + 4095) / 4096, 2 * cx.cu_count / n));
+    const int64_t part = ((v + want - 1) / want + 3) / 4 * 4, parts = (v + part - 1) / part;
+    const int64_t row_bytes = parts * ((int64_t)sizeof(RowSums) + 8 * all.k);
+    const int64_t block = std::min({n, std::max<int64_t>(1, kScoreBytes / row_bytes), std::max<int64_t>(1, (int64_t(1) << 22) / parts), int64_t(65535)});
+    char *ws = static_cast<char *>(cx.workspace(2, (size_t)(block * row_bytes)));
+    for (int64_t at = 0; at < n; at += block) {
+        ScoreArgs p = rows_from(all, at);
+        const unsigned rows = (unsigned)std::min(block, n - at);
+        p.part = part;
+        p.parts = (int)parts;
+        p.sums = reinterpret_cast<RowSums *>(ws);
+        p.best = reinterpret_cast<uint64_t *>(ws + block * parts * (int64_t)sizeof(RowSums));
+        launch_scores<true>(cx, p, dim3((unsigned)parts, rows), part);
+        hipLaunchKernelGGL(scores_join_kernel, dim3(rows), dim3(256), 0, cx.stream, p);
+        check_hip(hipGetLastError(), "token_logprobs launch");
     }
 }
 
@@ -608,20 +901,9 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     slots.load(p, row, k);
     slots.gather(p, k, t, [&](int j, int32_t) { return p.slot_z[row * (k + 1) + j]; });
     slots.store(k, sh);
-    // (one wave joins the parts' sums, in one order in every part)
     if (tid < 64) {
-        RowSums s = no_sums();
-        for (int j = tid; j < p.parts; j += 64) {
-            const RowSums two[2] = {s, p.sums[row * p.parts + j]};
-            s = with_nan(join_sums<KIND>(two, 2, kx));
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const RowSums o{__shfl_xor(s.m, off, 64), __shfl_xor(s.count, off, 64), __shfl_xor(s.a, off, 64), __shfl_xor(s.u, off, 64)};
-            const RowSums two[2] = {tid & off ? o : s, tid & off ? s : o};
-            s = with_nan(join_sums<KIND>(two, 2, kx));
-        }
-        if (tid == 0) sh.parts[0] = s;
+        const RowSums all = wave_join<KIND>(p.sums + row * p.parts, p.parts, kx);
+        if (tid == 0) sh.parts[0] = all;
     }
     __syncthreads();
     const RowSums s = row_sums(sh.parts[0]);
@@ -816,21 +1098,17 @@ int32_t mmh_token_logprobs(mmh_handle ctx, const float *logits, const int32_t *t
         Context &cx = context(ctx);
         if (!logprobs && !entropy && k == 0) return MMH_OK;
         const int32_t *targets = targets_host ? cx.stage_ids(targets_host, n, 1) : nullptr;
-        for (int64_t at = 0; at < n; at += kMaxRows) {
-            const int64_t rows = std::min(kMaxRows, n - at);
-            ScoreArgs p;
-            p.logits = logits + at * vocab;
-            p.targets = targets ? targets + at : nullptr;
-            p.vocab = vocab;
-            p.ignore = ignore;
-            p.k = (int)k;
-            p.logprobs = logprobs ? logprobs + at : nullptr;
-            p.entropy = entropy ? entropy + at : nullptr;
-            p.top_ids = top_ids + at * k;
-            p.top_logprobs = top_logprobs + at * k;
-            hipLaunchKernelGGL(scores_kernel, dim3((unsigned)rows), dim3(256), 0, cx.stream, p);
-            check_hip(hipGetLastError(), "token_logprobs launch");
-        }
+        ScoreArgs p{};
+        p.logits = logits;
+        p.targets = targets;
+        p.vocab = vocab;
+        p.ignore = ignore;
+        p.k = (int)k;
+        p.logprobs = logprobs;
+        p.entropy = entropy;
+        p.top_ids = top_ids;
+        p.top_logprobs = top_logprobs;
+        scores(cx, p, n);
         return MMH_OK;
     });
 }
