@@ -13,6 +13,7 @@
 // is log1p(rest): near a certain token the log probability and the entropy are as
 // small as the rest, and keep all their bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "mmh_args.h"
 #include "mmh_elementwise.h"
@@ -252,12 +253,22 @@ struct ScoreArgs {
 };
 
 constexpr int kList = 1024;  // entries of the list; kMaxTop at least
-// An entry: larger for what comes first, the larger logit or the lower column.
-__device__ __forceinline__ uint64_t entry_of(float z, uint32_t col) { return (uint64_t)order_of(z) << 32 | (uint32_t)~col; }
+constexpr int kColBits = 15; // of a column within its stretch
+// An entry of a stretch: larger for what comes first, the larger logit or the lower column.
+// Below 2^53, so an f64 holds it: those compare at the vector rate, 64-bit integers do not.
+__device__ __forceinline__ double entry_of(float z, int col) {
+    return (double)order_of(z) * (1 << kColBits) + (double)((1 << kColBits) - 1 - col);
+}
+// The same of a whole row.
+__device__ __forceinline__ uint64_t row_entry(double e, uint32_t first) {
+    const uint64_t b = (uint64_t)e;
+    const uint32_t col = (1u << kColBits) - 1 - (uint32_t)(b & ((1u << kColBits) - 1));
+    return b >> kColBits << 32 | (uint32_t)~(first + col);
+}
 
 struct TopShared {
-    uint32_t maxima[1024];  // of the threads, as orders
-    uint64_t list[kList];
+    __attribute__((aligned(16))) double list[kList + 16];
+    uint32_t maxima[512];  // of the threads, as orders
     int32_t count[16];
     int32_t n;              // entries of the list
     float above;            // logits above it are in the list
@@ -294,7 +305,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
     sh.maxima[tid] = order_of(mine);
     __syncthreads();
     if (tid < 64) {
-        // A value that k threads' maxima reach, and a quarter more at most where they differ:
+        // A value that k threads' maxima reach, and a quarter and 8 more at most where they differ:
         // halving the range of orders.
         uint32_t m[NT / 64], lo = lowest, hi = 0;
 #pragma unroll
@@ -312,7 +323,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
             for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(m[i] >= mid));
             if (n < k) hi = mid;
             else lo = mid;
-            if (n >= k && n <= k + k / 4) break;
+            if (n >= k && n <= k + k / 4 + 8) break;
         }
         if (tid == 0) {
             sh.above = value_of(lo);
@@ -321,18 +332,32 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
     }
     __syncthreads();
     float above = sh.above;
-    auto collect = [&] {
-        if (mine > above) {
+    // Each wave counts what it has, takes its places in the list at once and goes through
+    // its registers again; strips in which no lane has any cost three operations.
+    auto hits = [&](float over, auto &&f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (!(fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])) > above)) continue;
+        for (int i = 0; i < NV; ++i) {
+            if (!__any(fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])) > over)) continue;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (e[i][j] > above) {
-                        const int at = atomicAdd(&sh.n, 1);
-                        if (at < kList) sh.list[at] = entry_of(e[i][j], first + 4 * (tid + NT * i) + j);
-                    }
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t hit = __ballot(e[i][j] > over);
+                if (hit != 0) f(hit, e[i][j], 4 * (tid + NT * i) + j);
             }
+        }
+    };
+    auto collect = [&] {
+        float over = above;
+        int count = 0, at = 0;
+        hits(over, [&](uint64_t hit, float, int) { count += __popcll(hit); });
+        if (count > 0) {
+            if (lane == 0) at = atomicAdd(&sh.n, count);
+            at = __builtin_amdgcn_readfirstlane(at);
+            asm volatile("" : "+v"(over));  // (compared again: the masks kept would not fit the scalar registers)
+            hits(over, [&](uint64_t hit, float z, int col) {
+                const int to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+                if (z > over && to < kList) sh.list[to] = entry_of(z, col);
+                at += __popcll(hit);
+            });
         }
         __syncthreads();
     };
@@ -390,19 +415,34 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (hit[j] >> lane & 1) {
-                    if (before < k) sh.list[before] = entry_of(x[j], first + c0 + j);
+                    if (before < k) sh.list[before] = entry_of(x[j], c0 + j);
                     ++before;
                 }
         }
         __syncthreads();
         n = k;
     }
-    for (int i = tid; i < n; i += NT) {
-        const uint64_t me = sh.list[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.list[j] > me ? 1 : 0;
-        if (rank < k) place(rank, me);
-    }
+    // (zeros, below every entry, to a whole number of reads)
+    if (tid < 16) sh.list[n + tid] = 0.0;
+    __syncthreads();
+    auto ranks = [&](auto lanes) __attribute__((always_inline)) {
+        constexpr int L = decltype(lanes)::value;  // to an entry, each with its share of the others
+        for (int i = tid / L; i < n; i += NT / L) {
+            const double me = sh.list[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 2 * (tid % L); j < n; j += 2 * L) {
+                const double2 x = *reinterpret_cast<const double2 *>(&sh.list[j]);
+                rank += x.x > me ? 1 : 0;
+                rank += x.y > me ? 1 : 0;
+            }
+#pragma unroll
+            for (int off = 1; off < L; off <<= 1) rank += __shfl_xor(rank, off, 64);
+            if (tid % L == 0 && rank < k) place(rank, row_entry(me, first));
+        }
+    };
+    if (n <= NT / 4) ranks(std::integral_constant<int, 4>());
+    else ranks(std::integral_constant<int, 1>());
 }
 
 __device__ __forceinline__ void score_left_out(const ScoreArgs &p, int64_t row, int threads) {
@@ -468,20 +508,22 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
 
 // The parts of a row together: their sums, and of their lists the k that come first, each
 // entry's place the number of larger ones in its own list and, by halving, in the others.
-constexpr int kJoinEntries = 4096;
+constexpr int kJoinEntries = 3072;
 __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     __shared__ RowSums all;
-    __shared__ uint64_t held[kJoinEntries];
+    __shared__ uint64_t held[kJoinEntries], some[kJoinEntries];
+    __shared__ int32_t count;
     const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, k = p.k, entries = p.parts * k;
+    const int tid = threadIdx.x, k = p.k, parts = p.parts, entries = parts * k;
     const int32_t t = p.targets ? p.targets[row] : 0;
     if (p.targets && t == p.ignore) return score_left_out(p, row, 256);
-    const uint64_t *best = p.best + row * p.parts * k;
-    const bool in_lds = entries <= kJoinEntries;
+    const uint64_t *best = p.best + row * entries;
+    const bool in_lds = entries <= kJoinEntries && parts <= 256;
     if (in_lds)
         for (int i = tid; i < entries; i += 256) held[i] = best[i];
+    if (tid == 0) count = 0;
     if (tid < 64) {
-        const RowSums s = wave_join<KIND_SCORES>(p.sums + row * p.parts, p.parts, kLog2e);
+        const RowSums s = wave_join<KIND_SCORES>(p.sums + row * parts, parts, kLog2e);
         if (tid == 0) all = s;
     }
     __syncthreads();
@@ -489,32 +531,51 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     const float a = rest_of(s), rest = log1pf(a);
     if (tid == 0 && p.logprobs) p.logprobs[row] = (p.logits[row * p.vocab + t] - s.m) - rest;
     if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
+    if (k == 0) return;
     // (a part of fewer columns has a shorter list)
-    const int last = (int)min((int64_t)k, p.vocab - (int64_t)(p.parts - 1) * p.part), full = (int)min((int64_t)k, p.part);
-    auto place = [&](const uint64_t *lists) __attribute__((always_inline)) {
+    const int last = (int)min((int64_t)k, p.vocab - (int64_t)(parts - 1) * p.part), full = (int)min((int64_t)k, p.part);
+    auto length = [&](int q) { return q == parts - 1 ? last : full; };
+    auto larger = [](const uint64_t *list, int n, uint64_t than) {
+        int lo = 0;
+        while (lo < n) {
+            const int mid = (lo + n) / 2;
+            if (list[mid] > than) lo = mid + 1;
+            else n = mid;
+        }
+        return lo;
+    };
+    auto place = [&](int rank, uint64_t entry) {
+        p.top_ids[row * k + rank] = (int32_t) ~(uint32_t)entry;
+        p.top_logprobs[row * k + rank] = (value_of((uint32_t)(entry >> 32)) - s.m) - rest;
+    };
+    if (!in_lds) {
+        // Lists beyond LDS: each entry finds its place by halving every other list.
         for (int i = tid; i < entries; i += 256) {
             const int q = i / k;
             int rank = i - q * k;
-            if (rank >= (q == p.parts - 1 ? last : full)) continue;
-            const uint64_t me = lists[i];
-            for (int o = 0; o < p.parts && rank < k; ++o) {
-                if (o == q) continue;
-                const uint64_t *list = lists + (int64_t)o * k;
-                int lo = 0, hi = o == p.parts - 1 ? last : full;  // larger ones: lo at least, hi at most
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (list[mid] > me) lo = mid + 1;
-                    else hi = mid;
-                }
-                rank += lo;
-            }
-            if (rank >= k) continue;
-            p.top_ids[row * k + rank] = (int32_t) ~(uint32_t)me;
-            p.top_logprobs[row * k + rank] = (value_of((uint32_t)(me >> 32)) - s.m) - rest;
+            if (rank >= length(q)) continue;
+            const uint64_t me = best[i];
+            for (int o = 0; o < parts && rank < k; ++o)
+                if (o != q) rank += larger(best + (int64_t)o * k, length(o), me);
+            if (rank < k) place(rank, me);
         }
-    };
-    if (in_lds) place(held);
-    else place(best);
+        return;
+    }
+    // With r of each of the whole parts' entries at or above `least` there are k of them:
+    // only those (some dozens more than k as a rule) are compared with each other.
+    const int r = (k + parts - 2) / (parts - 1);
+    uint64_t least = ~0ull;
+    for (int q = 0; q < parts - 1; ++q) least = min(least, held[q * k + r - 1]);
+    for (int i = tid; i < entries; i += 256)
+        if (i % k < length(i / k) && held[i] >= least) some[atomicAdd(&count, 1)] = held[i];
+    __syncthreads();
+    const int n = count;
+    for (int i = tid; i < n; i += 256) {
+        const uint64_t me = some[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += some[j] > me ? 1 : 0;
+        if (rank < k) place(rank, me);
+    }
 }
 
 // Columns of a part at most, and the bytes that the parts' lists may take.
@@ -548,8 +609,9 @@ void scores(Context &cx, const ScoreArgs &all, int64_t n) {
             launch_scores<false>(cx, rows_from(all, at), dim3((unsigned)std::min(kMaxRows, n - at)), v);
         return;
     }
-    // parts for two workgroups per CU, of 4096 columns at least
-    const int64_t want = std::max((v + kScoreCols - 1) / kScoreCols, std::min((v + 4095) / 4096, 2 * cx.cu_count / n));
+    // parts for two workgroups per CU, of 4096 columns at least, whose lists fit the join's LDS
+    const int64_t fit = std::min<int64_t>(256, kJoinEntries / std::max(1, all.k));
+    const int64_t want = std::max((v + kScoreCols - 1) / kScoreCols, std::min({(v + 4095) / 4096, 2 * cx.cu_count / n, fit}));
     const int64_t part = ((v + want - 1) / want + 3) / 4 * 4, parts = (v + part - 1) / part;
     const int64_t row_bytes = parts * ((int64_t)sizeof(RowSums) + 8 * all.k);
     const int64_t block = std::min({n, std::max<int64_t>(1, kScoreBytes / row_bytes), std::max<int64_t>(1, (int64_t(1) << 22) / parts), int64_t(65535)});
