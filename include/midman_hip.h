@@ -568,8 +568,8 @@ int32_t mmh_rotary_tables(mmh_handle ctx, int64_t width, int64_t positions, floa
  * hd) rotated, (x0 c - x1 s, x1 c + x0 s), each product and sum rounded, and the other
  * columns as they are. positions_host [b, t]: the row of the tables (of `table` rows)
  * for each token, MMH_ERR_INDEX and nothing runs where it has none; NULL: 0..t-1.
- * f32, contiguous at any 4-byte alignment. q_out may be q and k_out k; other overlaps
- * are MMH_ERR_ARGUMENT. */
+ * f32, contiguous at any 4-byte alignment; up to 32767 heads each, b * t below 2^31.
+ * q_out may be q and k_out k; other overlaps are MMH_ERR_ARGUMENT. */
 int32_t mmh_rotary(mmh_handle ctx, int32_t layout, const float *q, const float *k,
                    const int32_t *positions_host, int64_t b, int64_t h, int64_t hkv, int64_t t,
                    int64_t hd, int64_t width, int64_t table, const float *cos_dev,

@@ -9,6 +9,8 @@
 #include <cmath>
 
 #include "mmh_args.h"
+#include "mmh_elementwise.h"
+#include "mmh_ids.h"
 #include "mmh_internal.h"
 
 namespace mmh {
@@ -34,47 +36,107 @@ __device__ double frequency(const RotaryTable &p, int64_t i) {
     return w;
 }
 
-__global__ __launch_bounds__(256) void rotary_tables_kernel(RotaryTable p, float *cos_t, float *sin_t) {
-    const int64_t half = p.width / 2, n = p.positions * half;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
-        double s, c;
-        sincos((double)(at / half) * frequency(p, at % half), &s, &c);
-        cos_t[at] = (float)(c * p.amplitude);
-        sin_t[at] = (float)(s * p.amplitude);
+// Lanes of a row of n units: a power of two, 256 at most.
+int lane_bits(int64_t n) {
+    int bits = 0;
+    while (bits < 8 && (int64_t(1) << bits) < n) ++bits;
+    return bits;
+}
+
+// A thread has a pair's column: its frequency is formed once, for `rows` positions.
+__global__ __launch_bounds__(256) void rotary_tables_kernel(RotaryTable p, int bits, int rows, float *cos_t, float *sin_t) {
+    const int64_t half = p.width / 2, step = 256 >> bits;
+    const int64_t first = (int64_t)blockIdx.x * rows * step + (threadIdx.x >> bits);
+    for (int64_t i = threadIdx.x & ((1 << bits) - 1); i < half; i += int64_t(1) << bits) {
+        const double w = frequency(p, i);
+        for (int r = 0; r < rows; ++r) {
+            const int64_t pos = first + r * step;
+            if (pos >= p.positions) break;
+            double s, c;
+            sincos((double)pos * w, &s, &c);
+            cos_t[pos * half + i] = (float)(c * p.amplitude);
+            sin_t[pos * half + i] = (float)(s * p.amplitude);
+        }
     }
 }
 
 struct RotaryArgs {
     const float *q, *k, *cos_t, *sin_t;
     float *q_out, *k_out;
-    const int32_t *positions;  // device [b, t], or null: 0 .. t-1
-    int64_t b, h, hkv, t, hd, width;
-    int interleaved;
+    HostIds positions;
+    int64_t hd, half, first;
+    int32_t places, t, h, heads;  // places: b * t, from `first` on; heads: those of q (h) and k
+    int32_t units, rotated;       // four columns (or pairs of columns) each; the others are copied
     float sign;
 };
 
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
-    const int64_t half = p.width / 2, units = half + p.hd - p.width;
-    const int64_t rows_q = p.q ? p.b * p.h * p.t : 0, rows_k = p.k ? p.b * p.hkv * p.t : 0;
-    const int64_t n = (rows_q + rows_k) * units;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
-        int64_t row = at / units;
-        const int64_t u = at - row * units;
-        const bool is_k = row >= rows_q;
-        if (is_k) row -= rows_q;
-        const float *x = (is_k ? p.k : p.q) + row * p.hd;
-        float *out = (is_k ? p.k_out : p.q_out) + row * p.hd;
-        if (u >= half) {
-            out[u + half] = x[u + half];
-            continue;
+// A unit of four pairs (half layout), of two (interleaved) or of four columns that are
+// copied, up to `count` columns of each of its float4s. H heads of one place at a
+// time: the table's row and the loads of all of them go out together.
+template <int H, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p, int bits) {
+    const int64_t place = p.first + (int64_t)blockIdx.x * (256 >> bits) + (threadIdx.x >> bits);
+    if (place >= p.places) return;
+    const uint32_t b = (uint32_t)place / (uint32_t)p.t, t = (uint32_t)place - b * (uint32_t)p.t;
+    const int64_t row = p.positions.given ? p.positions.at(place) : (int64_t)t;
+    const int head0 = blockIdx.y * H;
+    const int64_t hkv = p.heads - p.h;
+    for (int u = threadIdx.x & ((1 << bits) - 1); u < p.units; u += 1 << bits) {
+        const bool turn = u < p.rotated;
+        // the unit's first column, and that of the pairs' other halves
+        const int64_t width = 2 * p.half, c0 = turn ? 4 * (int64_t)u : width + 4 * (int64_t)(u - p.rotated), c1 = c0 + p.half;
+        const int count = (int)min((int64_t)4, (turn ? (INTERLEAVED ? width : p.half) : p.hd) - c0);
+        const bool both = turn && !INTERLEAVED;
+        float c[4] = {}, s[4] = {}, x[H][4], y[H][4];
+        if (turn) {
+            const int64_t at = row * p.half + (INTERLEAVED ? 2 : 4) * (int64_t)u;
+            load4(p.cos_t + at, INTERLEAVED ? count / 2 : count, c);
+            load4(p.sin_t + at, INTERLEAVED ? count / 2 : count, s);
         }
-        const int64_t t = row % p.t, b = row / (p.t * (is_k ? p.hkv : p.h));
-        const int64_t at_row = (p.positions ? p.positions[b * p.t + t] : t) * half + u;
-        const float c = p.cos_t[at_row], s = p.sin_t[at_row] * p.sign;
-        const int64_t i0 = p.interleaved ? 2 * u : u, i1 = p.interleaved ? i0 + 1 : u + half;
-        const float x0 = x[i0], x1 = x[i1];
-        out[i0] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
-        out[i1] = __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, s));
+        auto at_head = [&](int i, const float *&src, float *&dst) {
+            const int64_t j = head0 + i;
+            const bool is_k = j >= p.h;
+            const int64_t at = ((is_k ? b * hkv + (j - p.h) : (int64_t)b * p.h + j) * p.t + t) * p.hd;
+            src = (is_k ? p.k : p.q) + at;
+            dst = (is_k ? p.k_out : p.q_out) + at;
+        };
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if (head0 + i >= p.heads) break;
+            const float *src;
+            float *dst;
+            at_head(i, src, dst);
+            load4(src + c0, count, x[i]);
+            if (both) load4(src + c1, count, y[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if (head0 + i >= p.heads) break;
+            const float *src;
+            float *dst;
+            at_head(i, src, dst);
+            float o[4], o1[4];
+            if (INTERLEAVED && turn) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float sj = s[j] * p.sign, a = x[i][2 * j], d = x[i][2 * j + 1];
+                    o[2 * j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(d, sj));
+                    o[2 * j + 1] = __fadd_rn(__fmul_rn(d, c[j]), __fmul_rn(a, sj));
+                }
+            } else if (both) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float sj = s[j] * p.sign;
+                    o[j] = __fsub_rn(__fmul_rn(x[i][j], c[j]), __fmul_rn(y[i][j], sj));
+                    o1[j] = __fadd_rn(__fmul_rn(y[i][j], c[j]), __fmul_rn(x[i][j], sj));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = x[i][j];
+            }
+            store4(dst + c0, count, o);
+            if (both) store4(dst + c1, count, o1);
+        }
     }
 }
 
@@ -91,12 +153,14 @@ int32_t rotate(mmh_handle ctx, int32_t layout, const float *q, const float *k, c
     bounded(b, "batch");
     bounded(t, "time");
     bounded(hd, "head_dim");
-    if (q) bounded(h, "n_heads");
-    if (k) bounded(hkv, "n_kv_heads");
+    if (q) positive(h, "n_heads");
+    if (k) positive(hkv, "n_kv_heads");
+    if ((q ? h : 0) > 32767 || (k ? hkv : 0) > 32767) fail(MMH_ERR_SHAPE, "rotary: at most 32767 heads");
     bounded(table, "table");
     if (width < 2 || (width & 1) || width > hd)
         fail(MMH_ERR_SHAPE, "rotary: width must be even and 2 to " + std::to_string(hd) + ", got " + std::to_string(width));
     const int64_t places = extent(b, t, "positions");
+    bounded(places, "positions");
     const int64_t nq = q ? extent(extent(places, h, "q"), hd, "q") : 0, nk = k ? extent(extent(places, hkv, "k"), hd, "k") : 0;
     if (!positions && t > table)
         fail(MMH_ERR_SHAPE, "rotary: " + std::to_string(t) + " positions but tables of " + std::to_string(table));
@@ -109,11 +173,42 @@ int32_t rotate(mmh_handle ctx, int32_t layout, const float *q, const float *k, c
     apart(oq, {sk, ok, sc, ss});
     apart(ok, {sq, sc, ss});
     Context &cx = context(ctx);
-    RotaryArgs p{q, k, cos_dev, sin_dev, q_out, k_out, nullptr, b, h, hkv, t, hd, width, layout == MMH_ROTARY_INTERLEAVED, sign};
-    if (positions) p.positions = cx.stage_ids(positions, places, 0);
-    const int64_t n = (nq + nk) / hd * (hd - width / 2);
-    hipLaunchKernelGGL(rotary_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 65536)), dim3(256), 0, cx.stream, p);
-    check_hip(hipGetLastError(), "rotary launch");
+    const bool inter = layout == MMH_ROTARY_INTERLEAVED;
+    RotaryArgs p;
+    p.q = q;
+    p.k = k;
+    p.cos_t = cos_dev;
+    p.sin_t = sin_dev;
+    p.q_out = q_out;
+    p.k_out = k_out;
+    p.positions = host_ids(cx, positions, places, 0);
+    p.hd = hd;
+    p.half = width / 2;
+    p.places = (int32_t)places;
+    p.t = (int32_t)t;
+    p.h = q ? (int32_t)h : 0;
+    const int64_t heads = p.h + (k ? hkv : 0);
+    p.heads = (int32_t)heads;
+    p.rotated = (int32_t)(((inter ? width : width / 2) + 3) / 4);
+    p.units = p.rotated + (int32_t)((hd - width + 3) / 4);
+    p.sign = sign;
+    const int bits = lane_bits(p.units);
+    const int64_t blocks = (places + (256 >> bits) - 1) / (256 >> bits);
+    auto launch = [&](auto kernel, int64_t group) {
+        constexpr int64_t most = int64_t(1) << 23;  // (a launch has less than 2^32 threads)
+        for (int64_t at = 0; at < blocks; at += most) {
+            p.first = at * (256 >> bits);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(most, blocks - at), (unsigned)((heads + group - 1) / group)), dim3(256),
+                               0, cx.stream, p, bits);
+            check_hip(hipGetLastError(), "rotary launch");
+        }
+    };
+    // four heads of a place in a thread, where that leaves four workgroups for each CU
+    const bool four = blocks * ((heads + 3) / 4) >= 4 * cx.cu_count;
+    if (four && inter) launch(rotary_kernel<4, true>, 4);
+    else if (four) launch(rotary_kernel<4, false>, 4);
+    else if (inter) launch(rotary_kernel<1, true>, 1);
+    else launch(rotary_kernel<1, false>, 1);
     return MMH_OK;
 }
 
@@ -150,8 +245,11 @@ int32_t mmh_rotary_tables(mmh_handle ctx, int64_t width, int64_t positions, floa
         apart({cos_dev, n, "cos"}, {{sin_dev, n, "sin"}});
         Context &cx = context(ctx);
         const RotaryTable p{width, positions, theta, factor, (double)trained, low, high, amplitude, scaling};
-        hipLaunchKernelGGL(rotary_tables_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 65536)), dim3(256),
-                           0, cx.stream, p, cos_dev, sin_dev);
+        const int bits = lane_bits(width / 2);
+        // positions of a thread: 16, or as many as leave four workgroups for each CU
+        const int64_t step = 256 >> bits, rows = std::max<int64_t>(1, std::min<int64_t>(16, positions / (step * 4 * cx.cu_count)));
+        hipLaunchKernelGGL(rotary_tables_kernel, dim3((unsigned)((positions + rows * step - 1) / (rows * step))), dim3(256), 0,
+                           cx.stream, p, bits, (int)rows, cos_dev, sin_dev);
         check_hip(hipGetLastError(), "rotary tables launch");
         return MMH_OK;
     });

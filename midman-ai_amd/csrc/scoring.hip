@@ -17,6 +17,7 @@
 
 #include "mmh_args.h"
 #include "mmh_elementwise.h"
+#include "mmh_ids.h"
 #include "mmh_internal.h"
 #include "mmh_loss.h"
 
@@ -238,7 +239,7 @@ __device__ __forceinline__ float ranked(float z) { return z != z ? INFINITY : z;
 // number of larger ones.
 struct ScoreArgs {
     const float *logits;
-    const int32_t *targets;  // device, or null
+    HostIds targets;
     int64_t vocab;
     int32_t ignore;
     int k;
@@ -462,8 +463,8 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
     const int64_t row = PARTS ? blockIdx.y : blockIdx.x, at = PARTS ? (int64_t)blockIdx.x * p.part : 0;
     const float *z = p.logits + row * p.vocab;
     const int tid = threadIdx.x, cols = (int)(PARTS ? min(p.part, p.vocab - at) : p.vocab);
-    const int32_t t = p.targets ? p.targets[row] : 0;
-    if (p.targets && t == p.ignore) {
+    const int32_t t = p.targets.given ? p.targets.at(row) : 0;
+    if (p.targets.given && t == p.ignore) {
         if (!PARTS) score_left_out(p, row, NT);
         return;
     }
@@ -515,8 +516,8 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     __shared__ int32_t count;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, k = p.k, parts = p.parts, entries = parts * k;
-    const int32_t t = p.targets ? p.targets[row] : 0;
-    if (p.targets && t == p.ignore) return score_left_out(p, row, 256);
+    const int32_t t = p.targets.given ? p.targets.at(row) : 0;
+    if (p.targets.given && t == p.ignore) return score_left_out(p, row, 256);
     const uint64_t *best = p.best + row * entries;
     const bool in_lds = entries <= kJoinEntries && parts <= 256;
     if (in_lds)
@@ -594,7 +595,7 @@ void launch_scores(Context &cx, const ScoreArgs &p, dim3 grid, int64_t cols) {
 
 ScoreArgs rows_from(ScoreArgs p, int64_t row) {
     p.logits += row * p.vocab;
-    if (p.targets) p.targets += row;
+    p.targets.skip(row);
     if (p.logprobs) p.logprobs += row;
     if (p.entropy) p.entropy += row;
     if (p.top_ids) p.top_ids += row * p.k;
@@ -635,7 +636,7 @@ void scores(Context &cx, const ScoreArgs &all, int64_t n) {
 // teacher's slots and the target.
 struct RowArgs {
     const float *logits;
-    const int32_t *targets;  // or null
+    HostIds targets;
     int64_t vocab;
     int32_t ignore;
     float *out;              // dlogits, which may be the logits; null: the loss alone
@@ -820,8 +821,8 @@ __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     const int k = KIND == KIND_SCORES ? 0 : p.k;
     Slots<NT> slots;
     slots.load(p, row, k);
-    const int32_t t = p.targets ? p.targets[row] : -1;
-    if (p.targets && t == p.ignore) return left_out<NT>(p, row, 0, v);
+    const int32_t t = p.targets.given ? p.targets.at(row) : -1;
+    if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, 0, v);
     slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
     float e[NV][4];
     RowSums s = no_sums();
@@ -859,8 +860,8 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     const int k = KIND == KIND_SCORES ? 0 : p.k;
     Slots<NT> slots;
     slots.load(p, row, k);
-    const int32_t t = p.targets ? p.targets[row] : -1;
-    if (p.targets && t == p.ignore) return left_out<NT>(p, row, 0, v);
+    const int32_t t = p.targets.given ? p.targets.at(row) : -1;
+    if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, 0, v);
     slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
     slots.store(k, sh);
     const float kx = p.rate * kLog2e;
@@ -929,8 +930,8 @@ template <int NT, int NV, int KIND>
 __global__ __launch_bounds__(NT, 4) void parts_kernel(RowArgs p) {
     __shared__ RowSums parts[NT / 64];
     const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * p.part, v = p.vocab;
-    const int32_t t = p.targets ? p.targets[row] : -1;
-    if (p.targets && t == p.ignore) return;
+    const int32_t t = p.targets.given ? p.targets.at(row) : -1;
+    if (p.targets.given && t == p.ignore) return;
     const float *z = p.logits + row * v;
     const int cols = (int)min(p.part, v - at), k = KIND == KIND_SCORES ? 0 : p.k;
     for (int j = threadIdx.x; j <= k; j += NT) {
@@ -952,8 +953,8 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     __shared__ RowShared sh;
     const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * p.part, v = p.vocab;
     const int cols = (int)min(p.part, v - at);
-    const int32_t t = p.targets ? p.targets[row] : -1;
-    if (p.targets && t == p.ignore) return left_out<NT>(p, row, at, cols);
+    const int32_t t = p.targets.given ? p.targets.at(row) : -1;
+    if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, at, cols);
     const float *z = p.logits + row * v;
     const int k = KIND == KIND_SCORES ? 0 : p.k, tid = threadIdx.x;
     const float kx = p.rate * kLog2e;
@@ -989,7 +990,7 @@ constexpr int64_t kPartRows = 4096;
 // n rows from `row` on.
 RowArgs rows_from(RowArgs p, int64_t row) {
     p.logits += row * p.vocab;
-    if (p.targets) p.targets += row;
+    p.targets.skip(row);
     if (p.out) p.out += row * p.vocab;
     if (p.dlogprobs) p.dlogprobs += row;
     if (p.dentropy) p.dentropy += row;
@@ -1111,10 +1112,15 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
     p.wrong = pinned;
     *pinned = 0;
     float *rows = reinterpret_cast<float *>(pinned + 16);
-    int32_t *targets = pinned + 16 + d.n;
-    if (d.targets) std::copy(d.targets, d.targets + d.n, targets);
+    if (d.targets && d.n <= HostIds::kHere) {
+        p.targets = host_ids(cx, d.targets, d.n, 1);
+    } else if (d.targets) {
+        // (the call waits: its kernels read them where they are)
+        p.targets.given = 1;
+        p.targets.ids = pinned + 16 + d.n;
+        std::copy(d.targets, d.targets + d.n, pinned + 16 + d.n);
+    }
     p.logits = d.logits;
-    p.targets = d.targets ? targets : nullptr;
     p.ids = d.ids;
     p.teacher = d.teacher;
     p.row_loss = rows;
@@ -1159,10 +1165,9 @@ int32_t mmh_token_logprobs(mmh_handle ctx, const float *logits, const int32_t *t
         apart(st, {sz});
         Context &cx = context(ctx);
         if (!logprobs && !entropy && k == 0) return MMH_OK;
-        const int32_t *targets = targets_host ? cx.stage_ids(targets_host, n, 1) : nullptr;
         ScoreArgs p{};
         p.logits = logits;
-        p.targets = targets;
+        p.targets = host_ids(cx, targets_host, n, 1);
         p.vocab = vocab;
         p.ignore = ignore;
         p.k = (int)k;
@@ -1187,10 +1192,9 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits, const i
         apart_or_same(sd, {sz});
         apart(sd, {sl, se});
         Context &cx = context(ctx);
-        const int32_t *targets = targets_host ? cx.stage_ids(targets_host, n, 1) : nullptr;
         RowArgs p{};
         p.logits = logits;
-        p.targets = targets;
+        p.targets = host_ids(cx, targets_host, n, 1);
         p.vocab = vocab;
         p.ignore = ignore;
         p.dlogprobs = dlogprobs;

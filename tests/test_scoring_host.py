@@ -163,6 +163,8 @@ def test_rotary_refusals():
             refused(r(**{name: 0}), mh.ERR_SHAPE, "must be at least 1")
         for width in (0, 1, 5, 10, -2):
             refused(r(width=width), mh.ERR_SHAPE, "width must be even and 2 to 8")
+        refused(r(h=32768), mh.ERR_SHAPE, "at most 32767 heads")
+        refused(r(b=1 << 16, t=1 << 15, table=1 << 15), mh.ERR_SHAPE, "positions must be below 2^31")
         refused(r(t=6), mh.ERR_SHAPE, "6 positions but tables of 5")
         refused(r(pos=np.array([0, 1, 2, 3, 4, 5], np.int32)), mh.ERR_INDEX, "rotary position 5 is out of range for 5")
         refused(r(pos=np.array([0, 1, 2, 3, -1, 4], np.int32)), mh.ERR_INDEX, "rotary position -1")
