@@ -35,15 +35,38 @@ constexpr float kFar = -200.0f;
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// Over a wave, in every lane: within 16 lanes by DPP, then by halves. (Shuffles through
+// LDS take several times as long, and a short row is little else.)
+template <int CTRL>
+__device__ __forceinline__ int32_t dpp(int32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+template <class F>
+__device__ __forceinline__ int32_t wave_fold(int32_t v, F &&f) {
+    v = f(v, dpp<0xb1>(v));   // lane ^ 1
+    v = f(v, dpp<0x4e>(v));   // lane ^ 2
+    v = f(v, dpp<0x141>(v));  // mirrored within 8 lanes
+    v = f(v, dpp<0x140>(v));  // and within 16
+    auto c = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = f((int32_t)c[0], (int32_t)c[1]);
+    c = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    return f((int32_t)c[0], (int32_t)c[1]);
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+    return __int_as_float(wave_fold(__float_as_int(v), [](int32_t a, int32_t b) {
+        return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+    }));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    return __int_as_float(wave_fold(__float_as_int(v), [](int32_t a, int32_t b) {
+        return __float_as_int(__int_as_float(a) + __int_as_float(b));
+    }));
+}
+__device__ __forceinline__ int wave_sum(int v) {
+    return wave_fold(v, [](int32_t a, int32_t b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    return (uint32_t)wave_fold((int32_t)v, [](int32_t a, int32_t b) { return (int32_t)max((uint32_t)a, (uint32_t)b); });
 }
 
 // ---- a stretch of a row in registers ------------------------------------------
@@ -283,8 +306,7 @@ __device__ __forceinline__ int count_above(const float (&e)[NV][4], float t, Top
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) n += e[i][j] > t ? 1 : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+    n = wave_sum(n);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = n;
     __syncthreads();
@@ -314,9 +336,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
             m[i] = sh.maxima[lane + 64 * i];
             hi = max(hi, m[i]);
         }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, off, 64));
-        hi += 1;  // (lo is reached by k maxima or is the lowest, hi by none)
+        hi = wave_max(hi) + 1;  // (lo is reached by k maxima or is the lowest, hi by none)
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
             int n = 0;
@@ -1044,8 +1064,9 @@ void launch_parts(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
     }
 }
 
-// Rows in one workgroup's registers each, whole. Wider ones take a workgroup that fills a CU
-// and reads them twice; those past the last round of one for every CU go by parts.
+// Rows by a workgroup each. A few wide ones, a quarter of the CUs at most, by their parts:
+// 64 rows of 131071 26 -> 19 us for log probabilities' gradients, one 21 -> 12, but 128 rows
+// 29 -> 34; rows of up to kRowCols never (one of 32000 9 -> 12).
 // targets_host: of the n rows, where some may be left out.
 template <int KIND>
 void launch_rows(Context &cx, RowArgs p, int64_t n, const int32_t *targets_host) {
@@ -1053,11 +1074,8 @@ void launch_rows(Context &cx, RowArgs p, int64_t n, const int32_t *targets_host)
     if (p.vocab <= kRowCols) return launch_whole<KIND>(cx, p, 0, n);
     int64_t kept = n;
     if (targets_host) kept -= std::count(targets_host, targets_host + n, p.ignore);
-    int64_t rest = kept < 64 ? kept : 0, first = n;
-    for (; rest > 0; --first)
-        if (!targets_host || targets_host[first - 1] != p.ignore) --rest;
-    if (first > 0) launch_whole<KIND>(cx, p, 0, first);
-    if (first < n) launch_parts<KIND>(cx, p, first, n);
+    if (kept <= cx.cu_count / 4) launch_parts<KIND>(cx, p, 0, n);
+    else launch_whole<KIND>(cx, p, 0, n);
 }
 
 void check_logits(const char *what, const float *logits, const int32_t *targets, int64_t n, int64_t vocab,
