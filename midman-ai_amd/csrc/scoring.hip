@@ -70,24 +70,33 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 }
 
 // ---- a stretch of a row in registers ------------------------------------------
-// NT threads hold NV strips of 4 NT columns, thread t of strip i the columns 4 (t +
-// NT i) and three on; what lies past the stretch's `cols` is -inf. Rows begin at any
-// 4-byte address, at which gfx950 moves 16 bytes as well. Loads of whole float4s are
-// unconditional (from the last one past the end), so all of them are in flight at once.
+// Rows begin at any 4-byte address. They are taken as if they began `shift` floats
+// earlier, at a cache line, so that a wave's strips are whole lines (a row of 131071 as it
+// lies: 10% slower than one of 131072); columns below are of that longer row.
+constexpr int kLine = 32;
+__device__ __forceinline__ int line_shift(const float *row) { return (int)(reinterpret_cast<uintptr_t>(row) >> 2 & (kLine - 1)); }
+
+// NT threads hold NV strips of 4 NT columns of a stretch, thread t of strip i the columns
+// 4 (t + NT i) and three on; of the stretch the columns lo .. cols - 1 are the row's (lo
+// below kLine), the others -inf. Loads of whole float4s are unconditional (those that end
+// outside start from within), so all of them are in flight at once.
 template <int NT, int NV>
-__device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e)[NV][4], int tid = threadIdx.x) {
-    if (cols >= 4) {
+__device__ __forceinline__ void load_stretch(const float *z, int lo, int cols, float (&e)[NV][4], int tid = threadIdx.x) {
+    static_assert(4 * NT >= kLine, "lo lies in the first strip");
+    if (cols - lo >= 4) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) __builtin_memcpy(e[i], z + min(4 * (tid + NT * i), cols - 4), 16);
+        for (int i = 0; i < NV; ++i) {
+            const int c = min(4 * (tid + NT * i), cols - 4);
+            __builtin_memcpy(e[i], z + (i == 0 ? max(c, lo) : c), 16);
+        }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (4 * NT * (i + 1) <= cols) continue;
+        if ((i > 0 || lo == 0) && 4 * NT * (i + 1) <= cols) continue;
         const int c = 4 * (tid + NT * i);
-        if (c + 4 <= cols) continue;
-        // (a float4 at the end: its last columns, from the load at cols - 4)
+        if (c >= lo && c + 4 <= cols) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[i][j] = c + j < cols ? z[c + j] : -INFINITY;
+        for (int j = 0; j < 4; ++j) e[i][j] = c + j >= lo && c + j < cols ? z[c + j] : -INFINITY;
     }
 }
 // f of a stretch to `out`, each strip on its way as soon as it is formed. `stream`: past
@@ -95,27 +104,29 @@ __device__ __forceinline__ void load_stretch(const float *z, int cols, float (&e
 // both ways at the stores alone would hold them back until all is formed: 4096 x 32000
 // 227 -> 237 us.)
 template <bool STREAM, int NT, int NV, class F>
-__device__ __forceinline__ void write_strips(float *out, int cols, const float (&e)[NV][4], int tid, F &&f) {
+__device__ __forceinline__ void write_strips(float *out, int lo, int cols, const float (&e)[NV][4], int tid, F &&f) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = 4 * (tid + NT * i);
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = f(e[i][j]);
-        if (c + 4 <= cols) {
+        if ((i > 0 || c >= lo) && c + 4 <= cols) {
             float4u x;
             __builtin_memcpy(&x, v, 16);
             if (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<float4u *>(out + c));
             else *reinterpret_cast<float4u *>(out + c) = x;
         } else {
-            store4(out + c, max(0, cols - c), v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j >= lo && c + j < cols) out[c + j] = v[j];
         }
     }
 }
 template <int NT, int NV, class F>
-__device__ __forceinline__ void write_stretch(float *out, int cols, bool stream, const float (&e)[NV][4], int tid, F &&f) {
-    if (stream) write_strips<true, NT, NV>(out, cols, e, tid, f);
-    else write_strips<false, NT, NV>(out, cols, e, tid, f);
+__device__ __forceinline__ void write_stretch(float *out, int lo, int cols, bool stream, const float (&e)[NV][4], int tid, F &&f) {
+    if (stream) write_strips<true, NT, NV>(out, lo, cols, e, tid, f);
+    else write_strips<false, NT, NV>(out, lo, cols, e, tid, f);
 }
 
 // ---- a row's sums ---------------------------------------------------------------
@@ -270,7 +281,7 @@ struct ScoreArgs {
     int32_t *top_ids;
     float *top_logprobs;
     // rows over several workgroups: what a part leaves
-    int64_t part;         // columns of a part, a multiple of 4
+    int64_t part;         // columns of a part, a multiple of kLine, some hundreds at least
     int parts;
     RowSums *sums;        // [rows, parts]
     uint64_t *best;       // [rows, parts, k], the largest first
@@ -315,13 +326,13 @@ __device__ __forceinline__ int count_above(const float (&e)[NV][4], float t, Top
     return n;
 }
 
-// The k largest of a stretch (no NaN; -inf past its `cols`) to place(rank, entry), by
-// every thread of the workgroup; fewer where it has fewer columns.
+// The k largest of a stretch (no NaN) to place(rank, entry), by every thread of the
+// workgroup; fewer where it has fewer columns. Its column 0 is the row's `first`.
 template <int NT, int NV, class F>
-__device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32_t first, int k, TopShared &sh, F &&place) {
+__device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int cols, uint32_t first, int k, TopShared &sh, F &&place) {
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t lowest = order_of(-INFINITY);
-    k = min(k, cols);
+    k = min(k, max(0, cols - lo_col));
     float mine = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i) mine = fmaxf(mine, fmaxf(fmaxf(e[i][0], e[i][1]), fmaxf(e[i][2], e[i][3])));
@@ -419,7 +430,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int cols, uint32
             uint64_t hit[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                hit[j] = __ballot(x[j] == above && c0 + j < cols);
+                hit[j] = __ballot(x[j] == above && c0 + j >= lo_col && c0 + j < cols);
                 here += __popcll(hit[j]);
             }
             __syncthreads();
@@ -475,14 +486,17 @@ __device__ __forceinline__ void score_left_out(const ScoreArgs &p, int64_t row, 
     }
 }
 
-// A row of up to 4 NT NV columns (PARTS: a part of one) in a workgroup's registers.
+// A row of up to 4 NT NV columns, the shift's among them (PARTS: a part of one), in a
+// workgroup's registers.
 template <int NT, int NV, bool PARTS>
 __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
     __shared__ RowSums lds[NT / 64];
     __shared__ TopShared sh;
     const int64_t row = PARTS ? blockIdx.y : blockIdx.x, at = PARTS ? (int64_t)blockIdx.x * p.part : 0;
     const float *z = p.logits + row * p.vocab;
-    const int tid = threadIdx.x, cols = (int)(PARTS ? min(p.part, p.vocab - at) : p.vocab);
+    const int tid = threadIdx.x, shift = line_shift(z);
+    const int lo = PARTS ? (int)max((int64_t)0, shift - at) : shift;
+    const int cols = (int)(PARTS ? min(p.part, p.vocab + shift - at) : p.vocab + shift);
     const int32_t t = p.targets.given ? p.targets.at(row) : 0;
     if (p.targets.given && t == p.ignore) {
         if (!PARTS) score_left_out(p, row, NT);
@@ -490,7 +504,7 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
     }
     float e[NV][4];
     const float zt = !PARTS && p.logprobs && tid == 0 ? z[t] : 0.0f;
-    load_stretch<NT, NV>(z + at, cols, e);
+    load_stretch<NT, NV>(z + at - shift, lo, cols, e);
     RowSums s = no_sums();
     add_stretch<KIND_SCORES>(s, e, kLog2e);
     s = wave_sums(s);
@@ -517,7 +531,7 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
             for (int j = 0; j < 4; ++j) e[i][j] = e[i][j] != e[i][j] ? INFINITY : e[i][j];
     }
     const float m = s.m;
-    top_of<NT, NV>(e, cols, (uint32_t)at, p.k, sh, [&](int rank, uint64_t entry) {
+    top_of<NT, NV>(e, lo, cols, (uint32_t)(at - shift), p.k, sh, [&](int rank, uint64_t entry) {
         if constexpr (PARTS) {
             p.best[(row * p.parts + blockIdx.x) * p.k + rank] = entry;
         } else {
@@ -553,9 +567,12 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     if (tid == 0 && p.logprobs) p.logprobs[row] = (p.logits[row * p.vocab + t] - s.m) - rest;
     if (tid == 0 && p.entropy) p.entropy[row] = rest - s.u / (1.0f + a);
     if (k == 0) return;
-    // (a part of fewer columns has a shorter list)
-    const int last = (int)min((int64_t)k, p.vocab - (int64_t)(parts - 1) * p.part), full = (int)min((int64_t)k, p.part);
-    auto length = [&](int q) { return q == parts - 1 ? last : full; };
+    // (the first and the last parts may have fewer columns, and a shorter list)
+    const int shift = line_shift(p.logits + row * p.vocab);
+    auto length = [&](int q) {
+        const int64_t cols = min(p.part, p.vocab + shift - q * p.part) - (q == 0 ? shift : 0);
+        return (int)min((int64_t)k, max((int64_t)0, cols));
+    };
     auto larger = [](const uint64_t *list, int n, uint64_t than) {
         int lo = 0;
         while (lo < n) {
@@ -582,8 +599,8 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
         }
         return;
     }
-    // With r of each of the whole parts' entries at or above `least` there are k of them:
-    // only those (some dozens more than k as a rule) are compared with each other.
+    // With r of the entries of each part but the last (which have more columns than entries)
+    // at or above `least` there are k of them: only those (some dozens more than k as a rule) are compared with each other.
     const int r = (k + parts - 2) / (parts - 1);
     uint64_t least = ~0ull;
     for (int q = 0; q < parts - 1; ++q) least = min(least, held[q * k + r - 1]);
@@ -599,6 +616,11 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     }
 }
 
+int64_t round_line(int64_t v) { return (v + kLine - 1) / kLine * kLine; }
+// Columns of an array's rows with their shift, at most.
+int64_t line_cols(const float *rows, int64_t v) {
+    return (reinterpret_cast<uintptr_t>(rows) & (4 * kLine - 1)) == 0 && v % kLine == 0 ? v : v + kLine - 1;
+}
 // Columns of a part at most, and the bytes that the parts' lists may take.
 constexpr int64_t kScoreCols = 32768, kScoreBytes = int64_t(64) << 20;
 
@@ -625,15 +647,16 @@ ScoreArgs rows_from(ScoreArgs p, int64_t row) {
 
 void scores(Context &cx, const ScoreArgs &all, int64_t n) {
     const int64_t v = all.vocab;
-    if (v <= kScoreCols) {
+    const int64_t cols = line_cols(all.logits, v);
+    if (cols <= kScoreCols) {
         for (int64_t at = 0; at < n; at += kMaxRows)
-            launch_scores<false>(cx, rows_from(all, at), dim3((unsigned)std::min(kMaxRows, n - at)), v);
+            launch_scores<false>(cx, rows_from(all, at), dim3((unsigned)std::min(kMaxRows, n - at)), cols);
         return;
     }
     // parts for two workgroups per CU, of 4096 columns at least, whose lists fit the join's LDS
     const int64_t fit = std::min<int64_t>(256, kJoinEntries / std::max(1, all.k));
-    const int64_t want = std::max((v + kScoreCols - 1) / kScoreCols, std::min({(v + 4095) / 4096, 2 * cx.cu_count / n, fit}));
-    const int64_t part = ((v + want - 1) / want + 3) / 4 * 4, parts = (v + part - 1) / part;
+    const int64_t want = std::max((cols + kScoreCols - 1) / kScoreCols, std::min({(v + 4095) / 4096, 2 * cx.cu_count / n, fit}));
+    const int64_t part = round_line((cols + want - 1) / want), parts = (cols + part - 1) / part;
     const int64_t row_bytes = parts * ((int64_t)sizeof(RowSums) + 8 * all.k);
     const int64_t block = std::min({n, std::max<int64_t>(1, kScoreBytes / row_bytes), std::max<int64_t>(1, (int64_t(1) << 22) / parts), int64_t(65535)});
     char *ws = static_cast<char *>(cx.workspace(2, (size_t)(block * row_bytes)));
@@ -671,7 +694,7 @@ struct RowArgs {
     int32_t *wrong;                   // receives 1 for a teacher's id beyond the vocabulary
     bool stream;
     // a row over several workgroups (parts_kernel, parts_grad_kernel)
-    int64_t part;     // columns of a part, a multiple of 4
+    int64_t part;     // columns of a part, a multiple of kLine
     int parts;
     RowSums *sums;    // [rows, parts]
     float *slot_z;    // [rows, k + 1]
@@ -758,14 +781,18 @@ struct Slots {
     }
 };
 
-// A row that is left out. Its part of the output is zeros.
+// A row that is left out. Its columns at .. end - 1 of the output are zeros.
 template <int NT>
-__device__ __forceinline__ void left_out(const RowArgs &p, int64_t row, int64_t at, int64_t cols) {
+__device__ __forceinline__ void left_out(const RowArgs &p, int64_t row, int64_t at, int64_t end) {
     if (p.row_loss && at == 0 && threadIdx.x == 0) p.row_loss[row] = 0.0f;
     if (!p.out) return;
-    float *out = p.out + row * p.vocab + at;
+    float *out = p.out + row * p.vocab;
     const float zero[4] = {};
-    for (int64_t j = 4 * (int64_t)threadIdx.x; j < cols; j += 4 * NT) store4(out + j, (int)min((int64_t)4, cols - j), zero);
+    for (int64_t j = at + 4 * (int64_t)threadIdx.x; j < end; j += 4 * NT) store4(out + j, (int)min((int64_t)4, end - j), zero);
+}
+// The shift of a row that is read, or of the output's that is written.
+__device__ __forceinline__ int row_shift(const RowArgs &p, int64_t row) {
+    return line_shift((p.out ? p.out : p.logits) + row * p.vocab);
 }
 
 // A row's dense gradient exp2((z - m) k) (f0 + f1 (z - m)) (KIND_SCORES; KIND_ONE: f1 =
@@ -813,13 +840,13 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
     return g;
 }
 
-// The few tokens' own values, for columns at .. at + cols - 1, after the dense ones: an
+// The few tokens' own values, for columns at .. end - 1, after the dense ones: an
 // id's first slot takes the shares of all its slots.
 template <int NT, int KIND>
-__device__ __forceinline__ void patch(float *out, int64_t at, int64_t cols, int k, const Dense &g, const RowShared &sh) {
+__device__ __forceinline__ void patch(float *out, int64_t at, int64_t end, int k, const Dense &g, const RowShared &sh) {
     for (int j = threadIdx.x; j <= k; j += NT) {
         const int32_t id = sh.id[j];
-        if (id < at || id >= at + cols) continue;
+        if (id < at || id >= end) continue;
         float w = 0.0f;
         bool first = true;
         for (int i = 0; i <= k; ++i)
@@ -831,7 +858,8 @@ __device__ __forceinline__ void patch(float *out, int64_t at, int64_t cols, int 
     }
 }
 
-// A row of up to 4 NT NV columns in a workgroup's registers: read once.
+// A row of up to 4 NT NV columns, the shift's among them, in a workgroup's registers: read
+// once.
 template <int NT, int NV, int KIND>
 __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     __shared__ RowShared sh;
@@ -846,7 +874,8 @@ __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
     float e[NV][4];
     RowSums s = no_sums();
-    load_stretch<NT, NV>(z, v, e);
+    const int shift = row_shift(p, row);
+    load_stretch<NT, NV>(z - shift, shift, shift + v, e);
     slots.store(k, sh);
     add_stretch<KIND>(s, e, p.rate * kLog2e);
     s = wave_sums(s);
@@ -859,15 +888,15 @@ __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     // (addresses formed anew: kept from the loads they would take the row's registers)
     int me = tid;
     asm volatile("" : "+v"(me));
-    write_stretch<NT, NV>(out, v, p.stream, e, me, [&](float x) { return g.at<KIND>(x); });
+    write_stretch<NT, NV>(out - shift, shift, shift + v, p.stream, e, me, [&](float x) { return g.at<KIND>(x); });
     __syncthreads();
     patch<NT, KIND>(out, 0, v, k, g, sh);
 }
 
 // Wider rows, of 2048 R columns at least: 512 threads have a CU's registers, and hold the
-// row's last R strips there and L before them in LDS (98304 and 32768 columns of f32 with
-// 48 and 16). Only what comes before those is read twice. (`some`, 8 strips at a time, is
-// what passes through.)
+// row's first R strips there and L after them in LDS (98304 and 32768 columns of f32 with
+// 48 and 16). Only what follows those is read twice. (`some`, 8 strips at a time, is what
+// passes through.)
 template <int R, int L, int KIND>
 __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     constexpr int NT = 512, S = 8, kSome = 4 * NT * S;
@@ -886,19 +915,24 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     slots.store(k, sh);
     const float kx = p.rate * kLog2e;
     RowSums s = no_sums();
-    // the row from behind: R strips, L strips, and passes of S before them
-    const int64_t in_lds = v - 4 * NT * R, before = max((int64_t)0, in_lds - 4 * NT * L);
-    const int passes = (int)((before + kSome - 1) / kSome);
+    const int shift = row_shift(p, row);
+    constexpr int64_t kHeld = 4 * NT * R, kKept = kHeld + 4 * NT * L;
+    const int64_t total = v + shift;
+    const int passes = (int)(max((int64_t)0, total - kKept + kSome - 1) / kSome);
+    auto cols_at = [&](int64_t at, int64_t end) { return (int)max((int64_t)0, min((int64_t)kSome, min(total, end) - at)); };
+    z -= shift;
     {
         float some[S][4];
         for (int i = 0; i < passes; ++i) {
-            load_stretch<NT, S>(z + (int64_t)i * kSome, (int)min((int64_t)kSome, before - (int64_t)i * kSome), some);
+            const int64_t at = kKept + (int64_t)i * kSome;
+            load_stretch<NT, S>(z + at, 0, cols_at(at, total), some);
             add_stretch<KIND>(s, some, kx);
         }
 #pragma unroll 1
         for (int i = 0; i < L / S; ++i) {
-            const int64_t at = before + (int64_t)i * kSome;
-            load_stretch<NT, S>(z + at, (int)max((int64_t)0, min((int64_t)kSome, in_lds - at)), some);
+            const int64_t at = kHeld + (int64_t)i * kSome;
+            if (at >= total) break;
+            load_stretch<NT, S>(z + at, 0, cols_at(at, kKept), some);
             add_stretch<KIND>(s, some, kx);
 #pragma unroll
             for (int r = 0; r < S; ++r) __builtin_memcpy(__builtin_assume_aligned(&held[((i * S + r) * NT + tid) * 4], 16), some[r], 16);
@@ -908,8 +942,14 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     float e[R][4];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        __builtin_memcpy(e[r], reinterpret_cast<const char *>(z + in_lds) + 16 * NT * r + lane_at, 16);
+        // (columns below the shift: any of the row's in their place at first)
+        const uint32_t from = r == 0 ? max(lane_at, 4u * (uint32_t)shift) : lane_at;
+        __builtin_memcpy(e[r], reinterpret_cast<const char *>(z) + 16 * NT * r + from, 16);
         __builtin_amdgcn_sched_barrier(0);  // (one address at a time: no registers for more)
+    }
+    if (4 * tid < shift) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[0][j] = 4 * tid + j >= shift ? z[4 * tid + j] : -INFINITY;
     }
     add_stretch<KIND>(s, e, kx);
     s = wave_sums(s);
@@ -918,29 +958,30 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     s = row_sums(join_sums<KIND>(sh.parts, NT / 64, kx));
     const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
     if (!p.out) return;
-    float *out = p.out + row * v;
+    float *out = p.out + row * v - shift;
     // (the addresses from here on are formed anew: kept from the first pass they would
     // take the registers that hold the row)
     int me = tid;
     asm volatile("" : "+v"(me));
     auto turn = [&](float x) { return g.at<KIND>(x); };
-    write_stretch<NT, R>(out + in_lds, 4 * NT * R, p.stream, e, me, turn);
+    write_stretch<NT, R>(out, shift, (int)kHeld, p.stream, e, me, turn);
 #pragma unroll 1
     for (int i = 0; i < L / S; ++i) {
+        const int64_t at = kHeld + (int64_t)i * kSome;
+        if (at >= total) break;
         float some[S][4];
 #pragma unroll
         for (int r = 0; r < S; ++r) __builtin_memcpy(some[r], __builtin_assume_aligned(&held[((i * S + r) * NT + me) * 4], 16), 16);
-        const int64_t at = before + (int64_t)i * kSome;
-        write_stretch<NT, S>(out + at, (int)max((int64_t)0, min((int64_t)kSome, in_lds - at)), p.stream, some, me, turn);
+        write_stretch<NT, S>(out + at, 0, cols_at(at, kKept), p.stream, some, me, turn);
     }
     for (int i = passes - 1; i >= 0; --i) {
         float some[S][4];
-        const int cols = (int)min((int64_t)kSome, before - (int64_t)i * kSome);
-        load_stretch<NT, S>(z + (int64_t)i * kSome, cols, some, me);
-        write_stretch<NT, S>(out + (int64_t)i * kSome, cols, p.stream, some, me, turn);
+        const int64_t at = kKept + (int64_t)i * kSome;
+        load_stretch<NT, S>(z + at, 0, cols_at(at, total), some, me);
+        write_stretch<NT, S>(out + at, 0, cols_at(at, total), p.stream, some, me, turn);
     }
     __syncthreads();
-    patch<NT, KIND>(out, 0, v, k, g, sh);
+    patch<NT, KIND>(out + shift, 0, v, k, g, sh);
 }
 
 // A row over several workgroups, one part of at most 4 NT NV columns each: first the
@@ -953,14 +994,15 @@ __global__ __launch_bounds__(NT, 4) void parts_kernel(RowArgs p) {
     const int32_t t = p.targets.given ? p.targets.at(row) : -1;
     if (p.targets.given && t == p.ignore) return;
     const float *z = p.logits + row * v;
-    const int cols = (int)min(p.part, v - at), k = KIND == KIND_SCORES ? 0 : p.k;
+    const int shift = row_shift(p, row), k = KIND == KIND_SCORES ? 0 : p.k;
+    const int lo = (int)max((int64_t)0, shift - at), cols = (int)min(p.part, v + shift - at);
     for (int j = threadIdx.x; j <= k; j += NT) {
         const int32_t id = j < k ? p.ids[row * k + j] : t;
-        if (id >= at && id < at + cols) p.slot_z[row * (k + 1) + j] = z[id];
+        if (id >= 0 && (int64_t)id + shift >= at && (int64_t)id + shift < at + cols) p.slot_z[row * (k + 1) + j] = z[id];
     }
     float e[NV][4];
     RowSums s = no_sums();
-    load_stretch<NT, NV>(z + at, cols, e);
+    load_stretch<NT, NV>(z + at - shift, lo, cols, e);
     add_stretch<KIND>(s, e, p.rate * kLog2e);
     s = wave_sums(s);
     if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = s;
@@ -972,14 +1014,17 @@ template <int NT, int NV, int KIND>
 __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     __shared__ RowShared sh;
     const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * p.part, v = p.vocab;
-    const int cols = (int)min(p.part, v - at);
+    const int shift = row_shift(p, row);
+    const int lo = (int)max((int64_t)0, shift - at), cols = (int)min(p.part, v + shift - at);
+    // (the row's own columns)
+    const int64_t from = max((int64_t)0, at - shift), end = min(v, at - shift + p.part);
     const int32_t t = p.targets.given ? p.targets.at(row) : -1;
-    if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, at, cols);
+    if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, from, end);
     const float *z = p.logits + row * v;
     const int k = KIND == KIND_SCORES ? 0 : p.k, tid = threadIdx.x;
     const float kx = p.rate * kLog2e;
     float e[NV][4];
-    if (p.out) load_stretch<NT, NV>(z + at, cols, e);
+    if (p.out) load_stretch<NT, NV>(z + at - shift, lo, cols, e);
     Slots<NT> slots;
     slots.load(p, row, k);
     slots.gather(p, k, t, [&](int j, int32_t) { return p.slot_z[row * (k + 1) + j]; });
@@ -993,14 +1038,14 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     const Dense g = coefficients<KIND>(p, row, k, s, blockIdx.x == 0, sh);
     if (!p.out) return;
     float *out = p.out + row * v;
-    write_stretch<NT, NV>(out + at, cols, p.stream, e, tid, [&](float x) { return g.at<KIND>(x); });
+    write_stretch<NT, NV>(out + at - shift, lo, cols, p.stream, e, tid, [&](float x) { return g.at<KIND>(x); });
     __syncthreads();
-    patch<NT, KIND>(out, at, cols, k, g, sh);
+    patch<NT, KIND>(out, from, end, k, g, sh);
 }
 
 // Outputs from this size on pass the caches by (what the GPU's last cache holds).
 constexpr int64_t kStreamBytes = int64_t(256) << 20;
-// Rows of up to kRowCols columns stay in one workgroup's registers.
+// Rows of up to kRowCols columns, the shift's among them, stay in one workgroup's registers.
 constexpr int64_t kRowCols = 32768;
 constexpr int kPartThreads = 256, kPartStrips = 8;
 constexpr int64_t kPartCols = 4 * kPartThreads * kPartStrips;
@@ -1020,42 +1065,47 @@ RowArgs rows_from(RowArgs p, int64_t row) {
     return p;
 }
 
+int64_t row_cols(const RowArgs &p) { return line_cols(p.out ? p.out : p.logits, p.vocab); }
+
 template <int KIND>
-void launch_whole(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
-    for (int64_t at = first; at < end; at += kMaxRows) {
+void launch_whole(Context &cx, const RowArgs &all, int64_t n) {
+    const int64_t cols = row_cols(all);
+    for (int64_t at = 0; at < n; at += kMaxRows) {
         const RowArgs p = rows_from(all, at);
-        const int64_t rows = std::min(kMaxRows, end - at);
+        const int64_t rows = std::min(kMaxRows, n - at);
         auto launch = [&](auto kernel, int threads) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, cx.stream, p);
         };
-        if (p.vocab <= 1024) launch(rows_kernel<256, 1, KIND>, 256);
-        else if (p.vocab <= 4096) launch(rows_kernel<256, 4, KIND>, 256);
-        else if (p.vocab <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
-        else if (p.vocab <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
-        else if (p.vocab <= kRowCols) launch(rows_kernel<512, 16, KIND>, 512);
-        else if (p.vocab <= 65536) launch(wide_rows_kernel<16, 16, KIND>, 512);
-        else if (p.vocab <= 98304) launch(wide_rows_kernel<32, 16, KIND>, 512);
+        // (a row's columns with its shift; the wide kernels take what they do not hold in passes)
+        if (cols <= 1024) launch(rows_kernel<256, 1, KIND>, 256);
+        else if (cols <= 4096) launch(rows_kernel<256, 4, KIND>, 256);
+        else if (cols <= 8192) launch(rows_kernel<512, 4, KIND>, 512);
+        else if (cols <= 16384) launch(rows_kernel<512, 8, KIND>, 512);
+        else if (cols <= kRowCols) launch(rows_kernel<512, 16, KIND>, 512);
+        else if (p.vocab < 32768) launch(wide_rows_kernel<8, 16, KIND>, 512);
+        else if (p.vocab < 65536) launch(wide_rows_kernel<16, 16, KIND>, 512);
+        else if (p.vocab < 98304) launch(wide_rows_kernel<32, 16, KIND>, 512);
         else launch(wide_rows_kernel<48, 16, KIND>, 512);
         check_hip(hipGetLastError(), "rows launch");
     }
 }
 
 template <int KIND>
-void launch_parts(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
-    const int64_t v = all.vocab, n = end - first, slots = KIND == KIND_SCORES ? 1 : all.k + 1;
+void launch_parts(Context &cx, const RowArgs &all, int64_t n) {
+    const int64_t v = all.vocab, cols = row_cols(all), slots = KIND == KIND_SCORES ? 1 : all.k + 1;
     // parts for two workgroups per CU, of 1024 columns at least
-    const int64_t want = std::max((v + kPartCols - 1) / kPartCols, std::min((v + 1023) / 1024, 2 * cx.cu_count / n));
-    const int64_t part = ((v + want - 1) / want + 3) / 4 * 4, parts = (v + part - 1) / part;
+    const int64_t want = std::max((cols + kPartCols - 1) / kPartCols, std::min((v + 1023) / 1024, 2 * cx.cu_count / n));
+    const int64_t part = round_line((cols + want - 1) / want), parts = (cols + part - 1) / part;
     const int64_t block = std::min({n, kPartRows, std::max<int64_t>(1, (int64_t(1) << 23) / parts)});
     const size_t sums = (size_t)(block * parts) * sizeof(RowSums);
     char *ws = static_cast<char *>(cx.workspace(2, sums + (size_t)(block * slots) * 4));
-    for (int64_t at = first; at < end; at += block) {
+    for (int64_t at = 0; at < n; at += block) {
         RowArgs p = rows_from(all, at);
         p.part = part;
         p.parts = (int)parts;
         p.sums = reinterpret_cast<RowSums *>(ws);
         p.slot_z = reinterpret_cast<float *>(ws + sums);
-        const unsigned rows = (unsigned)std::min(block, end - at);
+        const unsigned rows = (unsigned)std::min(block, n - at);
         hipLaunchKernelGGL((parts_kernel<kPartThreads, kPartStrips, KIND>), dim3((unsigned)parts, rows), dim3(kPartThreads), 0, cx.stream, p);
         check_hip(hipGetLastError(), "row parts launch");
         hipLaunchKernelGGL((parts_grad_kernel<kPartThreads, kPartStrips, KIND>), dim3(p.out ? (unsigned)parts : 1u, rows),
@@ -1071,11 +1121,11 @@ void launch_parts(Context &cx, const RowArgs &all, int64_t first, int64_t end) {
 template <int KIND>
 void launch_rows(Context &cx, RowArgs p, int64_t n, const int32_t *targets_host) {
     p.stream = n * p.vocab * 4 >= kStreamBytes;
-    if (p.vocab <= kRowCols) return launch_whole<KIND>(cx, p, 0, n);
+    if (row_cols(p) <= kRowCols) return launch_whole<KIND>(cx, p, n);
     int64_t kept = n;
     if (targets_host) kept -= std::count(targets_host, targets_host + n, p.ignore);
-    if (kept <= cx.cu_count / 4) launch_parts<KIND>(cx, p, 0, n);
-    else launch_whole<KIND>(cx, p, 0, n);
+    if (kept <= cx.cu_count / 4) launch_parts<KIND>(cx, p, n);
+    else launch_whole<KIND>(cx, p, n);
 }
 
 void check_logits(const char *what, const float *logits, const int32_t *targets, int64_t n, int64_t vocab,
