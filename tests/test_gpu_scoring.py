@@ -41,6 +41,11 @@ def ptr(a):
 
 
 def near(got, value, tol, what):
+    with np.errstate(invalid="ignore"):
+        _near(got, value, tol, what)
+
+
+def _near(got, value, tol, what):
     err = np.abs(got.astype(np.float64) - value)
     bad = ~((err <= tol) | (got == value))
     assert not bad.any(), (what, int(bad.sum()), float(np.nanmax(err / np.maximum(tol, 1e-300))), np.argwhere(bad)[:3].tolist())
@@ -98,7 +103,9 @@ def teachers(r, z, k, noise=1.0):
 # (rows, vocab): one row and token, waves and strips that end inside, every width's kernel and its border, more rows than CUs
 SHAPES = [(1, 1), (3, 2), (5, 63), (7, 64), (2, 65), (64, 256), (9, 1000), (4, 1023), (3, 1024), (6, 1025), (17, 4096), (5, 4097),
           (3, 8191), (2, 8193), (3, 16385), (2, 32000), (3, 32768), (2, 32769), (1, 50257), (300, 4099), (520, 9001), (1, 131071),
-          (2, 262144), (5, 65537), (1030, 77), (260, 33000)]
+          (2, 262144), (5, 65537), (1030, 77), (260, 33000),
+          # as many wide rows that a workgroup takes each whole: what its registers and LDS hold, borders of both, more
+          (66, 32750), (70, 49153), (65, 65535), (66, 65600), (65, 98303), (66, 98400), (65, 131100), (65, 140001)]
 
 
 @pytest.mark.parametrize("i", range(len(SHAPES)))
@@ -393,6 +400,47 @@ def test_offsets_past_32_bits(ctx):
     near(tail[1:], want, g_tol, "dlogits")
     assert (tail[0] == 0).all()
     free.free()
+
+
+def test_more_rows_than_a_launch(ctx):
+    n, v = 2 ** 21 + 5, 3
+    z, y, r = drawn(n, v, 15)
+    lp, h, ids, top = run_logprobs(ctx, z, y, 2)
+    want_lp, want_h, (want_ids, want_top) = R.token_logprobs(z, y, 2)
+    near(lp, *want_lp, "logprobs")
+    near(h, *want_h, "entropy")
+    assert np.array_equal(ids, want_ids)
+    dl = r.standard_normal(n).astype(np.float32)
+    near(run_logprobs_bwd(ctx, z, y, dl, None), *R.token_logprobs_backward(z, y, dl, None), "dlogits")
+    row, tol, want, g_tol = R.distillation(z, y, want_ids, z[:, :2].copy(), 2.0, 0.5, n)
+    loss, g = run_distill(ctx, z, y, want_ids, z[:, :2].copy(), 2.0, 0.5)
+    near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
+    near(g, want, g_tol, "dlogits")
+
+
+@pytest.mark.parametrize("shift", [0, 5, 31])
+@pytest.mark.parametrize("v", [994, 1000, 1024, 32736, 32768, 98304])
+def test_rows_at_every_place_of_a_line(ctx, v, shift):
+    # rows and outputs that begin at other places of a cache line, lengths at the kernels' borders
+    n = 70 if v > 32000 else 9
+    z, y, r = drawn(n, v, v + shift)
+    lp, h, ids, top = run_logprobs(ctx, z, y, 17, shift=shift)
+    want_lp, want_h, (want_ids, want_top) = R.token_logprobs(z, y, 17)
+    near(lp, *want_lp, "logprobs")
+    near(h, *want_h, "entropy")
+    assert np.array_equal(ids, want_ids)
+    t_ids, teacher = teachers(r, z, 11)
+    row, tol, want, g_tol = R.distillation(z, y, t_ids, teacher, 2.0, 0.5, n)
+    for inplace in (False, True):
+        loss, g = run_distill(ctx, z, y, t_ids, teacher, 2.0, 0.5, shift=shift, inplace=inplace)
+        near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
+        near(g, want, g_tol, "dlogits")
+    # the output elsewhere in its line than the logits
+    Z, out = Box(ctx, z, shift), empty(ctx, (n, v), (shift + 3) % 32)
+    dl = r.standard_normal(n).astype(np.float32)
+    L = Box(ctx, dl)
+    mh.check(mh.lib().mmh_token_logprobs_backward(ctx.handle, Z.ptr, ptr(y), n, v, -1, L.ptr, None, out.ptr))
+    near(out.numpy(), *R.token_logprobs_backward(z, y, dl, None), "dlogits")
 
 
 def test_calls_that_follow_each_other_without_waiting(ctx):
