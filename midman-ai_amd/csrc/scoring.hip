@@ -339,22 +339,38 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int 
     sh.maxima[tid] = order_of(mine);
     __syncthreads();
     if (tid < 64) {
-        // A value that k threads' maxima reach, and a quarter and 8 more at most where they differ:
-        // halving the range of orders.
-        uint32_t m[NT / 64], lo = lowest, hi = 0;
+        // A value that k threads' maxima reach, and a quarter and 8 more at most where they
+        // differ. Their number falls by a factor for each step of the value, more or less, so a
+        // line through its logarithm finds it in a few tries; halving the range of orders ends it
+        // whatever the logits are.
+        uint32_t m[NT / 64], lo = ~0u, hi = 0;
 #pragma unroll
         for (int i = 0; i < NT / 64; ++i) {
             m[i] = sh.maxima[lane + 64 * i];
+            lo = min(lo, m[i]);
             hi = max(hi, m[i]);
         }
+        lo = NT < k ? lowest : ~wave_max(~lo);
         hi = wave_max(hi) + 1;  // (lo is reached by k maxima or is the lowest, hi by none)
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
+        float n_lo = (float)NT, n_hi = 0.5f;
+        for (int tries = 0; hi - lo > 1; ++tries) {
+            uint32_t mid = lo + (hi - lo) / 2;
+            if (tries < 5) {
+                const float v = value_of(lo), l = __builtin_amdgcn_logf(n_lo);
+                const float share = (l - __builtin_amdgcn_logf((float)(k + k / 8 + 4))) / (l - __builtin_amdgcn_logf(n_hi));
+                const float at = v + (value_of(hi - 1) - v) * share;
+                if (at > v) mid = max(lo + 1, min(hi - 1, order_of(at)));  // (not of a NaN or infinities)
+            }
             int n = 0;
 #pragma unroll
             for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(m[i] >= mid));
-            if (n < k) hi = mid;
-            else lo = mid;
+            if (n < k) {
+                hi = mid;
+                n_hi = fmaxf((float)n, 0.5f);
+            } else {
+                lo = mid;
+                n_lo = (float)n;
+            }
             if (n >= k && n <= k + k / 4 + 8) break;
         }
         if (tid == 0) {
