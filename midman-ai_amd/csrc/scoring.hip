@@ -304,6 +304,7 @@ __device__ __forceinline__ uint64_t row_entry(double e, uint32_t first) {
 struct TopShared {
     __attribute__((aligned(16))) double list[kList + 16];
     uint32_t maxima[512];  // of the threads, as orders
+    int32_t rank[kList];    // of the list's entries
     int32_t count[16];
     int32_t n;              // entries of the list
     float above;            // logits above it are in the list
@@ -470,27 +471,40 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int 
         __syncthreads();
         n = k;
     }
-    // (zeros, below every entry, to a whole number of reads)
-    if (tid < 16) sh.list[n + tid] = 0.0;
+    // Each wave compares its share of the list, read once for several entries of each lane, with
+    // all of it: an entry's rank is the sum of what the waves find above it.
+    constexpr int kWaves = NT / 64;
+    const int share = (n + 2 * kWaves - 1) / (2 * kWaves) * 2, from = (tid >> 6) * share;
+    for (int i = tid; i < n; i += NT) sh.rank[i] = 0;
+    if (tid < 16) sh.list[n + tid] = 0.0;  // (below every entry: the last reads end past it)
     __syncthreads();
-    auto ranks = [&](auto lanes) __attribute__((always_inline)) {
-        constexpr int L = decltype(lanes)::value;  // to an entry, each with its share of the others
-        for (int i = tid / L; i < n; i += NT / L) {
-            const double me = sh.list[i];
-            int rank = 0;
+    auto compare = [&](auto each) __attribute__((always_inline)) {
+        constexpr int E = decltype(each)::value;
+        const int to = min(n, from + share);
+        for (int at = lane; at < n + lane; at += 64 * E) {
+            double me[E];
+            int above[E] = {};
+#pragma unroll
+            for (int i = 0; i < E; ++i) me[i] = at + 64 * i < n ? sh.list[at + 64 * i] : 0.0;
 #pragma unroll 4
-            for (int j = 2 * (tid % L); j < n; j += 2 * L) {
+            for (int j = from; j < to; j += 2) {
                 const double2 x = *reinterpret_cast<const double2 *>(&sh.list[j]);
-                rank += x.x > me ? 1 : 0;
-                rank += x.y > me ? 1 : 0;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    above[i] += x.x > me[i] ? 1 : 0;
+                    above[i] += x.y > me[i] ? 1 : 0;
+                }
             }
 #pragma unroll
-            for (int off = 1; off < L; off <<= 1) rank += __shfl_xor(rank, off, 64);
-            if (tid % L == 0 && rank < k) place(rank, row_entry(me, first));
+            for (int i = 0; i < E; ++i)
+                if (at + 64 * i < n && above[i]) atomicAdd(&sh.rank[at + 64 * i], above[i]);
         }
     };
-    if (n <= NT / 4) ranks(std::integral_constant<int, 4>());
-    else ranks(std::integral_constant<int, 1>());
+    if (n <= 64) compare(std::integral_constant<int, 1>());
+    else compare(std::integral_constant<int, 2>());
+    __syncthreads();
+    for (int i = tid; i < n; i += NT)
+        if (sh.rank[i] < k) place(sh.rank[i], row_entry(sh.list[i], first));
 }
 
 __device__ __forceinline__ void score_left_out(const ScoreArgs &p, int64_t row, int threads) {
