@@ -402,6 +402,21 @@ def test_offsets_past_32_bits(ctx):
     free.free()
 
 
+def test_more_lists_than_a_join_holds(ctx):
+    # 16 parts with 256 entries each, equal values across them; a part that a row's place in its line leaves empty or short
+    for v in (500001, 16 * 32768 - 31, 16 * 32768 - 30):
+        z, y, _ = drawn(3, v, 16)
+        z[1] = np.round(2 * z[1]) / 2
+        z[2, :] = -1.0
+        for k in (256, 200, 3):
+            lp, h, ids, top = run_logprobs(ctx, z, y, k, shift=k % 32)
+            want_lp, want_h, (want_ids, want_top) = R.token_logprobs(z, y, k)
+            near(lp, *want_lp, "logprobs")
+            near(h, *want_h, "entropy")
+            assert np.array_equal(ids, want_ids)
+            near(top, *want_top, "top")
+
+
 def test_more_rows_than_a_launch(ctx):
     n, v = 2 ** 21 + 5, 3
     z, y, r = drawn(n, v, 15)
