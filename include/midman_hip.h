@@ -22,7 +22,8 @@
  * pointers from mmh_alloc and are asynchronous on the context's HIP stream.
  * Token ids and targets are always host arrays: they are validated on the host
  * (id < V, as ops_shape.rs:250-252 and ops_reduce.rs:250-252 do) before any
- * launch, so an out-of-range id is MMH_ERR_INDEX and nothing runs.
+ * launch, so an out-of-range id is MMH_ERR_INDEX and nothing runs. (A
+ * teacher's ids, mmh_distillation, are on the device and checked there.)
  *
  * Numerics: inputs, results and sums are f32 as in the reference. Products are
  * summed on the matrix cores in a different order from the reference's
