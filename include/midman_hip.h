@@ -507,7 +507,9 @@ int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const fl
  * log probabilities, top_ids and top_logprobs [n, k] (k = 0: none, up to 256 and to
  * vocab), the largest first, lower ids first among equals (-0 equals 0, and a NaN
  * counts as +inf). targets_host may be NULL where logprobs is: no row is left out
- * then. A row left out has 0, 0, ids -1 and log probabilities -inf. */
+ * then. A row left out has 0, 0, ids -1 and log probabilities -inf. For wide rows the
+ * context's workspace holds lists of 8 k bytes per 16384 columns or more: 64 MiB, or a
+ * row's where that is more. */
 int32_t mmh_token_logprobs(mmh_handle ctx, const float *logits, const int32_t *targets_host,
                            int64_t n, int64_t vocab, int32_t ignore, int64_t k, float *logprobs,
                            float *entropy, int32_t *top_ids, float *top_logprobs);
@@ -530,7 +532,7 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits,
  * empty slots has no first term. An id in several slots has all their shares.
  * temperature in [0.001, 1000], alpha in [0, 1] (at 0 the teacher is not looked at).
  * An id of vocab or more is MMH_ERR_INDEX, found by the kernels. The call waits for
- * its work. */
+ * its work, and holds 8 bytes of pinned host memory per row. */
 int32_t mmh_distillation(mmh_handle ctx, const float *logits, const int32_t *targets_host,
                          int64_t n, int64_t vocab, int32_t ignore, const int32_t *teacher_ids,
                          const float *teacher_logits, int64_t k, float temperature, float alpha,

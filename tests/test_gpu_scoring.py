@@ -402,6 +402,57 @@ def test_offsets_past_32_bits(ctx):
     free.free()
 
 
+@pytest.mark.parametrize("shape", [(5, 300), (3, 33001), (70, 33001), (300, 2000)])
+def test_outputs_that_are_not_asked_for(ctx, shape):
+    z, y, r = drawn(*shape, 17)
+    n, v = shape
+    Z = ctx.to_device(z)
+    full = mh.token_logprobs(ctx, Z, y, k=9)
+    lp, h, ids, top = (a.numpy() for a in full)
+    some = mh.token_logprobs(ctx, Z, y, entropy=False)
+    assert some.entropy is None and some.top_ids is None and np.array_equal(some.logprobs.numpy(), lp)
+    some = mh.token_logprobs(ctx, Z)
+    assert some.logprobs is None and np.array_equal(some.entropy.numpy(), h)
+    some = mh.token_logprobs(ctx, Z, k=9, entropy=False)
+    assert np.array_equal(some.top_ids.numpy(), ids) and np.array_equal(some.top_logprobs.numpy(), top)
+    out = Box(ctx, np.zeros((n, 9), np.float32)), Box(ctx, np.zeros((n, 9), np.int32))
+    y[0] = -1  # targets as a mask alone
+    mh.check(mh.lib().mmh_token_logprobs(ctx.handle, Z.ptr, ptr(y), n, v, -1, 9, None, None, out[1].ptr, out[0].ptr))
+    assert np.array_equal(out[1].numpy()[1:], ids[1:]) and (out[1].numpy()[0] == -1).all()
+    # the loss not asked for; the teacher's log probabilities in its logits' place
+    loss, g = mh.distillation_backward(ctx, Z, full.top_ids, full.top_logprobs, y, 2.0, 0.5)
+    G = Box(ctx, np.zeros((n, v), np.float32))
+    mh.check(mh.lib().mmh_distillation_backward(ctx.handle, Z.ptr, ptr(y), n, v, -1, full.top_ids.ptr, full.top_logprobs.ptr, 9, 2.0, 0.5,
+                                                G.ptr, None))
+    assert np.array_equal(G.numpy(), g.numpy())
+    logits = np.take_along_axis(z, ids.astype(np.int64), 1)
+    assert abs(mh.distillation(ctx, Z, full.top_ids, ctx.to_device(logits), y, 2.0, 0.5) - loss) <= 1e-5 * abs(loss) + 1e-6
+
+
+def test_more_slots_than_tokens(ctx):
+    for v, n in ((1, 4), (60, 7), (200, 300)):
+        z, y, r = drawn(n, v, 18)
+        ids = r.integers(-1, v, (n, 256)).astype(np.int32)
+        teacher = r.standard_normal((n, 256)).astype(np.float32)
+        row, tol, want, g_tol = R.distillation(z, y, ids, teacher, 1.5, 0.6, n)
+        loss, g = run_distill(ctx, z, y, ids, teacher, 1.5, 0.6)
+        near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
+        near(g, want, g_tol, "dlogits")
+
+
+def test_losses_that_share_pinned_memory(ctx):
+    z, y, r = drawn(700, 501, 19)
+    ids, teacher = teachers(r, z, 8)
+    x, w = (r.standard_normal(s).astype(np.float32) for s in ((900, 32), (501, 32)))
+    X, W, yy = ctx.to_device(x), ctx.to_device(w), r.integers(0, 501, 900).astype(np.int32)
+    first = run_distill(ctx, z, y, ids, teacher, 2.0, 0.5)
+    ce = mh.linear_cross_entropy(ctx, X, W, yy)
+    for _ in range(3):
+        again = run_distill(ctx, z, y, ids, teacher, 2.0, 0.5)
+        assert again[0] == first[0] and np.array_equal(again[1], first[1])
+        assert mh.linear_cross_entropy(ctx, X, W, yy) == ce
+
+
 def test_more_lists_than_a_join_holds(ctx):
     # 16 parts with 256 entries each, equal values across them; a part that a row's place in its line leaves empty or short
     for v in (500001, 16 * 32768 - 31, 16 * 32768 - 30):
