@@ -305,7 +305,11 @@ __device__ __forceinline__ uint64_t row_entry(double e, uint32_t first) {
 }
 
 struct TopShared {
-    __attribute__((aligned(16))) double list[kList + 16];
+    // as they are found, a logit and its column; in their order, entry_of
+    union __attribute__((aligned(16))) {
+        float2 found[kList + 16];
+        double list[kList + 16];
+    };
     uint32_t maxima[512];  // of the threads, as orders
     int32_t rank[kList];    // of the list's entries
     int32_t count[16];
@@ -407,7 +411,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int 
             asm volatile("" : "+v"(over));  // (compared again: the masks kept would not fit the scalar registers)
             hits(over, [&](uint64_t hit, float z, int col) {
                 const int to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
-                if (z > over && to < kList) sh.list[to] = entry_of(z, col);
+                if (z > over && to < kList) sh.found[to] = make_float2(z, __int_as_float(col));
                 at += __popcll(hit);
             });
         }
@@ -467,7 +471,7 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int 
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (hit[j] >> lane & 1) {
-                    if (before < k) sh.list[before] = entry_of(x[j], c0 + j);
+                    if (before < k) sh.found[before] = make_float2(x[j], __int_as_float(c0 + j));
                     ++before;
                 }
         }
@@ -478,7 +482,11 @@ __device__ __forceinline__ void top_of(const float (&e)[NV][4], int lo_col, int 
     // all of it: an entry's rank is the sum of what the waves find above it.
     constexpr int kWaves = NT / 64;
     const int share = (n + 2 * kWaves - 1) / (2 * kWaves) * 2, from = (tid >> 6) * share;
-    for (int i = tid; i < n; i += NT) sh.rank[i] = 0;
+    for (int i = tid; i < n; i += NT) {
+        sh.rank[i] = 0;
+        const float2 x = sh.found[i];
+        sh.list[i] = entry_of(x.x, __float_as_int(x.y));
+    }
     if (tid < 16) sh.list[n + tid] = 0.0;  // (below every entry: the last reads end past it)
     __syncthreads();
     auto compare = [&](auto each) __attribute__((always_inline)) {
