@@ -272,8 +272,8 @@ __device__ __forceinline__ float ranked(float z) { return z != z ? INFINITY : z;
 // more than k logits as a rule) goes to a list in LDS, where each entry's place is the
 // number of larger ones.
 // One read of the logits bounds it (4096 x 32000 without alternatives 93 us, 5.6 TB/s);
-// then the steps between barriers, of which two workgroups on a CU hide a part (k 16 101
-// us, 64 115, 128 136, 256 205; an argmax per alternative, as first built, k 64 7390).
+// then the steps between barriers, of which two workgroups on a CU hide a part (k 16 102
+// us, 64 112, 128 130, 256 192; an argmax per alternative, as first built, k 64 7390).
 struct ScoreArgs {
     const float *logits;
     HostIds targets;
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
 // The parts of a row together: their sums, and of their lists the k that come first, each
 // entry's place the number of larger ones. Latency: 4 rows of 131071, k 20, 13 us in the
 // two launches.
-constexpr int kJoinEntries = 3072;
+constexpr int kJoinEntries = 12 * 256;   // twelve of a thread: 48 KB for both lists
 __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
     __shared__ RowSums all;
     __shared__ uint64_t held[kJoinEntries], some[kJoinEntries];
