@@ -529,7 +529,8 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits,
  * and the loss their mean over the rows that are not left out (0 with none). The
  * cross entropy is of the row's target at temperature 1; with alpha = 1 targets_host
  * may be NULL. A slot whose id is negative or whose logit is -inf is empty; a row of
- * empty slots has no first term. An id in several slots has all their shares.
+ * empty slots has no first term, neither in the loss nor in its gradient. An id in
+ * several slots has all their shares.
  * temperature in [0.001, 1000], alpha in [0, 1] (at 0 the teacher is not looked at).
  * An id of vocab or more is MMH_ERR_INDEX, found by the kernels. The call waits for
  * its work, and holds 8 bytes of pinned host memory per row. */

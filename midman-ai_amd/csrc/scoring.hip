@@ -750,6 +750,7 @@ struct RowArgs {
 // What the threads of a row share after its sums are known.
 struct RowShared {
     RowSums parts[16];
+    int32_t filled[8];  // of the waves: whether one of their slots is the teacher's
     int32_t id[kMaxTop + 1];
     float weight[kMaxTop + 1], z[kMaxTop + 1];
 };
@@ -817,6 +818,7 @@ struct Slots {
         }
     }
     __device__ __forceinline__ void store(int k, RowShared &sh) const {
+        bool some = false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int j = threadIdx.x + NT * i;
@@ -824,7 +826,10 @@ struct Slots {
             sh.id[j] = id[i] < 0 ? -1 : id[i];
             sh.weight[j] = id[i] < 0 ? -INFINITY : weight[i];
             sh.z[j] = z[i];
+            some |= j < k && id[i] >= 0 && weight[i] != -INFINITY;
         }
+        some = __any(some);
+        if ((threadIdx.x & 63) == 0) sh.filled[threadIdx.x >> 6] = some;
     }
 };
 
@@ -857,7 +862,7 @@ struct Dense {
 
 // From the row's sums, by every thread; wave 0 turns the teacher's slots into shares,
 // and its lane 0 writes the row's loss where `loss`.
-template <int KIND>
+template <int NT, int KIND>
 __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int k, const RowSums &s, bool loss_too,
                                               RowShared &sh) {
     const float a = rest_of(s), total = 1.0f + a;
@@ -869,7 +874,12 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
         g.f1 = -dh / total;
         g.hit = -dl;
     } else {
-        const float soft = p.alpha * p.temperature * p.scale, hard = (1.0f - p.alpha) * p.scale;
+        // (the soft term's derivative is that of sum q (ln q - ln p_T), p_T times the sum of
+        // q, less q: a row of empty slots has neither)
+        int32_t filled = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) filled |= sh.filled[i];
+        const float soft = filled ? p.alpha * p.temperature * p.scale : 0.0f, hard = (1.0f - p.alpha) * p.scale;
         const float rest1 = s.u + (s.count - 1.0f);  // (KIND_BOTH)
         g.f0 = (KIND == KIND_BOTH ? soft : soft + hard) / total;
         if (KIND == KIND_BOTH) g.f1 = hard / (1.0f + rest1);
@@ -929,7 +939,7 @@ __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
     __syncthreads();
     s = row_sums(join_sums<KIND>(sh.parts, NT / 64, p.rate * kLog2e));
-    const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
+    const Dense g = coefficients<NT, KIND>(p, row, k, s, true, sh);
     if (!p.out) return;
     float *out = p.out + row * p.vocab;
     // (addresses formed anew: kept from the loads they would take the row's registers)
@@ -1003,7 +1013,7 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
     __syncthreads();
     s = row_sums(join_sums<KIND>(sh.parts, NT / 64, kx));
-    const Dense g = coefficients<KIND>(p, row, k, s, true, sh);
+    const Dense g = coefficients<NT, KIND>(p, row, k, s, true, sh);
     if (!p.out) return;
     float *out = p.out + row * v - shift;
     // (the addresses from here on are formed anew: kept from the first pass they would
@@ -1082,7 +1092,7 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     }
     __syncthreads();
     const RowSums s = row_sums(sh.parts[0]);
-    const Dense g = coefficients<KIND>(p, row, k, s, blockIdx.x == 0, sh);
+    const Dense g = coefficients<NT, KIND>(p, row, k, s, blockIdx.x == 0, sh);
     if (!p.out) return;
     float *out = p.out + row * v;
     write_stretch<NT, NV>(out + at - shift, lo, cols, p.stream, e, tid, [&](float x) { return g.at<KIND>(x); });

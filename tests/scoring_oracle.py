@@ -99,7 +99,7 @@ def distillation(z, targets, ids, teacher, temperature, alpha, count):
     kl = (q * gap).sum(-1)
     kl_tol = (q * (np.abs(gap) * q_err + 8 * U * size + q_err.max(-1, keepdims=True) + rest_tol)).sum(-1) + k * U * (q * np.abs(gap)).sum(-1) + k * TINY * 1e4
     row, tol = a * t * t * kl, a * t * t * (kl_tol + 6 * U * np.abs(kl))
-    soft, hard = a * t / count, (1.0 - a) / count
+    soft, hard = np.where(none, 0.0, a * t / count), (1.0 - a) / count  # (a row of empty slots has no first term)
     p, p1 = e / s, e1 / s1
     g = soft * p + hard * p1
     g_tol = (soft * p * ((28 + 6 * np.abs(np.maximum(dr, -1e4))) * U + err) + hard * p1 * ((28 + 6 * np.abs(np.maximum(dr1, -1e4))) * U + err1)
