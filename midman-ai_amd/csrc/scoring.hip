@@ -13,6 +13,7 @@
 // is log1p(rest): near a certain token the log probability and the entropy are as
 // small as the rest, and keep all their bits.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "mmh_args.h"
@@ -28,10 +29,31 @@ namespace {
 constexpr int64_t kMaxRows = int64_t(1) << 21;
 // Alternatives of a row, and slots of a teacher's, at most.
 constexpr int64_t kMaxTop = 256;
-constexpr float kLog2e = 1.4426950408889634f;
+
 // (exp(-200) is 0 in f32: a masked token's difference has this in its place, so that
 // its product with that 0 is one)
 constexpr float kFar = -200.0f;
+
+// log2 e / T in two floats of one sign, for exponentials of differences at temperature T.
+struct Rate {
+    float hi, lo;
+};
+inline Rate rate_of(double t) {
+    const double k = 1.4426950408889634074 / t;
+    float hi = (float)k;
+    if ((double)hi > k) hi = std::nextafterf(hi, 0.0f);
+    return Rate{hi, (float)(k - (double)hi)};
+}
+constexpr Rate kPlain{1.44269502f, 1.92596303e-8f};  // rate_of(1)
+// exp(d / T), d <= 0, off by up to (2 + |d| / T) 2^-24 of itself, to both sides alike: the
+// exponent rounds once. (With one float for log2 e every term is too large by 0.22 |d|
+// 2^-24, and ln S of 32000 logits by 7e-8; both cost the same within 1%. Carrying the exponent's rounding along as
+// well would leave 2^-23 alone, beside the |d| / T 2^-24 of d's own rounding: 4096 x
+// 32000 with both terms 227 -> 257 us, log probabilities 109 -> 114.) An infinite d has
+// -inf from both products.
+__device__ __forceinline__ float exp_of(float d, const Rate &k) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.hi, d * k.lo));
+}
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -143,7 +165,7 @@ __device__ __forceinline__ RowSums no_sums() { return RowSums{-INFINITY, 0.0f, 0
 // wave's largest logit lies in one group of strips as a rule: only there are its terms
 // told from the others, by a branch that the whole wave takes.
 template <int KIND, int NV>
-__device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4], float k) {
+__device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4], const Rate &k) {
     constexpr int G = NV < 16 ? (NV + 3) / 4 : 4;
     float top = -INFINITY, group[NV / G];
 #pragma unroll
@@ -158,9 +180,9 @@ __device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4],
     if (top > s.m) {
         // what is there is scaled to the new largest logit; its ones are ordinary terms
         if (s.m > -INFINITY) {
-            const float d = s.m - top, w = __builtin_amdgcn_exp2f(d * k);
+            const float d = s.m - top, w = exp_of(d, k);
             if (KIND == KIND_SCORES) s.u = (s.u + fmaxf(d, kFar) * (s.a + s.count)) * w;
-            if (KIND == KIND_BOTH) s.u = (s.u + s.count) * __builtin_amdgcn_exp2f(d * kLog2e);
+            if (KIND == KIND_BOTH) s.u = (s.u + s.count) * exp_of(d, kPlain);
             s.a = (s.a + s.count) * w;
         }
         s.m = top;
@@ -169,7 +191,7 @@ __device__ __forceinline__ void add_stretch(RowSums &s, const float (&e)[NV][4],
     const float m = s.m == -INFINITY ? 0.0f : s.m;  // (nothing but -inf: terms of 0)
     auto add = [&](float z, bool look) __attribute__((always_inline)) {
         const float d = z - m;
-        float x = __builtin_amdgcn_exp2f(d * k), x1 = KIND == KIND_BOTH ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.0f;
+        float x = exp_of(d, k), x1 = KIND == KIND_BOTH ? exp_of(d, kPlain) : 0.0f;
         if (look) {
             // (selected by arithmetic: a selection would become a branch around the exponentials)
             const float one = d == 0.0f ? 1.0f : 0.0f;
@@ -204,7 +226,7 @@ __device__ __forceinline__ RowSums wave_sums(RowSums s) {
 // The sums of n parts of a row together. (A part of nothing but -inf adds nothing; inf -
 // inf is NaN.)
 template <int KIND>
-__device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, float k) {
+__device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, const Rate &k) {
     RowSums s = no_sums();
     for (int i = 0; i < n; ++i) s.m = fmaxf(s.m, parts[i].m);
     for (int i = 0; i < n; ++i) {
@@ -216,10 +238,10 @@ __device__ __forceinline__ RowSums join_sums(const RowSums *parts, int n, float 
             s.a += p.a;
             s.u += p.u;
         } else {
-            const float w = __builtin_amdgcn_exp2f(d * k), all = p.a + p.count;
+            const float w = exp_of(d, k), all = p.a + p.count;
             s.a += all * w;
             if (KIND == KIND_SCORES) s.u += (p.u + fmaxf(d, kFar) * all) * w;
-            if (KIND == KIND_BOTH) s.u += (p.u + p.count) * __builtin_amdgcn_exp2f(d * kLog2e);
+            if (KIND == KIND_BOTH) s.u += (p.u + p.count) * exp_of(d, kPlain);
         }
     }
     return s;
@@ -237,7 +259,7 @@ __device__ __forceinline__ RowSums row_sums(RowSums s) {
 }
 // The sums of a row's n parts, by one wave: in every lane, in one order.
 template <int KIND>
-__device__ __forceinline__ RowSums wave_join(const RowSums *parts, int n, float k) {
+__device__ __forceinline__ RowSums wave_join(const RowSums *parts, int n, const Rate &k) {
     const int lane = threadIdx.x & 63;
     RowSums s = no_sums();
     for (int j = lane; j < n; j += 64) {
@@ -547,11 +569,11 @@ __global__ __launch_bounds__(NT, 4) void scores_kernel(ScoreArgs p) {
     const float zt = !PARTS && p.logprobs && tid == 0 ? z[t] : 0.0f;
     load_stretch<NT, NV>(z + at - shift, lo, cols, e);
     RowSums s = no_sums();
-    add_stretch<KIND_SCORES>(s, e, kLog2e);
+    add_stretch<KIND_SCORES>(s, e, kPlain);
     s = wave_sums(s);
     if ((tid & 63) == 0) lds[tid >> 6] = s;
     __syncthreads();
-    s = join_sums<KIND_SCORES>(lds, NT / 64, kLog2e);
+    s = join_sums<KIND_SCORES>(lds, NT / 64, kPlain);
     const bool odd = s.a != s.a;
     float rest = 0.0f;
     if constexpr (PARTS) {
@@ -600,7 +622,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(ScoreArgs p) {
         for (int i = tid; i < entries; i += 256) held[i] = best[i];
     if (tid == 0) count = 0;
     if (tid < 64) {
-        const RowSums s = wave_join<KIND_SCORES>(p.sums + row * parts, parts, kLog2e);
+        const RowSums s = wave_join<KIND_SCORES>(p.sums + row * parts, parts, kPlain);
         if (tid == 0) all = s;
     }
     __syncthreads();
@@ -736,7 +758,7 @@ struct RowArgs {
     const float *teacher;
     int k;
     float temperature, alpha, scale;  // scale: 1 / the rows that count
-    float rate;                       // of the first exponential: 1 / temperature, or 1 (KIND_SCORES, alpha 0)
+    Rate rate;                        // of the first exponential: at the temperature, or 1 (KIND_SCORES, alpha 0)
     float *row_loss;                  // [rows], 0 for a row that is left out
     int32_t *wrong;                   // receives 1 for a teacher's id beyond the vocabulary
     bool stream;
@@ -747,6 +769,12 @@ struct RowArgs {
     float *slot_z;    // [rows, k + 1]
 };
 
+// (log probabilities' is a constant)
+template <int KIND>
+__device__ __forceinline__ Rate rate_for(const RowArgs &p) {
+    return KIND == KIND_SCORES ? kPlain : p.rate;
+}
+
 // What the threads of a row share after its sums are known.
 struct RowShared {
     RowSums parts[16];
@@ -756,8 +784,9 @@ struct RowShared {
 };
 
 // The teacher's softmax over the slots in LDS (values in weight), by one wave: weight
-// becomes soft q. Returns sum_j q_j (ln q_j - (d_j rate - rest)).
-__device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate, float soft, float m, float rest) {
+// becomes soft q. Returns sum_j q_j (ln q_j - (d_j / temperature - rest)).
+__device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate &rate, float temperature, float soft, float m,
+                                               float rest) {
     const int lane = threadIdx.x & 63;
     float t[kMaxTop / 64], top = -INFINITY;
 #pragma unroll
@@ -768,11 +797,12 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate,
     top = wave_max(top);
     // (a row of empty slots has no teacher: every share 0)
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    float sum = 0.0f, e[kMaxTop / 64];
 #pragma unroll
     for (int i = 0; i < kMaxTop / 64; ++i) {
-        t[i] = (t[i] - base) * rate;
-        sum += __builtin_amdgcn_exp2f(t[i] * kLog2e);
+        t[i] -= base;
+        e[i] = exp_of(t[i], rate);
+        sum += e[i];
     }
     sum = wave_sum(sum);
     const float f = top == -INFINITY ? 0.0f : 1.0f / sum, log_sum = logf(sum);
@@ -781,8 +811,8 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, float rate,
     for (int i = 0; i < kMaxTop / 64; ++i) {
         const int j = lane + 64 * i;
         if (j >= k) break;
-        const float q = __builtin_amdgcn_exp2f(t[i] * kLog2e) * f;
-        if (q != 0.0f) kl += q * ((t[i] - log_sum) - ((sh.z[j] - m) * rate - rest));
+        const float q = e[i] * f;
+        if (q != 0.0f) kl += q * ((t[i] / temperature - log_sum) - ((sh.z[j] - m) / temperature - rest));
         sh.weight[j] = soft * q;
     }
     return wave_sum(kl);
@@ -847,16 +877,17 @@ __device__ __forceinline__ int row_shift(const RowArgs &p, int64_t row) {
     return line_shift((p.out ? p.out : p.logits) + row * p.vocab);
 }
 
-// A row's dense gradient exp2((z - m) k) (f0 + f1 (z - m)) (KIND_SCORES; KIND_ONE: f1 =
+// A row's dense gradient exp((z - m) rate) (f0 + f1 (z - m)) (KIND_SCORES; KIND_ONE: f1 =
 // 0; KIND_BOTH: f1 times the second exponential instead), and what its target has less.
 struct Dense {
-    float m, kx, f0, f1, hit;
+    Rate rate;
+    float m, f0, f1, hit;
     template <int KIND>
     __device__ __forceinline__ float at(float x) const {
-        const float d = x - m;
-        if (KIND == KIND_SCORES) return __builtin_amdgcn_exp2f(d * kx) * __builtin_fmaf(fmaxf(d, kFar), f1, f0);
-        const float g = __builtin_amdgcn_exp2f(d * kx) * f0;
-        return KIND == KIND_BOTH ? __builtin_fmaf(__builtin_amdgcn_exp2f(d * kLog2e), f1, g) : g;
+        const float d = x - m, e = exp_of(d, rate);
+        if (KIND == KIND_SCORES) return e * __builtin_fmaf(fmaxf(d, kFar), f1, f0);
+        const float g = e * f0;
+        return KIND == KIND_BOTH ? __builtin_fmaf(exp_of(d, kPlain), f1, g) : g;
     }
 };
 
@@ -866,7 +897,7 @@ template <int NT, int KIND>
 __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int k, const RowSums &s, bool loss_too,
                                               RowShared &sh) {
     const float a = rest_of(s), total = 1.0f + a;
-    Dense g{s.m, p.rate * kLog2e, 0.0f, 0.0f, 0.0f};
+    Dense g{rate_for<KIND>(p), s.m, 0.0f, 0.0f, 0.0f};
     if constexpr (KIND == KIND_SCORES) {
         const float rest = log1pf(a), h = rest - s.u / total;
         const float dl = p.dlogprobs ? p.dlogprobs[row] : 0.0f, dh = p.dentropy ? p.dentropy[row] : 0.0f;
@@ -885,7 +916,7 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
         if (KIND == KIND_BOTH) g.f1 = hard / (1.0f + rest1);
         g.hit = hard;
         if (threadIdx.x < 64) {
-            const float kl = teacher_terms(sh, k, p.rate, soft, s.m, log1pf(a));
+            const float kl = teacher_terms(sh, k, p.rate, p.temperature, soft, s.m, log1pf(a));
             float loss = 0.0f;
             if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
             if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(KIND == KIND_BOTH ? rest1 : a) - (sh.z[k] - s.m));
@@ -934,11 +965,11 @@ __global__ __launch_bounds__(NT, 4) void rows_kernel(RowArgs p) {
     const int shift = row_shift(p, row);
     load_stretch<NT, NV>(z - shift, shift, shift + v, e);
     slots.store(k, sh);
-    add_stretch<KIND>(s, e, p.rate * kLog2e);
+    add_stretch<KIND>(s, e, rate_for<KIND>(p));
     s = wave_sums(s);
     if ((tid & 63) == 0) sh.parts[tid >> 6] = s;
     __syncthreads();
-    s = row_sums(join_sums<KIND>(sh.parts, NT / 64, p.rate * kLog2e));
+    s = row_sums(join_sums<KIND>(sh.parts, NT / 64, rate_for<KIND>(p)));
     const Dense g = coefficients<NT, KIND>(p, row, k, s, true, sh);
     if (!p.out) return;
     float *out = p.out + row * p.vocab;
@@ -970,7 +1001,7 @@ __global__ __launch_bounds__(512, 2) void wide_rows_kernel(RowArgs p) {
     if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, 0, v);
     slots.gather(p, k, t, [&](int, int32_t id) { return z[id]; });
     slots.store(k, sh);
-    const float kx = p.rate * kLog2e;
+    const Rate kx = rate_for<KIND>(p);
     RowSums s = no_sums();
     const int shift = row_shift(p, row);
     constexpr int64_t kHeld = 4 * NT * R, kKept = kHeld + 4 * NT * L;
@@ -1060,11 +1091,11 @@ __global__ __launch_bounds__(NT, 4) void parts_kernel(RowArgs p) {
     float e[NV][4];
     RowSums s = no_sums();
     load_stretch<NT, NV>(z + at - shift, lo, cols, e);
-    add_stretch<KIND>(s, e, p.rate * kLog2e);
+    add_stretch<KIND>(s, e, rate_for<KIND>(p));
     s = wave_sums(s);
     if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) p.sums[row * p.parts + blockIdx.x] = with_nan(join_sums<KIND>(parts, NT / 64, p.rate * kLog2e));
+    if (threadIdx.x == 0) p.sums[row * p.parts + blockIdx.x] = with_nan(join_sums<KIND>(parts, NT / 64, rate_for<KIND>(p)));
 }
 
 template <int NT, int NV, int KIND>
@@ -1079,7 +1110,7 @@ __global__ __launch_bounds__(NT, 4) void parts_grad_kernel(RowArgs p) {
     if (p.targets.given && t == p.ignore) return left_out<NT>(p, row, from, end);
     const float *z = p.logits + row * v;
     const int k = KIND == KIND_SCORES ? 0 : p.k, tid = threadIdx.x;
-    const float kx = p.rate * kLog2e;
+    const Rate kx = rate_for<KIND>(p);
     float e[NV][4];
     if (p.out) load_stretch<NT, NV>(z + at - shift, lo, cols, e);
     Slots<NT> slots;
@@ -1234,7 +1265,7 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
     p.k = d.alpha > 0.0f ? (int)d.k : 0;  // (the teacher has no share at alpha 0)
     p.temperature = d.temperature;
     p.alpha = d.alpha;
-    p.rate = d.alpha > 0.0f ? 1.0f / d.temperature : 1.0f;
+    p.rate = rate_of(d.alpha > 0.0f ? (double)d.temperature : 1.0);
     p.scale = 1.0f / (float)std::max<int64_t>(1, kept);
     p.wrong = pinned;
     *pinned = 0;
@@ -1326,7 +1357,6 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits, const i
         p.ignore = ignore;
         p.dlogprobs = dlogprobs;
         p.dentropy = dentropy;
-        p.rate = 1.0f;
         p.out = dlogits;
         launch_rows<KIND_SCORES>(cx, p, n, targets_host);
         return MMH_OK;
