@@ -10,8 +10,9 @@
 //   alpha T (p_T - q) + (1 - alpha) (p - onehot), p and p_T the row's softmax at 1 and T.
 //
 // S is kept as 1 + rest, without one of the largest logits' terms, and its logarithm
-// is log1p(rest): near a certain token the log probability and the entropy are as
-// small as the rest, and keep all their bits.
+// is log1p(rest): near a certain token the log probability, the entropy and the target's
+// gradient are as small as the rest, and keep all their bits. (A teacher's share q does
+// not: p_T - q is off by a rounding of q.)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -47,10 +48,10 @@ inline Rate rate_of(double t) {
 constexpr Rate kPlain{1.44269502f, 1.92596303e-8f};  // rate_of(1)
 // exp(d / T), d <= 0, off by up to (2 + |d| / T) 2^-24 of itself, to both sides alike: the
 // exponent rounds once. (With one float for log2 e every term is too large by 0.22 |d|
-// 2^-24, and ln S of 32000 logits by 7e-8; both cost the same within 1%. Carrying the exponent's rounding along as
-// well would leave 2^-23 alone, beside the |d| / T 2^-24 of d's own rounding: 4096 x
-// 32000 with both terms 227 -> 257 us, log probabilities 109 -> 114.) An infinite d has
-// -inf from both products.
+// 2^-24, and ln S of 32000 logits by 7e-8; both cost the same within 1%. Carrying the
+// exponent's rounding along as well would leave 2^-23 alone, beside the |d| / T 2^-24 of
+// d's own rounding: 4096 x 32000 with both terms 227 -> 257 us, log probabilities 109 ->
+// 114.) An infinite d has -inf from both products.
 __device__ __forceinline__ float exp_of(float d, const Rate &k) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.hi, d * k.lo));
 }
@@ -781,6 +782,7 @@ struct RowShared {
     int32_t filled[8];  // of the waves: whether one of their slots is the teacher's
     int32_t id[kMaxTop + 1];
     float weight[kMaxTop + 1], z[kMaxTop + 1];
+    float own;           // the target's gradient but for the teacher's shares, if its logit is the largest
 };
 
 // The teacher's softmax over the slots in LDS (values in weight), by one wave: weight
@@ -899,11 +901,13 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
     const float a = rest_of(s), total = 1.0f + a;
     Dense g{rate_for<KIND>(p), s.m, 0.0f, 0.0f, 0.0f};
     if constexpr (KIND == KIND_SCORES) {
-        const float rest = log1pf(a), h = rest - s.u / total;
+        // (ln p + H is d - sum exp(d) d / S: what a certain token has there is as small as u)
         const float dl = p.dlogprobs ? p.dlogprobs[row] : 0.0f, dh = p.dentropy ? p.dentropy[row] : 0.0f;
-        g.f0 = (-dl - dh * (h - rest)) / total;
+        const float bent = dh * (s.u / total);
+        g.f0 = (bent - dl) / total;
         g.f1 = -dh / total;
         g.hit = -dl;
+        if (threadIdx.x == 0) sh.own = dl * (a / total) + bent / total;
     } else {
         // (the soft term's derivative is that of sum q (ln q - ln p_T), p_T times the sum of
         // q, less q: a row of empty slots has neither)
@@ -915,11 +919,13 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
         g.f0 = (KIND == KIND_BOTH ? soft : soft + hard) / total;
         if (KIND == KIND_BOTH) g.f1 = hard / (1.0f + rest1);
         g.hit = hard;
+        const float other = KIND == KIND_BOTH ? rest1 : a;
+        if (threadIdx.x == 0) sh.own = soft / total - hard * (other / (1.0f + other));
         if (threadIdx.x < 64) {
             const float kl = teacher_terms(sh, k, p.rate, p.temperature, soft, s.m, log1pf(a));
             float loss = 0.0f;
             if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
-            if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(KIND == KIND_BOTH ? rest1 : a) - (sh.z[k] - s.m));
+            if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(other) - (sh.z[k] - s.m));
             // (without a distribution the loss is NaN, also where no term above has met it)
             if (a != a) loss = a;
             if (loss_too && threadIdx.x == 0) p.row_loss[row] = loss;
@@ -929,7 +935,8 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
 }
 
 // The few tokens' own values, for columns at .. end - 1, after the dense ones: an
-// id's first slot takes the shares of all its slots.
+// id's first slot takes the shares of all its slots. A target whose logit is the largest
+// has 1 - p = rest / S, which keeps its bits where p is near 1.
 template <int NT, int KIND>
 __device__ __forceinline__ void patch(float *out, int64_t at, int64_t end, int k, const Dense &g, const RowShared &sh) {
     for (int j = threadIdx.x; j <= k; j += NT) {
@@ -937,12 +944,15 @@ __device__ __forceinline__ void patch(float *out, int64_t at, int64_t end, int k
         if (id < at || id >= end) continue;
         float w = 0.0f;
         bool first = true;
-        for (int i = 0; i <= k; ++i)
+        for (int i = 0; i < k; ++i)
             if (sh.id[i] == id) {
                 first = first && i >= j;
-                w += i < k ? sh.weight[i] : g.hit;
+                w += sh.weight[i];
             }
-        if (first) out[id] = g.at<KIND>(sh.z[j]) - w;
+        if (!first) continue;
+        const float z = sh.z[j];
+        const bool target = sh.id[k] == id;
+        out[id] = target && z == g.m ? sh.own - w : g.at<KIND>(z) - (target ? w + g.hit : w);
     }
 }
 

@@ -81,3 +81,28 @@ def test_log_probabilities_are_not_biased(ctx):
     y = np.abs(want + 12.0).argmin(1).astype(np.int32)
     lp, h, ids, top = run_logprobs(ctx, z, y, 0)
     assert abs((lp - want[np.arange(n), y]).mean()) <= 2.6e-8
+
+
+# One token far ahead of the others: 1 - p is as small as exp(-gap), and the target's gradient is right relative to itself.
+# In steps of u: the small sum's exponential (3 + 2 gap) (d is exact here but for its exponent, which rounds), its sum and
+# quotients 3 each, the factors 3; the entropy's has a product by the gap and one quotient more.
+@pytest.mark.parametrize("n,v", KERNELS)
+def test_a_certain_targets_gradient_keeps_its_bits(ctx, n, v):
+    gaps = np.array([1.0, 5.0, 20.0, 40.0, 80.0])[np.arange(n) % 5]
+    z = np.full((n, v), -np.inf, np.float32)
+    at, y = np.full(n, v // 3), np.full(n, v - 2, np.int32)
+    rows = np.arange(n)
+    z[rows, y], z[rows, at] = 3.0, 3.0 - gaps
+    x = np.exp(-gaps)
+    tol = (20 + 2 * gaps) * R.U
+    one = np.ones(n, np.float32)
+    g = run_logprobs_bwd(ctx, z, y, one, None)
+    assert (np.abs(g[rows, y] / (x / (1 + x)) - 1) <= tol).all()
+    g = run_logprobs_bwd(ctx, z, y, None, one)
+    assert (np.abs(g[rows, y] / (-gaps * x / (1 + x) ** 2) - 1) <= tol).all()
+    # the cross entropy's, alone and beside a teacher's term that has nothing there
+    ids = np.full((n, 2), -1, np.int32)
+    for temperature, alpha in ((1.0, 0.0), (1.0, 0.5), (2.0, 0.5)):
+        _, g = run_distill(ctx, z, y, ids, np.zeros((n, 2), np.float32), temperature, alpha)
+        want = -(1 - alpha) / n * x / (1 + x)
+        assert (np.abs(g[rows, y] / want - 1) <= tol).all(), (temperature, alpha)
