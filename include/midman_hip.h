@@ -509,7 +509,7 @@ int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const fl
  * vocab), the largest first, lower ids first among equals (-0 equals 0, and a NaN
  * counts as +inf). targets_host may be NULL where logprobs is: no row is left out
  * then. A row left out has 0, 0, ids -1 and log probabilities -inf. For wide rows the
- * context's workspace holds lists of 8 k bytes per 16384 columns or more: 64 MiB, or a
+ * context's workspace holds lists of 8 k bytes per 10944 columns or more: 64 MiB, or a
  * row's where that is more. */
 int32_t mmh_token_logprobs(mmh_handle ctx, const float *logits, const int32_t *targets_host,
                            int64_t n, int64_t vocab, int32_t ignore, int64_t k, float *logprobs,

@@ -686,17 +686,25 @@ int64_t round_line(int64_t v) { return (v + kLine - 1) / kLine * kLine; }
 int64_t line_cols(const float *rows, int64_t v) {
     return (reinterpret_cast<uintptr_t>(rows) & (4 * kLine - 1)) == 0 && v % kLine == 0 ? v : v + kLine - 1;
 }
-// Columns of a part at most, and the bytes that the parts' lists may take.
-constexpr int64_t kScoreCols = 32768, kScoreBytes = int64_t(64) << 20;
+// Columns of a part at most, of one at least (a row of one column more than a part makes
+// three of 16384 at most: a third, in whole lines), and the bytes that the parts' lists
+// may take.
+constexpr int64_t kScoreCols = 32768, kPartLeast = (kScoreCols / 3 + kLine) / kLine * kLine, kScoreBytes = int64_t(64) << 20;
+static_assert(kPartLeast == 10944, "as the header says");
 
 template <bool PARTS>
 void launch_scores(Context &cx, const ScoreArgs &p, dim3 grid, int64_t cols) {
     auto launch = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, cx.stream, p); };
-    if (cols <= 1024) launch(scores_kernel<256, 1, PARTS>, 256);
-    else if (cols <= 4096) launch(scores_kernel<256, 4, PARTS>, 256);
-    else if (cols <= 8192) launch(scores_kernel<512, 4, PARTS>, 512);
-    else if (cols <= 16384) launch(scores_kernel<512, 8, PARTS>, 512);
-    else launch(scores_kernel<512, 16, PARTS>, 512);
+    if constexpr (PARTS) {  // (of kPartLeast columns at least)
+        if (cols <= 16384) launch(scores_kernel<512, 8, true>, 512);
+        else launch(scores_kernel<512, 16, true>, 512);
+    } else {
+        if (cols <= 1024) launch(scores_kernel<256, 1, false>, 256);
+        else if (cols <= 4096) launch(scores_kernel<256, 4, false>, 256);
+        else if (cols <= 8192) launch(scores_kernel<512, 4, false>, 512);
+        else if (cols <= 16384) launch(scores_kernel<512, 8, false>, 512);
+        else launch(scores_kernel<512, 16, false>, 512);
+    }
     check_hip(hipGetLastError(), "token_logprobs launch");
 }
 
@@ -718,8 +726,9 @@ void scores(Context &cx, const ScoreArgs &all, int64_t n) {
             launch_scores<false>(cx, rows_from(all, at), dim3((unsigned)std::min(kMaxRows, n - at)), cols);
         return;
     }
-    // parts for two workgroups per CU, of 16384 columns at least (of 4096: 4 x 131071 15.2 -> 17.9 us,
-    // 1 x 262144 15.6 -> 24.5: more lists to join), whose lists fit the join's LDS
+    // parts for two workgroups per CU, of 16384 columns or the few thousand less that parts of
+    // one size come to, kPartLeast (of 4096: 4 x 131071 15.2 -> 17.9 us, 1 x 262144 15.6 ->
+    // 24.5: more lists to join), whose lists fit the join's LDS
     const int64_t fit = std::min<int64_t>(256, kJoinEntries / std::max(1, all.k));
     const int64_t want = std::max((cols + kScoreCols - 1) / kScoreCols, std::min({(cols + 16383) / 16384, 2 * cx.cu_count / n, fit}));
     const int64_t part = round_line((cols + want - 1) / want), parts = (cols + part - 1) / part;
