@@ -106,3 +106,132 @@ def test_a_certain_targets_gradient_keeps_its_bits(ctx, n, v):
         _, g = run_distill(ctx, z, y, ids, np.zeros((n, 2), np.float32), temperature, alpha)
         want = -(1 - alpha) / n * x / (1 + x)
         assert (np.abs(g[rows, y] / want - 1) <= tol).all(), (temperature, alpha)
+
+
+# (rows, vocab): odd lengths, so that the rows begin at every place of a cache line, on both sides of each kernel's width;
+# 33 rows wider than a workgroup's registers go by parts, 70 by a workgroup each
+ODD = [(40, v) for v in (1, 3, 63, 991, 993, 995, 1025, 4063, 4065, 4067, 8159, 8161, 8163, 16353, 16355, 32735, 32737)]
+ODD += [(n, v) for v in (32739, 32767, 32769, 65535, 65537, 98303, 98305, 131041, 131073, 140001) for n in (33, 70)] + [(33, 262143)]
+HALF = float(np.float32(np.log(2.0)))  # exp(-HALF / T T) is 1/2 in f32, and sums of halves and quarters are exact
+
+
+@pytest.mark.parametrize("n,v", ODD)
+def test_every_column_counts_once(ctx, n, v):
+    # Rows of equal logits, and of one with all the others log 2 (at T) below it: every sum is exact, so a column that is
+    # lost or counted twice moves a gradient by 1 / v of itself, where its factor's roundings (the mean's, the temperature's,
+    # a quotient, a sum of two terms, the hardware's 2^x) are within 16 u, and a log probability by 1 / v, where log1p and a
+    # difference are within 2.5 steps of its value.
+    assert 1.0 / v > 24 * R.U
+    y, at = (np.arange(n) * 13 % v).astype(np.int32), (np.arange(n) * 7 + v // 2) % v
+    rows, free = np.arange(n), np.ones((n, v), bool)
+    free[rows, y] = free[rows, at] = False
+    one, none = np.ones(n, np.float32), np.zeros((n, 1), np.float32)
+    ids = y[:, None].copy()
+    for low in (0.0, HALF):
+        for t in (1.0, 2.0):
+            z = np.full((n, v), -t * low, np.float32)
+            z[rows, at] = 0.0
+            x, x1 = (1.0, 1.0) if low == 0.0 else (0.5, 0.5 ** t)
+            s, s1 = 1.0 + (v - 1) * x, 1.0 + (v - 1) * x1
+
+            def factor(got, want, what):
+                assert np.abs(got[free] / want - 1.0).max(initial=0.0) <= 16 * R.U, (what, low, t, np.abs(got[free] / want - 1.0).max() / R.U)
+
+            if t == 1.0:
+                lp, h, _, top = run_logprobs(ctx, z, y, 1, shift=n % 32)
+                step = np.spacing(np.float32(max(np.log(s), 1e-30)))
+                d = z[rows, y].astype(np.float64)
+                assert np.abs(lp - (d - np.log(s))).max() <= 2.5 * max(step, float(np.spacing(np.float32(abs(lp).max()))))
+                assert np.abs(top[:, 0] + np.log(s)).max() <= 2.5 * step
+                factor(run_logprobs_bwd(ctx, z, y, one, None, shift=3), -x / s, "log probabilities")
+            factor(run_distill(ctx, z, None, ids, none, t, 1.0, shift=1)[1], t / n * x / s, "softened")
+            if t != 1.0:
+                factor(run_distill(ctx, z, y, ids, none, t, 0.5, inplace=True)[1], (0.5 * t * x / s + 0.5 * x1 / s1) / n, "both")
+
+
+@pytest.mark.parametrize("n,v", [(n, v) for n, v in ODD if v > 200])
+def test_entropies_of_tokens_at_borders(ctx, n, v):
+    # All but 48 tokens of a row masked: its ends, and others on both sides of cache lines, where strips, passes and parts
+    # begin. Masked ones add 0 exactly, so 48 terms and 64 joins round, three times each.
+    r = np.random.default_rng(v)
+    f = 48
+    z = np.full((n, v), -np.inf, np.float32)
+    for i in range(n):
+        shift = (5 + i * v) % 32
+        line = 32 * r.integers(1, v // 32 + 1, 300) - shift - r.integers(0, 2, 300)
+        line = np.unique(line[(line >= 2) & (line < v - 2)])
+        cols = np.concatenate([[0, 1, v - 2, v - 1], r.permutation(line)[:f - 4]])
+        z[i, cols] = r.integers(0, 64, len(cols)) / 64.0
+    y = z.argmax(1).astype(np.int32)
+    lp, h, ids, top = run_logprobs(ctx, z, y, 20, shift=5)
+    d = z.astype(np.float64) - z.max(1, keepdims=True)
+    e = np.exp(d)
+    s = e.sum(1)
+    want_h = np.log(s) - np.where(e > 0, e * np.maximum(d, -1e9), 0.0).sum(1) / s
+    tol = 3 * (f + 64) * R.U
+    assert np.abs(lp + np.log(s)).max() <= tol + 8 * R.U * np.log(s).max()
+    assert np.abs(h - want_h).max() <= 3 * tol + 8 * R.U * want_h.max()
+    want_ids = np.argsort(-z, axis=1, kind="stable")[:, :20]
+    assert np.array_equal(ids, want_ids)
+
+
+@pytest.mark.parametrize("v", [999, 4001, 8001, 16001, 32001, 32751, 49999, 90001, 120001, 140001])
+def test_outputs_past_the_caches(ctx, v):
+    # 256 MiB of gradients and more, rows by a workgroup each: 67 different ones over and over, at every place of a line
+    base = 67
+    reps = (1 << 26) // (base * v) + 1
+    n = base * reps
+    assert n * v * 4 >= 1 << 28
+    z, y, r = drawn(base, v, v)
+    y[5] = -1
+    keep = y != -1
+    dl, dh = r.standard_normal(base).astype(np.float32), (0.1 * r.standard_normal(base)).astype(np.float32)
+    ids, teacher = teachers(r, z, 9)
+    Z, yy = np.tile(z, (reps, 1)), np.tile(y, reps)
+
+    def rows(got, want, tol, what):
+        want, tol = want.astype(np.float32), (tol + R.U * np.abs(want)).astype(np.float32)
+        for g in got.reshape(reps, base, v):
+            assert (g[~keep] == 0).all() and (np.abs(g[keep] - want) <= tol).all(), (what, np.abs(g[keep] - want).max())
+
+    kept = int(keep.sum()) * reps
+    print(f"\n[past the caches] {n} x {v}", flush=True)
+    g = run_logprobs_bwd(ctx, Z, yy, np.tile(dl, reps), np.tile(dh, reps), shift=1)
+    rows(g, *R.token_logprobs_backward(z[keep], y[keep], dl[keep], dh[keep]), "log probabilities")
+    for temperature, inplace in ((1.0, False), (2.0, True)):
+        row, tol, want, g_tol = R.distillation(z[keep], y[keep], ids[keep], teacher[keep], temperature, 0.5, kept)
+        loss, g = run_distill(ctx, Z, yy, np.tile(ids, (reps, 1)), np.tile(teacher, (reps, 1)), temperature, 0.5, inplace=inplace)
+        near(np.float32(loss), row.mean(), tol.mean() + R.U * abs(row.mean()), "loss")
+        rows(g, want, g_tol, ("distillation", temperature))
+
+
+def test_more_lists_than_the_workspace_takes(ctx):
+    # 16257 rows' lists of 256 entries in two parts are 64 MiB: rows on both sides of that, behind others that are left out
+    v, n, k = 32800, 16300, 256
+    Z = ctx.empty((n, v))
+    z, y, _ = drawn(6, v, 22)
+    at = 16254
+    targets = np.full(n, -1, np.int32)
+    targets[at:at + 6] = y
+    mh.check(mh.lib().mmh_upload(ctx.handle, Z.offset(at * v), z.ctypes.data, z.nbytes))
+    s = mh.token_logprobs(ctx, Z, targets, k=k)
+    want_lp, want_h, (want_ids, want_top) = R.token_logprobs(z, y, k)
+    near(s.logprobs.numpy()[at:at + 6], *want_lp, "logprobs")
+    near(s.entropy.numpy()[at:at + 6], *want_h, "entropy")
+    ids, top = s.top_ids.numpy(), s.top_logprobs.numpy()
+    assert np.array_equal(ids[at:at + 6], want_ids)
+    near(top[at:at + 6], *want_top, "top")
+    assert (np.delete(ids, np.arange(at, at + 6), 0) == -1).all()
+    Z.free()
+
+
+def test_more_parts_than_a_join_holds(ctx):
+    z, y, _ = drawn(2, 257 * 32768 + 5, 23)
+    z[0, -1], z[1, 0] = 30.0, 30.0
+    for k in (0, 3):
+        lp, h, ids, top = run_logprobs(ctx, z, y, k, shift=7)
+        want_lp, want_h, (want_ids, want_top) = R.token_logprobs(z, y, k)
+        near(lp, *want_lp, "logprobs")
+        near(h, *want_h, "entropy")
+        assert np.array_equal(ids, want_ids)
+        near(top, *want_top, "top")
