@@ -532,7 +532,9 @@ int32_t mmh_token_logprobs_backward(mmh_handle ctx, const float *logits,
  * may be NULL. A slot whose id is negative or whose logit is -inf is empty; a row of
  * empty slots has no first term, neither in the loss nor in its gradient. An id in
  * several slots has all their shares.
- * temperature in [0.001, 1000], alpha in [0, 1] (at 0 the teacher is not looked at).
+ * temperature in [0.001, 1000], alpha in [0, 1] (at 0 the teacher is not looked at). The
+ * first term's sums are f32 and their error has the factor temperature^2: 0.1 x 2^-24
+ * temperature^2 for a student near its teacher over 200 tokens, 0.004 at 1000.
  * An id of vocab or more is MMH_ERR_INDEX, found by the kernels. The call waits for
  * its work, and holds 8 bytes of pinned host memory per row. */
 int32_t mmh_distillation(mmh_handle ctx, const float *logits, const int32_t *targets_host,

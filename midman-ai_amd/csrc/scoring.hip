@@ -795,9 +795,12 @@ struct RowShared {
 };
 
 // The teacher's softmax over the slots in LDS (values in weight), by one wave: weight
-// becomes soft q. Returns sum_j q_j (ln q_j - (d_j / temperature - rest)).
+// becomes soft q. Returns sum_j q_j (ln q_j - ln p_T(id_j)), `a` the S - 1 of p_T. Logits are
+// subtracted from logits and the logarithm taken of the two sums' quotient, by what it
+// differs from 1 where that is little: each ln q and ln p on its own is some 10, whose
+// rounding T^2 would make larger than a small term.
 __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate &rate, float temperature, float soft, float m,
-                                               float rest) {
+                                               float a) {
     const int lane = threadIdx.x & 63;
     float t[kMaxTop / 64], top = -INFINITY;
 #pragma unroll
@@ -808,22 +811,24 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate 
     top = wave_max(top);
     // (a row of empty slots has no teacher: every share 0)
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, e[kMaxTop / 64];
+    float some = 0.0f, e[kMaxTop / 64];
+    int count = 0;
 #pragma unroll
     for (int i = 0; i < kMaxTop / 64; ++i) {
         t[i] -= base;
         e[i] = exp_of(t[i], rate);
-        sum += e[i];
+        count += __popcll(__ballot(t[i] == 0.0f));
+        some += t[i] == 0.0f ? 0.0f : e[i];
     }
-    sum = wave_sum(sum);
-    const float f = top == -INFINITY ? 0.0f : 1.0f / sum, log_sum = logf(sum);
+    const float rest = wave_sum(some) + (float)(count - 1), sum = 1.0f + rest, total = 1.0f + a, off = (rest - a) / total;
+    const float f = top == -INFINITY ? 0.0f : 1.0f / sum, log_ratio = fabsf(off) < 0.5f ? log1pf(off) : logf(sum / total);
     float kl = 0.0f;
 #pragma unroll
     for (int i = 0; i < kMaxTop / 64; ++i) {
         const int j = lane + 64 * i;
         if (j >= k) break;
         const float q = e[i] * f;
-        if (q != 0.0f) kl += q * ((t[i] / temperature - log_sum) - ((sh.z[j] - m) / temperature - rest));
+        if (q != 0.0f) kl += q * ((t[i] - (sh.z[j] - m)) / temperature - log_ratio);
         sh.weight[j] = soft * q;
     }
     return wave_sum(kl);
@@ -931,7 +936,7 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
         const float other = KIND == KIND_BOTH ? rest1 : a;
         if (threadIdx.x == 0) sh.own = soft / total - hard * (other / (1.0f + other));
         if (threadIdx.x < 64) {
-            const float kl = teacher_terms(sh, k, p.rate, p.temperature, soft, s.m, log1pf(a));
+            const float kl = teacher_terms(sh, k, p.rate, p.temperature, soft, s.m, a);
             float loss = 0.0f;
             if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
             if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(other) - (sh.z[k] - s.m));

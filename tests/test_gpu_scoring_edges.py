@@ -235,3 +235,40 @@ def test_more_parts_than_a_join_holds(ctx):
         near(h, *want_h, "entropy")
         assert np.array_equal(ids, want_ids)
         near(top, *want_top, "top")
+
+
+@pytest.mark.parametrize("v", [2, 3, 50, 100, 200, 255, 256])
+def test_a_student_that_is_its_teacher(ctx, v):
+    # Every token has a slot, in another order, and the same logit but for a constant: the loss is 0, and so it is here, since
+    # all sums of equal logits and of halves are exact and every logarithm is of 1. Temperatures up to 1000 do not change it.
+    n = 6
+    r = np.random.default_rng(v)
+    ids = np.stack([r.permutation(v) for _ in range(n)]).astype(np.int32)
+    for t in (1.0, 2.0, 64.0, 1000.0):
+        for low in (0.0, t * HALF if t != 1000.0 else 0.0):
+            z = np.full((n, v), -low, np.float32)
+            z[np.arange(n), r.integers(0, v, n)] = 0.0
+            teacher = np.take_along_axis(z, ids.astype(np.int64), 1)
+            if low == 0.0:
+                teacher += np.float32(8.0)
+            loss, g = run_distill(ctx, z, None, ids, teacher, t, 1.0)
+            assert loss == 0.0, (t, low, loss)
+            assert np.abs(g).max() <= 8 * R.U * t / n
+
+
+def test_losses_at_high_temperatures(ctx):
+    # A student near its teacher: beside the exact sums above, each exponential is within (3 + 2 |d| / T) u, and a sum of 200
+    # has 14 roundings on its way at most, so both sums' quotient is within 2 (3 + 2 |d| / T + 14) + 3 u, and the loss within
+    # T^2 of that.
+    n, v = 64, 200
+    r = np.random.default_rng(31)
+    z = (2 * r.standard_normal((n, v))).astype(np.float32)
+    ids = np.stack([r.permutation(v) for _ in range(n)]).astype(np.int32)
+    teacher = (np.take_along_axis(z, ids.astype(np.int64), 1) + 0.3 * r.standard_normal((n, v))).astype(np.float32)
+    for t in (1.0, 5.0, 50.0, 200.0, 1000.0):
+        row, tol, want, g_tol = R.distillation(z, None, ids, teacher, t, 1.0, n)
+        loss, g = run_distill(ctx, z, None, ids, teacher, t, 1.0)
+        print(f"\n[high temperature] T={t}: loss {loss}, off by {abs(loss - row.mean()) / t ** 2 / R.U:.2f} u T^2", flush=True)
+        d = np.abs(z - z.max(1, keepdims=True)).max() + 1.0
+        assert abs(loss - row.mean()) <= t * t * (2 * (3 + 2 * d / t + 14) + 3) * R.U + 16 * R.U * row.mean()
+        near(g, want, g_tol, "dlogits")
