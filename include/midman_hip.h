@@ -496,11 +496,13 @@ int32_t mmh_linear_cross_entropy_backward(mmh_handle ctx, int32_t form, const fl
  * logits [n, vocab] f32, contiguous at any 4-byte alignment; targets on the host
  * (MMH_ERR_INDEX, and nothing runs, for one outside [0, vocab) that is not
  * `ignore`, any value, -1 say). A row whose target is `ignore` is left out, and
- * nothing it holds is read. Sums are f32; the exponential of a difference d at temperature
- * T is off by up to (3 + 2 |d| / T) 2^-24 of itself (d and d / T log2 e round). A logit of -inf is a masked token: its
- * probability is 0, and so is its gradient. A row whose largest logit is not finite
- * (nothing but -inf, a +inf, a NaN) has no distribution: its log probabilities,
- * entropy, loss and gradients are NaN. An output that overlaps another buffer of
+ * nothing it holds is read. Sums are f32; the exponential of a difference d at
+ * temperature T is off by up to (3 + 2 |d| / T) 2^-24 of itself (d rounds, and its
+ * exponent). A logit of -inf is a masked token: its probability is 0, and so is its
+ * gradient, but for the target's and a filled teacher slot's, which keep what the formula
+ * leaves them (dlogprob; less a share). A row whose largest logit is not finite (nothing
+ * but -inf, a +inf, a NaN) has no distribution: its log probabilities, entropy, loss and
+ * gradients are NaN. An output that overlaps another buffer of
  * the call is MMH_ERR_ARGUMENT, except that dlogits may be logits. */
 
 /* Per row, each where it is wanted (else NULL): logprobs [n], the log probability

@@ -272,3 +272,26 @@ def test_losses_at_high_temperatures(ctx):
         d = np.abs(z - z.max(1, keepdims=True)).max() + 1.0
         assert abs(loss - row.mean()) <= t * t * (2 * (3 + 2 * d / t + 14) + 3) * R.U + 16 * R.U * row.mean()
         near(g, want, g_tol, "dlogits")
+
+
+@pytest.mark.parametrize("n,v", KERNELS)
+def test_masked_targets_and_slots_keep_their_share(ctx, n, v):
+    # a target of logit -inf: its log probability is -inf, its gradient dlogprob (less nothing), the others' as they are
+    z, y, r = drawn(n, v, v + 1)
+    z[np.arange(n), y] = -np.inf
+    lp, h, ids, top = run_logprobs(ctx, z, y, 2)
+    _, want_h, _ = R.token_logprobs(z, None, 2)
+    assert (lp == -np.inf).all()
+    near(h, *want_h, "entropy")
+    dl, dh = r.standard_normal(n).astype(np.float32), r.standard_normal(n).astype(np.float32)
+    g = run_logprobs_bwd(ctx, z, y, dl, dh)
+    near(g, *R.token_logprobs_backward(z, y, dl, dh), "dlogits")
+    assert (g[np.arange(n), y] == dl).all()
+    ids, teacher = y[:, None].copy(), np.zeros((n, 1), np.float32)
+    for temperature, alpha in ((1.0, 0.5), (2.0, 0.5), (2.0, 1.0)):
+        loss, g = run_distill(ctx, z, y, ids, teacher, temperature, alpha)
+        assert loss == np.inf
+        want = -(alpha * temperature + (1 - alpha)) / n
+        assert np.abs(g[np.arange(n), y] / want - 1).max() <= 8 * R.U
+        with np.errstate(invalid="ignore"):
+            near(g, *R.distillation(z, y, ids, teacher, temperature, alpha, n)[2:], "dlogits")
