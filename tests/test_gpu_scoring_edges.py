@@ -295,3 +295,28 @@ def test_masked_targets_and_slots_keep_their_share(ctx, n, v):
         assert np.abs(g[np.arange(n), y] / want - 1).max() <= 8 * R.U
         with np.errstate(invalid="ignore"):
             near(g, *R.distillation(z, y, ids, teacher, temperature, alpha, n)[2:], "dlogits")
+
+
+def test_many_ids_of_queued_calls_are_each_calls_own(ctx):
+    # behind work that takes a while, with ids of 16 MiB that change as soon as the call is back
+    a = ctx.empty((8192, 8192))
+    out = ctx.empty((8192, 8192))
+    n = 1 << 22
+    r = np.random.default_rng(41)
+    X, tables = ctx.to_device(r.standard_normal((1, 1, n, 2)).astype(np.float32)), mh.ScaledRotaryTables(ctx, 2, 1000)
+    Z = ctx.to_device(r.standard_normal((n, 2)).astype(np.float32))
+    cos, sin, x, z = tables.cos.numpy(), tables.sin.numpy(), X.numpy(), Z.numpy()
+    at, y = r.integers(0, 1000, (1, n)).astype(np.int32), r.integers(0, 2, n).astype(np.int32)
+    at0, y0 = at.copy(), y.copy()
+    for _ in range(4):
+        mh.gemm(ctx, "nn", a, a, out, 8192, 8192, 8192)
+    q = mh.rotary(ctx, X, None, tables, positions=at)[0]
+    at[:] = 0
+    for _ in range(4):
+        mh.gemm(ctx, "nn", a, a, out, 8192, 8192, 8192)
+    s = mh.token_logprobs(ctx, Z, y)
+    y[:] = 0
+    assert np.array_equal(q.numpy(), R.rotate(x, cos[at0][:, None], sin[at0][:, None], "half", 2))
+    d = z.astype(np.float64) - z.max(1, keepdims=True)
+    want = d[np.arange(n), y0] - np.log(np.exp(d).sum(1))
+    near(s.logprobs.numpy(), want, 64 * R.U * (1 + np.abs(want)), "logprobs")
