@@ -35,26 +35,27 @@ constexpr int64_t kMaxTop = 256;
 // its product with that 0 is one)
 constexpr float kFar = -200.0f;
 
-// log2 e / T in two floats of one sign, for exponentials of differences at temperature T.
+// A factor in two floats, both above 0.
 struct Rate {
     float hi, lo;
 };
-inline Rate rate_of(double t) {
-    const double k = 1.4426950408889634074 / t;
+inline Rate rate_of(double k) {
     float hi = (float)k;
     if ((double)hi > k) hi = std::nextafterf(hi, 0.0f);
-    return Rate{hi, (float)(k - (double)hi)};
+    return Rate{hi, std::max((float)(k - (double)hi), hi * 0x1p-60f)};
 }
-constexpr Rate kPlain{1.44269502f, 1.92596303e-8f};  // rate_of(1)
+// The product, rounded once. (An infinite d has its own sign in both.)
+__device__ __forceinline__ float times(float d, const Rate &k) { return __builtin_fmaf(d, k.hi, d * k.lo); }
+// log2 e / T, for exponentials of differences at temperature T = 1.
+constexpr double kLog2e = 1.4426950408889634074;
+constexpr Rate kPlain{1.44269502f, 1.92596303e-8f};  // rate_of(kLog2e)
 // exp(d / T), d <= 0, off by up to (2 + |d| / T) 2^-24 of itself, to both sides alike: the
 // exponent rounds once. (With one float for log2 e every term is too large by 0.22 |d|
 // 2^-24, and ln S of 32000 logits by 7e-8; both cost the same within 1%. Carrying the
 // exponent's rounding along as well would leave 2^-23 alone, beside the |d| / T 2^-24 of
 // d's own rounding: 4096 x 32000 with both terms 227 -> 257 us, log probabilities 109 ->
-// 114.) An infinite d has -inf from both products.
-__device__ __forceinline__ float exp_of(float d, const Rate &k) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.hi, d * k.lo));
-}
+// 114.)
+__device__ __forceinline__ float exp_of(float d, const Rate &k) { return __builtin_amdgcn_exp2f(times(d, k)); }
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -769,6 +770,7 @@ struct RowArgs {
     int k;
     float temperature, alpha, scale;  // scale: 1 / the rows that count
     Rate rate;                        // of the first exponential: at the temperature, or 1 (KIND_SCORES, alpha 0)
+    Rate inverse;                     // 1 / temperature
     float *row_loss;                  // [rows], 0 for a row that is left out
     int32_t *wrong;                   // receives 1 for a teacher's id beyond the vocabulary
     bool stream;
@@ -798,9 +800,10 @@ struct RowShared {
 // becomes soft q. Returns sum_j q_j (ln q_j - ln p_T(id_j)), `a` the S - 1 of p_T. Logits are
 // subtracted from logits and the logarithm taken of the two sums' quotient, by what it
 // differs from 1 where that is little: each ln q and ln p on its own is some 10, whose
-// rounding T^2 would make larger than a small term.
-__device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate &rate, float temperature, float soft, float m,
-                                               float a) {
+// rounding T^2 would make larger than a small term. log_hard: ln(1 + hard), formed beside
+// the others.
+__device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate &rate, const Rate &inverse, float soft, float m,
+                                               float a, float hard, float &log_hard) {
     const int lane = threadIdx.x & 63;
     float t[kMaxTop / 64], top = -INFINITY;
 #pragma unroll
@@ -820,15 +823,22 @@ __device__ __forceinline__ float teacher_terms(RowShared &sh, int k, const Rate 
         count += __popcll(__ballot(t[i] == 0.0f));
         some += t[i] == 0.0f ? 0.0f : e[i];
     }
-    const float rest = wave_sum(some) + (float)(count - 1), sum = 1.0f + rest, total = 1.0f + a, off = (rest - a) / total;
-    const float f = top == -INFINITY ? 0.0f : 1.0f / sum, log_ratio = fabsf(off) < 0.5f ? log1pf(off) : logf(sum / total);
+    // (a lane to each logarithm: one after another, 2048 rows of 4096 11 -> 12 us. Elsewhere the
+    // difference of two: logf of the quotient is off by half a step of f32 on average, 5e-8 of
+    // losses over 4096 rows.)
+    const float rest = wave_sum(some) + (float)(count - 1), off = (rest - a) / (1.0f + a);
+    const float log = log1pf(lane == 0 ? rest : lane == 1 ? a : lane == 2 ? off : hard);
+    auto log_of = [&](int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(log), i)); };
+    const float f = top == -INFINITY ? 0.0f : 1.0f / (1.0f + rest);
+    const float log_ratio = fabsf(off) < 0.5f ? log_of(2) : log_of(0) - log_of(1);
+    log_hard = log_of(3);
     float kl = 0.0f;
 #pragma unroll
     for (int i = 0; i < kMaxTop / 64; ++i) {
         const int j = lane + 64 * i;
         if (j >= k) break;
         const float q = e[i] * f;
-        if (q != 0.0f) kl += q * ((t[i] - (sh.z[j] - m)) / temperature - log_ratio);
+        if (q != 0.0f) kl += q * (times(t[i] - (sh.z[j] - m), inverse) - log_ratio);
         sh.weight[j] = soft * q;
     }
     return wave_sum(kl);
@@ -936,10 +946,10 @@ __device__ __forceinline__ Dense coefficients(const RowArgs &p, int64_t row, int
         const float other = KIND == KIND_BOTH ? rest1 : a;
         if (threadIdx.x == 0) sh.own = soft / total - hard * (other / (1.0f + other));
         if (threadIdx.x < 64) {
-            const float kl = teacher_terms(sh, k, p.rate, p.temperature, soft, s.m, a);
-            float loss = 0.0f;
+            float loss = 0.0f, log_hard;
+            const float kl = teacher_terms(sh, k, p.rate, p.inverse, soft, s.m, a, other, log_hard);
             if (p.alpha > 0.0f) loss = p.alpha * p.temperature * p.temperature * kl;
-            if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log1pf(other) - (sh.z[k] - s.m));
+            if (p.alpha < 1.0f) loss += (1.0f - p.alpha) * (log_hard - (sh.z[k] - s.m));
             // (without a distribution the loss is NaN, also where no term above has met it)
             if (a != a) loss = a;
             if (loss_too && threadIdx.x == 0) p.row_loss[row] = loss;
@@ -1289,7 +1299,8 @@ void distill(Context &cx, const Distill &d, float *dlogits, float *loss_host) {
     p.k = d.alpha > 0.0f ? (int)d.k : 0;  // (the teacher has no share at alpha 0)
     p.temperature = d.temperature;
     p.alpha = d.alpha;
-    p.rate = rate_of(d.alpha > 0.0f ? (double)d.temperature : 1.0);
+    p.rate = rate_of(kLog2e / (d.alpha > 0.0f ? (double)d.temperature : 1.0));
+    p.inverse = rate_of(1.0 / (double)d.temperature);
     p.scale = 1.0f / (float)std::max<int64_t>(1, kept);
     p.wrong = pinned;
     *pinned = 0;

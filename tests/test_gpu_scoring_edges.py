@@ -320,3 +320,16 @@ def test_many_ids_of_queued_calls_are_each_calls_own(ctx):
     d = z.astype(np.float64) - z.max(1, keepdims=True)
     want = d[np.arange(n), y0] - np.log(np.exp(d).sum(1))
     near(s.logprobs.numpy(), want, 64 * R.U * (1 + np.abs(want)), "logprobs")
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])
+def test_losses_of_many_rows_are_not_biased(ctx, temperature):
+    # Each of 4096 rows' terms (5 to 9, over T^2) rounds by half a step of 2^-20 at most, either way, as do its logarithms,
+    # so their mean is within 2 x 2.6e-8 as above, and the loss rounds once more.
+    n, v = 4096, 8000
+    z, y, r = drawn(n, v, 24)
+    d = (z.astype(np.float64) - z.max(1, keepdims=True)) / temperature
+    want = temperature ** 2 * np.log(np.exp(d).sum(1)).mean()
+    ids = z.argmax(1).astype(np.int32)[:, None].copy()
+    loss, _ = run_distill(ctx, z, None, ids, np.zeros((n, 1), np.float32), temperature, 1.0, grad=False)
+    assert abs(loss - want) <= np.spacing(np.float32(want)) / 2 + temperature ** 2 * 5.2e-8
