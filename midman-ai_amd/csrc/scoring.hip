@@ -53,8 +53,8 @@ constexpr Rate kPlain{1.44269502f, 1.92596303e-8f};  // rate_of(kLog2e)
 // exponent rounds once. (With one float for log2 e every term is too large by 0.22 |d|
 // 2^-24, and ln S of 32000 logits by 7e-8; both cost the same within 1%. Carrying the
 // exponent's rounding along as well would leave 2^-23 alone, beside the |d| / T 2^-24 of
-// d's own rounding: 4096 x 32000 with both terms 227 -> 257 us, log probabilities 109 ->
-// 114.)
+// d's own rounding, and take longer: 4096 x 32000 with both terms 228 -> 257 us, log
+// probabilities 109 -> 114.)
 __device__ __forceinline__ float exp_of(float d, const Rate &k) { return __builtin_amdgcn_exp2f(times(d, k)); }
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -295,9 +295,10 @@ __device__ __forceinline__ float ranked(float z) { return z != z ? INFINITY : z;
 // maxima is no larger than the k-th largest logit, and only what is above it (a little
 // more than k logits as a rule) goes to a list in LDS, where each entry's place is the
 // number of larger ones.
-// One read of the logits bounds it (4096 x 32000 without alternatives 93 us, 5.6 TB/s);
-// then the steps between barriers, of which two workgroups on a CU hide a part (k 16 102
-// us, 64 112, 128 130, 256 192; an argmax per alternative, as first built, k 64 7390).
+// One read of the logits bounds it (4096 x 32000 without targets and alternatives 86 us,
+// 6.1 TB/s); then the steps between barriers, of which two workgroups on a CU hide a part
+// (k 16 93 us, 64 105, 128 123, 256 187; an argmax per alternative, as first built, k 64
+// 7390).
 struct ScoreArgs {
     const float *logits;
     HostIds targets;
@@ -754,9 +755,9 @@ void scores(Context &cx, const ScoreArgs &all, int64_t n) {
 // KIND_BOTH with a second exponential at rate 1, less a weight at a few tokens: the
 // teacher's slots and the target. A row's logits stay in registers between the sums and
 // the gradient, so that the logits are read and the gradient written once, which bounds
-// it: 4096 x 32000 with both terms 205 us, 5.1 TB/s (a copy of as much 215), log
+// it: 4096 x 32000 with both terms 208 us, 5.0 TB/s (a copy of as much 215), log
 // probabilities' with a quarter of the rows left out 175, 5.2 TB/s; 817 rows of 131071 and 204
-// left out 207, 4.7 TB/s.
+// left out 212, 4.6 TB/s.
 struct RowArgs {
     const float *logits;
     HostIds targets;
@@ -1239,7 +1240,7 @@ void launch_parts(Context &cx, const RowArgs &all, int64_t n) {
 }
 
 // Rows by a workgroup each. A few wide ones, a quarter of the CUs at most, by their parts:
-// 64 rows of 131071 26 -> 19 us for log probabilities' gradients, one 21 -> 12, but 128 rows
+// 64 rows of 131071 26 -> 20 us for log probabilities' gradients, one 21 -> 11, but 128 rows
 // 29 -> 34; rows of up to kRowCols never (one of 32000 9 -> 12).
 // targets_host: of the n rows, where some may be left out.
 template <int KIND>
